@@ -562,6 +562,54 @@ int keep_vq_grouped_gemm_nested_q8(const void* x, int x_dtype, int64_t x_rows, c
 int keep_route_combine(const float* y, const float* w, int64_t T, int64_t k, int64_t H, void* out, int out_dtype,
                        void* stream);
 
+/* The same sum over rows of any float type: y [T k, H], out [T, H]; w NULL: weights of one (a token's rows added). */
+int keep_route_combine_rows(const void* y, int y_dtype, const float* w, int64_t T, int64_t k, int64_t H, void* out,
+                            int out_dtype, void* stream);
+
+/* The combine's gradients: dy[t, j] = w[t, j] dout[t] (dy [T k, H], y's dtype) and dw[t, j] = <y[t, j], dout[t]>
+ * (fp32 [T, k]). Either may be NULL; y may be NULL without dw. */
+int keep_route_combine_grad(const void* y, int y_dtype, const float* w, const void* dout, int dout_dtype, int64_t T,
+                            int64_t k, int64_t H, void* dy, float* dw, void* stream);
+
+/* Routed product with dense expert weights: out[r] = W[rhs[r]] x[row_r] with row_r = lhs[r], or r / x_div without lhs.
+ * x [x_rows, K] and weight of one dtype; weight [E, N, K], or with transposed [E, K, N]; out [routes, N]; fp32 sums. A
+ * route whose expert or row is out of range gives a NaN row.
+ * order / tile_expert / tile_offset / tile_count: a route plan's tiles (keep_route_plan) of tile = 16 routes, n_tiles of
+ * them (empty ones too); all NULL: routes are grouped in the kernel, in windows of 128 (for few routes, or any number
+ * of experts). */
+int keep_gather_mm(const void* x, int dtype, int64_t x_rows, const void* weight, int transposed, const int32_t* rhs,
+                   const int32_t* lhs, int64_t routes, int64_t x_div, int64_t num_experts, int64_t N, int64_t K,
+                   const int32_t* order, const int32_t* tile_expert, const int32_t* tile_offset,
+                   const int32_t* tile_count, int64_t n_tiles, void* out, int out_dtype, void* stream);
+
+/* Its weights' gradient: dw[e] = sum over the routes r of expert e of dy[r]^T x[r / x_div] ([E, N, K] of x's dtype, summed
+ * in fp32 in sorted order; zeros for experts without routes). dy [routes, N]; order, offsets and counts from
+ * keep_route_plan, whatever its tile. */
+int keep_gather_mm_grad_weight(const void* x, int dtype, int64_t x_rows, const void* dy, int64_t routes, int64_t x_div,
+                               int64_t num_experts, int64_t N, int64_t K, const int32_t* order, const int32_t* offsets,
+                               const int32_t* counts, void* dw, void* stream);
+
+/* Low-rank adapters of many requests: out[r] = base[r] + scales[a] (x[r / x_div] A[a]^T) B[a]^T with a = idx[r].
+ * x [x_rows, K], A [adapters, rank, K] and B [adapters, N, rank] of one dtype, rank in 1..128; scales fp32 [adapters]
+ * or NULL (ones); base [routes, N] or NULL (zeros). idx < 0: no adapter; idx >= adapters: a NaN row. order (or NULL): a
+ * permutation of the routes that brings those of one adapter together (keep_route_plan's). t_out (or NULL): the scaled
+ * low-rank rows, fp32 [routes, keep_lora_rank_stride(rank)], zeros without an adapter. The workspace holds
+ * keep_lora_workspace_bytes, 16-byte aligned. x = dy, A = B^T [adapters, rank, N], B = A^T [adapters, K, rank] gives the
+ * gradient of x. */
+int keep_lora(const void* x, int dtype, int64_t x_rows, const void* a, const void* b, const float* scales,
+              const int32_t* idx, const int32_t* order, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank,
+              int64_t K, int64_t N, const void* base, int base_dtype, float* t_out, void* workspace,
+              int64_t workspace_bytes, void* out, int out_dtype, void* stream);
+int64_t keep_lora_workspace_bytes(int dtype, int64_t routes, int64_t rank, int64_t K);
+int64_t keep_lora_rank_stride(int64_t rank);
+
+/* Gradient of one adapter factor: the sum over the routes r of each adapter of t[r]^T rows[r / x_div], [adapters, rank,
+ * dim], or with rank_inner [adapters, dim, rank]. t fp32 [routes, t_stride] (keep_lora's t_out; for A that of the call
+ * that gives the gradient of x); order, offsets and counts from keep_route_plan over idx. */
+int keep_lora_grad(const void* rows, int dtype, int64_t n_rows, int64_t x_div, int64_t dim, const float* t,
+                   int64_t t_stride, int64_t rank, int rank_inner, int64_t routes, int64_t adapters,
+                   const int32_t* order, const int32_t* offsets, const int32_t* counts, void* out, void* stream);
+
 /* Random-sign Walsh-Hadamard transform of T rows of n activations (16 <= n <= 8192,
  * a power of two): forward y = FWHT(x * signs) / sqrt(n), inverse (inverse != 0)
  * y = (FWHT(x) / sqrt(n)) * signs; signs = NULL applies the plain orthonormal FWHT.

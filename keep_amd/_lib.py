@@ -52,6 +52,18 @@ _SIGS = {
                              _P, _P, _P, _P, _P, _P, _P, c_int64, _P, c_int, _P],
     "keep_vq_grouped_gemm_q8_workspace_bytes": [c_int64, c_int64],
     "keep_route_combine": [_P, _P, c_int64, c_int64, c_int64, _P, c_int, _P],
+    "keep_route_combine_rows": [_P, c_int, _P, c_int64, c_int64, c_int64, _P, c_int, _P],
+    "keep_route_combine_grad": [_P, c_int, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, _P],
+    "keep_gather_mm": [_P, c_int, c_int64, _P, c_int, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P,
+                       _P, c_int64, _P, c_int, _P],
+    "keep_gather_mm_grad_weight": [_P, c_int, c_int64, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P, _P,
+                                   _P],
+    "keep_lora": [_P, c_int, c_int64, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P,
+                  c_int, _P, _P, c_int64, _P, c_int, _P],
+    "keep_lora_workspace_bytes": [c_int, c_int64, c_int64, c_int64],
+    "keep_lora_rank_stride": [c_int64],
+    "keep_lora_grad": [_P, c_int, c_int64, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int64, c_int64, _P, _P, _P,
+                       _P, _P],
     "keep_rht": [_P, c_int, _P, c_int, c_int64, c_int64, _P, c_int, _P],
     "keep_rmsnorm_quant_rht": [_P, c_int, c_int64, c_int64, _P, c_int, c_float, c_int64, c_int, _P, _P, _P, c_int, _P],
     "keep_moe_combine_add": [_P, _P, c_int, _P, c_int, c_int64, _P, c_int, _P],
@@ -108,7 +120,8 @@ _SIGS = {
 }
 _RESTYPE = {"keep_last_error": c_char_p, "keep_moe_tiles_workspace_bytes": c_int64,
             "keep_moe_layer1_workspace_bytes": c_int64,
-            "keep_vq_grouped_gemm_q8_workspace_bytes": c_int64}
+            "keep_vq_grouped_gemm_q8_workspace_bytes": c_int64,
+            "keep_lora_workspace_bytes": c_int64, "keep_lora_rank_stride": c_int64}
 EXPORTED = tuple(_SIGS)
 
 _lib = None

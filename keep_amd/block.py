@@ -68,9 +68,11 @@ def rmsnorm_quant_rht(x: torch.Tensor, gamma: torch.Tensor | None = None, eps: f
 
 def combine_add(routed: torch.Tensor, shared: torch.Tensor | None = None, residual: torch.Tensor | None = None,
                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``round_out(residual + (routed + shared))`` with fp32 sums; ``routed`` is float32."""
+    """``round_out(residual + (routed + shared))`` with fp32 sums; ``routed`` is float32. Differentiable: every
+    term's gradient is the output's, in its dtype."""
 
-    from keep_amd.ops import _DT, _stream
+    from keep_amd import _grad
+    from keep_amd.ops import _DT
 
     if routed.dtype != torch.float32 or not routed.is_cuda:
         raise ValueError("routed must be a float32 device tensor")
@@ -78,6 +80,15 @@ def combine_add(routed: torch.Tensor, shared: torch.Tensor | None = None, residu
         if t is not None and (tuple(t.shape) != tuple(routed.shape) or t.dtype not in _DT):
             raise ValueError(f"{name} must match routed's shape {tuple(routed.shape)} in a float dtype")
     od = out_dtype or (residual.dtype if residual is not None else torch.float32)
+    if _grad.wanted(routed, shared, residual):
+        held = _grad.check_capture(routed, shared, residual)  # noqa: F841
+        return _CombineAdd.apply(routed, shared, residual, od)
+    return _combine_add(routed, shared, residual, od)
+
+
+def _combine_add(routed, shared, residual, od: torch.dtype) -> torch.Tensor:
+    from keep_amd.ops import _DT, _stream
+
     r = routed.contiguous()
     sh = None if shared is None else shared.contiguous()
     rs = None if residual is None else residual.contiguous()
@@ -86,3 +97,15 @@ def combine_add(routed: torch.Tensor, shared: torch.Tensor | None = None, residu
               _DT[sh.dtype] if sh is not None else 0, None if rs is None else rs.data_ptr(),
               _DT[rs.dtype] if rs is not None else 0, r.numel(), out.data_ptr(), _DT[od], _stream(routed.device))
     return out
+
+
+class _CombineAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, routed, shared, residual, od):
+        ctx.dtypes = [None if t is None else t.dtype for t in (routed, shared, residual)]
+        return _combine_add(routed, shared, residual, od)
+
+    @staticmethod
+    def backward(ctx, dout):
+        return (*(None if dt is None or not need else dout.to(dt)
+                  for dt, need in zip(ctx.dtypes, ctx.needs_input_grad)), None)

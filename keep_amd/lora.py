@@ -1,0 +1,198 @@
+"""Low-rank adapters of many requests at once beside a shared projection.
+
+``gather_lora`` adds each row's own adapter to the projection's output,
+``out[r] = base[r] + s[a] (x[r] A[a]^T) B[a]^T`` with ``a = indices[r]`` (negative:
+no adapter; past the end: a NaN row), in two launches whatever the mix of
+requests (``keep_lora``). It is differentiable in ``x``, ``A``, ``B`` and
+``base``. ``LoraAdapters`` holds the adapters of a layer: a dense projection
+(``QuantizedVQLinear``) or routed experts, one adapter per expert
+(``SwitchLinear``, ``QuantizedVQSwitchLinear``). Adapters of a lower rank than
+the layer's are padded with zeros.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from keep_amd import _grad, _lib, ops
+from keep_amd.dense import _Plan
+
+MAX_RANK = 128
+# Routes (2D indices) from which a plan brings the routes of one adapter together first: rows of a request lie together
+# as they are, its routes' experts do not.
+PLANNED_ROUTES = 512
+
+
+def _launch(x, a, b, scales, idx, order, x_div: int, base, out, t_out) -> torch.Tensor:
+    n, rank, K = a.shape
+    R = idx.numel()
+    lib = _lib.load()
+    ws = torch.empty(lib.keep_lora_workspace_bytes(ops._DT[x.dtype], R, rank, K), dtype=torch.uint8, device=x.device)
+    _lib.call("keep_lora", x.data_ptr(), ops._DT[x.dtype], x.shape[0], a.data_ptr(), b.data_ptr(), ops._ptr(scales),
+              idx.data_ptr(), order, R, x_div, n, rank, K, b.shape[1], ops._ptr(base),
+              ops._DT[base.dtype] if base is not None else 0, ops._ptr(t_out), ws.data_ptr(), ws.numel(),
+              out.data_ptr(), ops._DT[out.dtype], ops._stream(x.device))
+    return out
+
+
+def _forward(x, a, b, scales, idx, x_div: int, base, out_dtype, t_out=None, plan=None):
+    R, N = idx.numel(), b.shape[1]
+    out = torch.empty((R, N), dtype=out_dtype, device=x.device)
+    if R == 0:
+        return out
+    if plan is None and idx.ndim == 2 and R >= PLANNED_ROUTES and a.shape[0] <= ops.PLAN_EXPERTS:
+        plan = _Plan(idx, a.shape[0], 16)
+    return _launch(x, a, b, scales, idx, plan and plan.order, x_div, base, out, t_out)
+
+
+class _GatherLora(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, a, b, base, scales, idx, x_div, out_dtype):
+        xc, ac, bc = x.contiguous(), a.contiguous(), b.contiguous()
+        R, rank = idx.numel(), a.shape[1]
+        # the scaled low-rank rows, for B's gradient
+        t = torch.empty((R, _lib.load().keep_lora_rank_stride(rank)), dtype=torch.float32, device=x.device)
+        plan = _Plan(idx, a.shape[0], 16) if R and a.shape[0] <= ops.PLAN_EXPERTS else None
+        out = _forward(xc, ac, bc, scales, idx, x_div, None if base is None else base.contiguous(), out_dtype, t,
+                       plan if idx.ndim == 2 else None)
+        ctx.save_for_backward(xc, ac, bc, scales, idx, t)
+        ctx.plan, ctx.x_div = plan, x_div
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, a, b, scales, idx, t = ctx.saved_tensors
+        nx, na, nb, nbase = ctx.needs_input_grad[:4]
+        with ops._on(x.device):
+            dx, da, db = _backward(x, a, b, scales, idx, t, ctx.plan, ctx.x_div, dy, nx, na, nb)
+        return dx, da, db, dy if nbase else None, None, None, None, None
+
+
+def _backward(x, a, b, scales, idx, t, plan, x_div: int, dy, nx: bool, na: bool, nb: bool):
+    (n, rank, K), N, R = a.shape, b.shape[1], idx.numel()
+    if R == 0:
+        return (torch.zeros_like(x) if nx else None, torch.zeros_like(a) if na else None,
+                torch.zeros_like(b) if nb else None)
+    g = dy.to(x.dtype).contiguous()  # a float32 output over 16-bit rows: its gradient enters the products in 16 bits
+    dx = da = db = None
+    if nx or na:  # dt = s dy B, dx = dt A: the same two products on the transposed factors
+        dt = torch.empty_like(t)
+        k = x_div
+        rows = torch.empty((R, K), dtype=x.dtype if k == 1 else torch.float32, device=x.device)
+        _launch(g, b.transpose(1, 2).contiguous(), a.transpose(1, 2).contiguous(), scales, idx,
+                plan.order if plan is not None and idx.ndim == 2 else None, 1, None, rows, dt)
+        if nx:
+            dx = rows if k == 1 else ops._sum_routes(rows, k, x.dtype)
+        if na:
+            da = torch.empty_like(a)
+            _lib.call("keep_lora_grad", x.data_ptr(), ops._DT[x.dtype], x.shape[0], x_div, K, dt.data_ptr(),
+                      dt.shape[1], rank, 0, R, n, plan.order, plan.offsets, plan.counts, da.data_ptr(),
+                      ops._stream(x.device))
+    if nb:
+        db = torch.empty_like(b)
+        _lib.call("keep_lora_grad", g.data_ptr(), ops._DT[g.dtype], R, 1, N, t.data_ptr(), t.shape[1], rank, 1, R, n,
+                  plan.order, plan.offsets, plan.counts, db.data_ptr(), ops._stream(x.device))
+    return dx, da, db
+
+
+def gather_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, indices, *,
+                base: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                validate_indices: bool = False) -> torch.Tensor:
+    """Each row's own low-rank adapter: ``x [T, K]``, ``lora_a [n, r, K]``, ``lora_b [n, N, r]`` (``r <= 128``).
+
+    ``indices [T]`` -> ``[T, N]``; ``indices [T, k]`` (an adapter per route of a token) -> ``[T, k, N]``. ``base`` (of
+    the output's shape) is added, in float32 with one rounding; the output has its dtype, without it ``x``'s. ``scales``
+    (``[n]``, kept in float32) multiplies each adapter and takes no gradient. Gradients of the factors need
+    ``n <= 1024``. In 16 bits the low-rank row enters the second product in ``x``'s dtype.
+    """
+
+    device = ops._dense_device(x, lora_a, lora_b, base)
+    if x.ndim != 2:
+        raise ValueError(f"x must be 2D [tokens, hidden], found {tuple(x.shape)}")
+    if lora_a.ndim != 3 or lora_b.ndim != 3 or 0 in lora_a.shape or 0 in lora_b.shape:
+        raise ValueError(f"lora_a and lora_b must be [adapters, rank, in] and [adapters, out, rank], found "
+                         f"{tuple(lora_a.shape)} and {tuple(lora_b.shape)}")
+    n, rank, K = lora_a.shape
+    N = lora_b.shape[1]
+    if lora_b.shape[0] != n or lora_b.shape[2] != rank:
+        raise ValueError(f"lora_b must be [{n}, out, {rank}], found {tuple(lora_b.shape)}")
+    if rank > MAX_RANK:
+        raise ValueError(f"the rank must be at most {MAX_RANK}, found {rank}")
+    if x.dtype not in ops._DT or lora_a.dtype != x.dtype or lora_b.dtype != x.dtype:
+        raise ValueError("x, lora_a and lora_b must share a dtype of float32, float16 or bfloat16, found "
+                         f"{x.dtype}, {lora_a.dtype} and {lora_b.dtype}")
+    if x.shape[1] != K:
+        raise ValueError(f"x trailing dimension must be {K}, found {x.shape[1]}")
+    idx = ops._index_tensor(indices, device)
+    if idx.ndim not in (1, 2) or idx.shape[0] != x.shape[0]:
+        raise ValueError(f"indices must be [{x.shape[0]}] or [{x.shape[0]}, top_k], found {tuple(idx.shape)}")
+    x_div = idx.shape[1] if idx.ndim == 2 else 1
+    shape = (*idx.shape, N)
+    if base is not None and (tuple(base.shape) != shape or base.dtype not in ops._DT):
+        raise ValueError(f"base must have shape {shape} in float32, float16 or bfloat16, found {tuple(base.shape)} "
+                         f"in {base.dtype}")
+    if scales is not None:
+        if torch.is_grad_enabled() and scales.requires_grad:
+            raise ValueError("scales take no gradient")
+        if tuple(scales.shape) != (n,):
+            raise ValueError(f"scales must have shape ({n},), found {tuple(scales.shape)}")
+        scales = ops._to_dev(scales.detach(), device, torch.float32)
+    if validate_indices and idx.numel() and int(idx.max()) >= n:
+        raise ValueError(f"indices must be below {n}, found {int(idx.max())}")
+    od = x.dtype if base is None else base.dtype
+    with ops._on(device):
+        if not _grad.wanted(x, lora_a, lora_b, base):
+            return _forward(x.detach().contiguous(), lora_a.detach().contiguous(), lora_b.detach().contiguous(), scales,
+                            idx, max(x_div, 1), None if base is None else base.detach().contiguous(), od).view(shape)
+        if (lora_a.requires_grad or lora_b.requires_grad) and n > ops.PLAN_EXPERTS:
+            raise ValueError(f"gradients of the factors need at most {ops.PLAN_EXPERTS} adapters, found {n}")
+        held = _grad.check_capture(x, lora_a, lora_b, base)  # noqa: F841
+        flat = None if base is None else base.reshape(-1, N)
+        return _GatherLora.apply(x, lora_a, lora_b, flat, scales, idx, max(x_div, 1), od).view(shape)
+
+
+class LoraAdapters:
+    """The adapters of one layer, a row of factors per adapter: ``a [n, r, K]``, ``b [n, N, r]`` for a dense
+    projection; ``a [n, E, r, K]``, ``b [n, E, N, r]`` for routed experts. ``scales [n]`` (e.g. alpha / r)."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor | None = None):
+        if a.ndim not in (3, 4) or b.ndim != a.ndim or a.shape[:-2] != b.shape[:-2] or a.shape[-2] != b.shape[-1]:
+            raise ValueError("adapters must be a [n, r, K] and b [n, N, r], or with experts a [n, E, r, K] and "
+                             f"b [n, E, N, r], found {tuple(a.shape)} and {tuple(b.shape)}")
+        if not 1 <= a.shape[-2] <= MAX_RANK:
+            raise ValueError(f"the rank must be in 1..{MAX_RANK}, found {a.shape[-2]}")
+        if scales is not None and tuple(scales.shape) != (a.shape[0],):
+            raise ValueError(f"scales must have shape ({a.shape[0]},), found {tuple(scales.shape)}")
+        self.a, self.b, self.scales = a, b, scales
+        self.num_adapters, self.rank = a.shape[0], a.shape[-2]
+        self.num_experts = a.shape[1] if a.ndim == 4 else None
+        self.input_dims, self.output_dims = a.shape[-1], b.shape[-2]
+        # a scale per (adapter, expert), laid out once
+        self._scales = scales if scales is None or a.ndim == 3 else scales.detach().repeat_interleave(a.shape[1])
+
+    def check(self, layer) -> None:
+        experts = getattr(layer, "num_experts", None)
+        if self.num_experts != experts:
+            raise ValueError("a dense projection takes adapters a [n, r, K]" if experts is None else
+                             f"routed experts take adapters a [n, {experts}, r, K]")
+        if self.input_dims != layer.input_dims or self.output_dims != layer.output_dims:
+            raise ValueError(f"adapters map {self.input_dims} -> {self.output_dims}, the layer "
+                             f"{layer.input_dims} -> {layer.output_dims}")
+
+    def add(self, base: torch.Tensor, x: torch.Tensor, adapter_indices, experts: torch.Tensor | None = None):
+        """``base`` plus the adapters of ``x``'s rows: ``x [T, K]``, ``adapter_indices [T]``; with ``experts [T, k]``
+        the adapters of every route."""
+
+        idx = ops._index_tensor(adapter_indices, x.device)
+        if tuple(idx.shape) != (x.shape[0],):
+            raise ValueError(f"adapter_indices must hold one adapter per row ({x.shape[0]}), found {tuple(idx.shape)}")
+        if experts is None:
+            return gather_lora(x, self.a, self.b, idx, base=base, scales=self._scales)
+        E = self.num_experts
+        e = ops._index_tensor(experts, x.device)
+        # a route without an expert has a NaN base row already
+        none = (idx < 0)[:, None] | (e < 0) | (e >= E)
+        flat = torch.where(none, -1, idx.clamp(max=self.num_adapters)[:, None] * E + e)
+        return gather_lora(x, self.a.flatten(0, 1), self.b.flatten(0, 1), flat, base=base, scales=self._scales)

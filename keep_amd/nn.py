@@ -9,6 +9,8 @@
   ``src/ramp/models/glm4_moe_adapter.py:113-390``: few-token calls run the
   decode mat-vec per projection, prefill runs one device route plan shared by
   the three MFMA grouped GEMMs (``_shared_sorted_route_prefill``).
+- ``SwitchLinear`` -- the same stacked projection on dense weights, for experts
+  that stay unquantised; differentiable.
 - ``LimitedSwiGLU`` -- ``deepseek_v4_flash_adapter.py:962-986``.
 - ``RoutedVQMoE`` -- router + experts + weighted combine
   (``DeepseekV4FlashVQMoE.__call__``, ``deepseek_v4_flash_adapter.py:1776-1784``),
@@ -23,6 +25,8 @@ import numpy as np
 import torch
 
 from keep_amd import _lib, ops
+from keep_amd.dense import gather_mm
+from keep_amd.lora import LoraAdapters
 from keep_amd.router import RouterOutput, _slot_args, router_dual_topk
 
 CODEWORD_DIM = 8
@@ -46,14 +50,25 @@ class LimitedSwiGLU:
         return (torch.nn.functional.silu(g) * u).to(dtype)
 
 
+def _check_adapters(layer, x: torch.Tensor, *, frozen: bool) -> None:
+    """What a call with adapter indices needs; ``frozen``: a layer on codes, whose product has no gradient."""
+
+    if layer.adapters is None:
+        raise ValueError("adapter_indices need a layer with adapters")
+    if frozen and torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("a product with codes has no gradient: the layer's input must not require one")
+
+
 class QuantizedVQLinear:
     """Dense linear layer on E8 VQ codes (torch, GPU): ``vq_qmv`` for one row,
     ``vq_qmm`` for more, after the optional RHT or input rotation, plus bias
     (reference ``src/ramp/nn/linear.py:17-121``). ``x @ rotation_matrix`` runs
-    in ``x``'s dtype, as ``apply_rotation_mx`` does (``keep/quant/rotation.py:39-43``)."""
+    in ``x``'s dtype, as ``apply_rotation_mx`` does (``keep/quant/rotation.py:39-43``). ``adapters`` with
+    ``adapter_indices`` (one per row, -1: none) adds each row's low-rank adapter of the untransformed input."""
 
     def __init__(self, *, input_dims: int, output_dims: int, codes, scales, codebook=None, bias=None,
-                 group_size: int = 512, code_bits: int = 8, rht_signs=None, rotation_matrix=None):
+                 group_size: int = 512, code_bits: int = 8, rht_signs=None, rotation_matrix=None,
+                 adapters: LoraAdapters | None = None):
         if input_dims <= 0 or output_dims <= 0:
             raise ValueError("input_dims and output_dims must be positive")
         if input_dims % CODEWORD_DIM != 0:
@@ -90,10 +105,16 @@ class QuantizedVQLinear:
             check_signs(self.rht_signs)
         self.rotation_matrix = None if rotation_matrix is None else ops._to_dev(rotation_matrix, device,
                                                                                 torch.float32)
+        self.adapters = adapters
+        if adapters is not None:
+            adapters.check(self)
 
-    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+    def __call__(self, x: torch.Tensor, adapter_indices=None) -> torch.Tensor:
         if x.shape[-1] != self.input_dims:
             raise ValueError(f"input trailing dimension must be {self.input_dims}, found {x.shape[-1]}")
+        if adapter_indices is not None:
+            _check_adapters(self, x, frozen=True)
+        rows = x
         if self.rht_signs is not None:
             from keep_amd.rht import apply_rht
             x = apply_rht(x, self.rht_signs, validate_signs=False)  # checked once, at construction
@@ -108,6 +129,9 @@ class QuantizedVQLinear:
         y = y.reshape(x.shape[:-1] + (self.output_dims,))
         if self.bias is not None:
             y = y + self.bias  # type promotion as MLX's: a float32 bias gives a float32 result
+        if adapter_indices is not None:  # of the layer's input as it came: no transform
+            y = self.adapters.add(y.reshape(-1, self.output_dims), rows.reshape(-1, self.input_dims),
+                                  ops._index_tensor(adapter_indices, x.device).reshape(-1)).reshape(y.shape)
         return y
 
     def _extra_repr(self) -> str:
@@ -146,7 +170,8 @@ class QuantizedVQSwitchLinear:
                  scales: torch.Tensor, codebook: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                  group_size: int = 512, code_bits: int = 8, use_gather_vqmm: bool = True,
                  route_strategy: str = "auto", gather_codebook_duplication: int = 8,
-                 rht_signs: torch.Tensor | None = None, rotation_matrix: torch.Tensor | None = None, **sidecars):
+                 rht_signs: torch.Tensor | None = None, rotation_matrix: torch.Tensor | None = None,
+                 adapters: LoraAdapters | None = None, **sidecars):
         if input_dims <= 0 or output_dims <= 0 or num_experts <= 0:
             raise ValueError("input_dims, output_dims, and num_experts must be positive")
         if input_dims % CODEWORD_DIM != 0:
@@ -192,6 +217,9 @@ class QuantizedVQSwitchLinear:
             check_signs(self.rht_signs)
         self.rotation_matrix = None if rotation_matrix is None else ops._to_dev(rotation_matrix, device,
                                                                                 torch.float32)
+        self.adapters = adapters
+        if adapters is not None:
+            adapters.check(self)
 
     @classmethod
     def from_weights(cls, weight, bias=None, *, group_size: int = 512, code_bits: int = 8,
@@ -242,8 +270,11 @@ class QuantizedVQSwitchLinear:
         from keep_amd.rht import apply_rht
         return apply_rht(x, self.rht_signs, validate_signs=False)  # checked once, at construction
 
-    def __call__(self, x: torch.Tensor, indices: torch.Tensor, *, sorted_indices: bool = False) -> torch.Tensor:
-        x = self._rht(x)
+    def __call__(self, x: torch.Tensor, indices: torch.Tensor, *, sorted_indices: bool = False,
+                 adapter_indices=None) -> torch.Tensor:
+        if adapter_indices is not None:
+            _check_adapters(self, x, frozen=True)
+        rows, x = x, self._rht(x)
         kw = dict(input_dims=self.input_dims, output_dims=self.output_dims, group_size=self.group_size,
                   code_bits=self.code_bits, route_strategy=self.route_strategy, sorted_indices=sorted_indices,
                   codebook_duplication=self.gather_codebook_duplication)
@@ -263,7 +294,62 @@ class QuantizedVQSwitchLinear:
                              "the per-route layout")
         if self.bias is not None:
             y = y + self.bias[indices.long()].to(y.dtype)
-        return y
+        return y if adapter_indices is None else _add_adapters(self, y, rows, indices, adapter_indices)
+
+
+def _add_adapters(layer, y: torch.Tensor, x: torch.Tensor, indices: torch.Tensor, adapter_indices) -> torch.Tensor:
+    """The adapters of every route: ``x`` in the token or per-route layout (then one adapter index per route)."""
+
+    experts = indices.reshape(-1, indices.shape[-1] if y.ndim == x.ndim + 1 else 1)
+    rows = x.reshape(-1, layer.input_dims)
+    base = y.reshape(*experts.shape, layer.output_dims)
+    ad = ops._index_tensor(adapter_indices, x.device).reshape(-1)
+    return layer.adapters.add(base, rows, ad, experts).reshape(y.shape)
+
+
+class SwitchLinear:
+    """Switch-linear layer on dense expert weights ``[E, out, in]`` (torch, GPU): ``QuantizedVQSwitchLinear`` for
+    experts that stay unquantised, in the same places (``QuantizedVQSwitchGLU``, ``RoutedVQMoE``). ``gather_mm`` in the
+    weights' dtype, differentiable in ``x``, ``weight``, ``bias`` and the adapters. Weights stay as they are given (a
+    tensor that requires a gradient gets it)."""
+
+    code_bits = None  # no codes: the fused VQ paths do not take it
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                 adapters: LoraAdapters | None = None):
+        if weight.ndim != 3 or 0 in weight.shape:
+            raise ValueError(f"weight must be 3D [experts, out, in], none of them 0, found {tuple(weight.shape)}")
+        if weight.dtype not in ops._DT:
+            raise ValueError(f"weight must be float32, float16 or bfloat16, found {weight.dtype}")
+        self.num_experts, self.output_dims, self.input_dims = weight.shape
+        if bias is not None and tuple(bias.shape) != (self.num_experts, self.output_dims):
+            raise ValueError(f"bias must have shape ({self.num_experts}, {self.output_dims}), found "
+                             f"{tuple(bias.shape)}")
+        self.weight, self.bias = weight, bias
+        self.rht_signs = self.rotation_matrix = None
+        self.adapters = adapters
+        if adapters is not None:
+            adapters.check(self)
+
+    def __call__(self, x: torch.Tensor, indices: torch.Tensor, *, sorted_indices: bool = False,
+                 adapter_indices=None) -> torch.Tensor:
+        if adapter_indices is not None:
+            _check_adapters(self, x, frozen=False)
+        if x.shape[-1] != self.input_dims:
+            raise ValueError(f"x trailing dimension must be {self.input_dims}, found {x.shape[-1]}")
+        lead = tuple(x.shape[:-1])
+        rows = x.reshape(-1, self.input_dims).to(self.weight.dtype)
+        if x.ndim >= 2 and indices.ndim >= 2 and lead == tuple(indices.shape[:-1]):
+            y = gather_mm(rows, self.weight, indices.reshape(-1, indices.shape[-1]))
+            y = y.reshape(tuple(indices.shape) + (self.output_dims,))
+        elif x.ndim >= 2 and lead == tuple(indices.shape):
+            y = gather_mm(rows, self.weight, indices.reshape(-1, 1)).reshape(lead + (self.output_dims,))
+        else:
+            raise ValueError(f"x {tuple(x.shape)} and indices {tuple(indices.shape)} match neither the token nor "
+                             "the per-route layout")
+        if self.bias is not None:
+            y = y + self.bias[indices.long().clamp(0, self.num_experts - 1)].to(y.dtype)  # (routes out of range: NaN)
+        return y if adapter_indices is None else _add_adapters(self, y, rows.view(x.shape), indices, adapter_indices)
 
 
 class HotTier:
@@ -393,6 +479,8 @@ class QuantizedVQSwitchGLU:
         self.hidden_dims = gate_proj.output_dims
         self.num_experts = gate_proj.num_experts
         if hot_tier is not None:
+            if any(isinstance(p, SwitchLinear) for p in (gate_proj, up_proj, down_proj)):
+                raise ValueError("a hot tier adds to codes: it takes no dense projection")
             hot_tier.check(self)
         self.hot_tier = hot_tier
 
@@ -532,7 +620,10 @@ class QuantizedVQSwitchGLU:
         y = nested(h, d, "down", 1)
         return y.reshape(lead + (k, d.output_dims))
 
-    def __call__(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
+    def __call__(self, x: torch.Tensor, indices: torch.Tensor, adapter_indices=None) -> torch.Tensor:
+        projections = (self.gate_proj, self.up_proj, self.down_proj)
+        if adapter_indices is not None or any(isinstance(p, SwitchLinear) for p in projections):
+            return self._by_projection(x, indices, adapter_indices)
         if self._can_use_shared_sorted_route_prefill(x, indices):
             return self._shared_sorted_route_prefill(x, indices)
         if self.hot_tier is not None:
@@ -540,6 +631,29 @@ class QuantizedVQSwitchGLU:
         gate = self.gate_proj(x, indices)
         up = self.up_proj(x, indices)
         return self.down_proj(self._apply_activation(up, gate), indices)
+
+    def _by_projection(self, x: torch.Tensor, indices: torch.Tensor, adapter_indices) -> torch.Tensor:
+        """Dense projections and projections with adapters, one after the other. ``adapter_indices`` holds one
+        adapter per token; projections without adapters leave it out."""
+
+        if self.hot_tier is not None:
+            raise ValueError("adapters and the hot tier do not combine")
+        if adapter_indices is not None and all(p.adapters is None
+                                               for p in (self.gate_proj, self.up_proj, self.down_proj)):
+            raise ValueError("adapter_indices need a projection with adapters")
+
+        def project(p, rows, ad):
+            if torch.is_grad_enabled() and rows.requires_grad and not isinstance(p, SwitchLinear):
+                raise ValueError("a product with codes has no gradient: its input must not require one")
+            return p(rows, indices, adapter_indices=ad if p.adapters is not None else None)
+
+        gate = project(self.gate_proj, x, adapter_indices)
+        up = project(self.up_proj, x, adapter_indices)
+        per_route = None
+        if adapter_indices is not None:  # down's rows are the routes
+            ad = ops._index_tensor(adapter_indices, x.device).reshape(tuple(x.shape[:-1]))
+            per_route = ad[..., None].expand(indices.shape) if indices.ndim == x.ndim else ad
+        return project(self.down_proj, self._apply_activation(up, gate), per_route)
 
 
 def moe_decode(x: torch.Tensor, idx: torch.Tensor, weight: torch.Tensor, gate, up, down, *, limit: float = 0.0,
@@ -914,6 +1028,10 @@ class RoutedVQMoE:
     faster, but it assumes all 256 of its blocks are resident together, so a
     caller sharing the GPU with other work checks ``layer_status`` for a wait
     that gave up (NaN output).
+
+    ``glu`` may hold dense projections (``SwitchLinear``): the layer is then differentiable in ``x``, the experts'
+    weights, the shared expert's and ``residual`` (the router's outputs take no gradient). ``adapter_indices`` (one
+    per token, -1: none) adds the adapters of the projections that have some.
     """
 
     def __init__(self, glu: QuantizedVQSwitchGLU, *, top_k: int, score_func: str = "softmax",
@@ -955,10 +1073,12 @@ class RoutedVQMoE:
         return se(x, idx).reshape(T, -1).float()
 
     def experts(self, x: torch.Tensor, idx: torch.Tensor, weight: torch.Tensor, *,
-                out_dtype: torch.dtype | None = None) -> torch.Tensor:
+                out_dtype: torch.dtype | None = None, adapter_indices=None) -> torch.Tensor:
         g, u, d = self.glu.gate_proj, self.glu.up_proj, self.glu.down_proj
         od = out_dtype or self.out_dtype
         T = x.shape[0]
+        if adapter_indices is not None:
+            return ops.route_combine(self.glu(x, idx, adapter_indices), weight, od)
         if (T <= self.decode_max_tokens and self.glu._all_e8p() and self.glu.hot_tier is None
                 and x.dtype in (torch.float16, torch.bfloat16)):
             return moe_decode(x, idx, weight, (g.codes, g.scales), (u.codes, u.scales), (d.codes, d.scales),
@@ -989,16 +1109,17 @@ class RoutedVQMoE:
             return None  # fewer logits than pool rows: routed apart
         return None if entry is None else entry + "_layer"
 
-    def __call__(self, x: torch.Tensor, logits: torch.Tensor, *, residual: torch.Tensor | None = None):
+    def __call__(self, x: torch.Tensor, logits: torch.Tensor, *, residual: torch.Tensor | None = None,
+                 adapter_indices=None):
         extra = self.shared_experts is not None or residual is not None
         od = torch.float32 if extra else self.out_dtype
-        entry = self._tiles_layer_path(x, logits)
+        entry = self._tiles_layer_path(x, logits) if adapter_indices is None else None
         if entry is not None:
             g, u, d = self.glu.gate_proj, self.glu.up_proj, self.glu.down_proj
             out, r = _tiles_layer(entry, x, logits, (g.codes, g.scales), (u.codes, u.scales), (d.codes, d.scales),
                                   self.top_k, self.bias_served, self.bias_demand, self.score_func, self.renormalize,
                                   self.route_scale, self.tau, self.limit, g.codebook, od, self.slot_map)
-        elif self._layer_path(x):
+        elif adapter_indices is None and self._layer_path(x):
             g, u, d = self.glu.gate_proj, self.glu.up_proj, self.glu.down_proj
             one = self.one_launch and _one_launch_ok(x.device, logits.shape[-1], g.input_dims, g.output_dims,
                                                      self.top_k)
@@ -1012,7 +1133,7 @@ class RoutedVQMoE:
                                  score_func=self.score_func, renormalize=self.renormalize,
                                  route_scale=self.route_scale, tau=self.tau, slot_map=self.slot_map,
                                  num_slots=self.glu.num_experts)
-            out = self.experts(x, r.idx, r.weight, out_dtype=od)
+            out = self.experts(x, r.idx, r.weight, out_dtype=od, adapter_indices=adapter_indices)
         if not extra:
             return out, r
         from keep_amd.block import combine_add

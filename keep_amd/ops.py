@@ -24,15 +24,16 @@ tensors on a ROCm device instead of ``mx.array``. Differences, each deliberate:
 from __future__ import annotations
 
 import weakref
-from contextlib import contextmanager
+from contextlib import contextmanager, nullcontext
 from contextvars import ContextVar
 from functools import lru_cache
 from typing import Any, Iterator, Literal
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
-from keep_amd import _lib
+from keep_amd import _grad, _lib
 
 CODEWORD_DIM = 8
 NO_RESIDUAL = 0xFFFFFFFF
@@ -353,6 +354,30 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+def _dense_device(*ts: torch.Tensor | None) -> torch.device:
+    """The one GPU that every tensor is on."""
+
+    device = None
+    for t in ts:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise ValueError(f"Expected a cuda device, but got: {t.device if isinstance(t, torch.Tensor) else type(t)}")
+        if device is not None and t.device != device:
+            raise ValueError(f"tensors must be on one device, found {device} and {t.device}")
+        device = t.device
+    return device
+
+
+_HERE = nullcontext()
+
+
+def _on(device: torch.device):
+    """The context in which launches for ``device``'s tensors are made (none where it is the current device)."""
+
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 # --------------------------------------------------------------------------- raw launchers
 
 
@@ -640,19 +665,73 @@ def grouped_gemm_nested(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     return out
 
 
+class _RouteCombine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weight, od):
+        yc, wc = y.contiguous(), weight.float().contiguous()
+        ctx.save_for_backward(yc, wc)
+        ctx.weight_dtype = weight.dtype
+        return _combine_rows(yc, wc, od)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        y, w = ctx.saved_tensors
+        T, k, H = y.shape
+        d = dout.contiguous()
+        dy = torch.empty_like(y) if ctx.needs_input_grad[0] else None
+        dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
+        if y.numel():
+            with _on(y.device):
+                _lib.call("keep_route_combine_grad", y.data_ptr(), _DT[y.dtype], w.data_ptr(), d.data_ptr(),
+                          _DT[d.dtype], T, k, H, _ptr(dy), _ptr(dw), _stream(y.device))
+        elif dw is not None:
+            dw.zero_()
+        return dy, None if dw is None else dw.to(ctx.weight_dtype), None
+
+
+def _combine_rows(y: torch.Tensor, w: torch.Tensor | None, od: torch.dtype) -> torch.Tensor:
+    T, k, H = y.shape
+    out = torch.empty((T, H), dtype=od, device=y.device)
+    if T and not (k and H):
+        return out.zero_()
+    if y.dtype == torch.float32 and w is not None and H % 4 == 0:
+        _lib.call("keep_route_combine", y.data_ptr(), w.data_ptr(), T, k, H, out.data_ptr(), _DT[od],
+                  _stream(y.device))
+    else:
+        _lib.call("keep_route_combine_rows", y.data_ptr(), _DT[y.dtype], _ptr(w), T, k, H, out.data_ptr(), _DT[od],
+                  _stream(y.device))
+    return out
+
+
+def _sum_routes(rows: torch.Tensor, k: int, od: torch.dtype) -> torch.Tensor:
+    """``rows [T k, H]`` added per token, in float32 and in order."""
+
+    return _combine_rows(rows.view(-1, k, rows.shape[1]), None, od)
+
+
 def route_combine(y: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``keep_route_combine``: ``sum_j w[t, j] * y[t, j, :]`` in fp32 for
-    ``y [T, k, H]`` (``glm4_moe_adapter.py:367-372``)."""
+    """``sum_j w[t, j] * y[t, j, :]`` in fp32 for ``y [T, k, H]`` of any float dtype
+    (``glm4_moe_adapter.py:367-372``), differentiable in ``y`` and ``weight``:
+    ``dy[t, j] = w[t, j] dout[t]``, ``dw[t, j] = <y[t, j], dout[t]>``."""
 
     T, k, H = y.shape
     od = out_dtype or torch.float32
-    yf = y.float().contiguous()
-    wf = weight.reshape(T, k).float().contiguous()
     if H % 4:
         raise ValueError(f"route_combine needs H a multiple of 4, found {H}")
-    out = torch.empty((T, H), dtype=od, device=y.device)
-    _lib.call("keep_route_combine", yf.data_ptr(), wf.data_ptr(), T, k, H, out.data_ptr(), _DT[od], _stream(y.device))
-    return out
+    if y.dtype not in _DT:
+        y = y.float()
+    if weight.device != y.device:
+        raise ValueError(f"tensors must be on one device, found {y.device} and {weight.device}")
+    weight = weight.reshape(T, k)
+    if _grad.wanted(y, weight):
+        _dense_device(y)
+        if od not in _DT:
+            raise ValueError(f"unsupported output dtype {od}")
+        held = _grad.check_capture(y, weight)  # noqa: F841
+        with _on(y.device):
+            return _RouteCombine.apply(y, weight, od)
+    return _combine_rows(y.contiguous(), weight.float().contiguous(), od)
 
 
 def gemm_eligible(*, code_bits: int, x_dtype: torch.dtype, input_dims: int, group_size: int) -> bool:
