@@ -574,13 +574,16 @@ int keep_route_combine_grad(const void* y, int y_dtype, const float* w, const vo
 /* Routed product with dense expert weights: out[r] = W[rhs[r]] x[row_r] with row_r = lhs[r], or r / x_div without lhs.
  * x [x_rows, K] and weight of one dtype; weight [E, N, K], or with transposed [E, K, N]; out [routes, N]; fp32 sums. A
  * route whose expert or row is out of range gives a NaN row.
- * order / tile_expert / tile_offset / tile_count: a route plan's tiles (keep_route_plan) of tile = 16 routes, n_tiles of
- * them (empty ones too); all NULL: routes are grouped in the kernel, in windows of 128 (for few routes, or any number
- * of experts). */
+ * order .. valid_tiles: a route plan's arrays (keep_route_plan; valid_tiles is its n_tiles), n_tiles the descriptors to
+ * look at (empty ones too) and tile its tile, one keep_gather_mm_tile_supported takes: 16 any sizes and types; 64, 128 and
+ * 256 (the large products, through LDS) fp16 and bf16 rows of whole 16-byte pieces at aligned addresses. All NULL: routes
+ * are grouped in the kernel, in windows of 128 (for few routes, or any number of experts). */
 int keep_gather_mm(const void* x, int dtype, int64_t x_rows, const void* weight, int transposed, const int32_t* rhs,
                    const int32_t* lhs, int64_t routes, int64_t x_div, int64_t num_experts, int64_t N, int64_t K,
-                   const int32_t* order, const int32_t* tile_expert, const int32_t* tile_offset,
-                   const int32_t* tile_count, int64_t n_tiles, void* out, int out_dtype, void* stream);
+                   const int32_t* order, const int32_t* offsets, const int32_t* counts, const int32_t* tile_expert,
+                   const int32_t* tile_offset, const int32_t* tile_count, const int32_t* valid_tiles, int64_t n_tiles,
+                   int64_t tile, void* out, int out_dtype, void* stream);
+int keep_gather_mm_tile_supported(int dtype, int transposed, int64_t N, int64_t K, int64_t tile);
 
 /* Its weights' gradient: dw[e] = sum over the routes r of expert e of dy[r]^T x[r / x_div] ([E, N, K] of x's dtype, summed
  * in fp32 in sorted order; zeros for experts without routes). dy [routes, N]; order, offsets and counts from

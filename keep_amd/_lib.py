@@ -55,7 +55,8 @@ _SIGS = {
     "keep_route_combine_rows": [_P, c_int, _P, c_int64, c_int64, c_int64, _P, c_int, _P],
     "keep_route_combine_grad": [_P, c_int, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, _P],
     "keep_gather_mm": [_P, c_int, c_int64, _P, c_int, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P,
-                       _P, c_int64, _P, c_int, _P],
+                       _P, _P, _P, _P, c_int64, c_int64, _P, c_int, _P],
+    "keep_gather_mm_tile_supported": [c_int, c_int, c_int64, c_int64, c_int64],
     "keep_gather_mm_grad_weight": [_P, c_int, c_int64, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P, _P,
                                    _P],
     "keep_lora": [_P, c_int, c_int64, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P,

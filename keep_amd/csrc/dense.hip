@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "dense_dev.h"
+#include "dense_gemm.h"
 #include "dense_outer.h"
 
 namespace keep {
@@ -307,20 +308,30 @@ static void gather_launch(GatherArgs a, int64_t tiles, bool transposed, bool vec
 
 using namespace keep;
 
+extern "C" int keep_gather_mm_tile_supported(int dtype, int transposed, int64_t N, int64_t K, int64_t tile) {
+  if (!dims_ok({N, K, tile})) return 0;
+  if (tile == 16) return 1;
+  return (dtype == KEEP_F16 || dtype == KEEP_BF16) && dense_gemm_tile(tile) && K % 8 == 0 && (!transposed || N % 8 == 0);
+}
+
 extern "C" int keep_gather_mm(const void* x, int dtype, int64_t x_rows, const void* weight, int transposed,
                               const int32_t* rhs, const int32_t* lhs, int64_t routes, int64_t x_div,
-                              int64_t num_experts, int64_t N, int64_t K, const int32_t* order,
-                              const int32_t* tile_expert, const int32_t* tile_offset, const int32_t* tile_count,
-                              int64_t n_tiles, void* out, int out_dtype, void* stream) {
-  KEEP_REQUIRE_DIMS(x_rows, routes, x_div, num_experts, N, K, n_tiles);
+                              int64_t num_experts, int64_t N, int64_t K, const int32_t* order, const int32_t* offsets,
+                              const int32_t* counts, const int32_t* tile_expert, const int32_t* tile_offset,
+                              const int32_t* tile_count, const int32_t* valid_tiles, int64_t n_tiles, int64_t tile,
+                              void* out, int out_dtype, void* stream) {
+  KEEP_REQUIRE_DIMS(x_rows, routes, x_div, num_experts, N, K, n_tiles, tile);
   KEEP_REQUIRE(dtype_ok(dtype) && dtype_ok(out_dtype), "bad dtype enum");
   KEEP_REQUIRE(num_experts > 0 && N > 0 && K > 0, "num_experts, N and K must be positive");
   if (routes == 0) return KEEP_OK;
   KEEP_REQUIRE(x && weight && rhs && out && x_rows > 0, "null pointer argument");
   KEEP_REQUIRE(lhs || x_div > 0, "x_div must be > 0 without lhs");
-  KEEP_REQUIRE(!order == !tile_expert && !order == !tile_offset && !order == !tile_count,
-               "a route plan needs order and all three tile arrays");
+  for (const int32_t* p : {offsets, counts, tile_expert, tile_offset, tile_count, valid_tiles})
+    KEEP_REQUIRE(!order == !p, "a route plan needs all of its arrays");
   KEEP_REQUIRE(!order || n_tiles > 0, "a route plan needs n_tiles > 0");
+  const bool gemm = order && tile != 16;
+  KEEP_REQUIRE(!gemm || keep_gather_mm_tile_supported(dtype, transposed, N, K, tile),
+               "tiles of %lld routes need 16-bit rows of whole 16-byte pieces", (long long)tile);
   const int64_t size = dtype_size(dtype);
   KEEP_REQUIRE(aligned(x, size) && aligned(weight, size) && aligned(out, dtype_size(out_dtype)), "misaligned pointer");
   GatherArgs a{};
@@ -330,7 +341,19 @@ extern "C" int keep_gather_mm(const void* x, int dtype, int64_t x_rows, const vo
   a.order = order; a.te = tile_expert; a.to = tile_offset; a.tc = tile_count;
   a.out = out; a.odt = out_dtype;
   const int64_t tiles = order ? n_tiles : routes;
-  KEEP_REQUIRE(tiles <= 0x7fffffffLL / ((N + 15) / 16), "too many outputs");
+  KEEP_REQUIRE(tiles <= 0x7ffffff0LL / ((N + 15) / 16), "too many outputs");
+  if (gemm) {
+    KEEP_REQUIRE(aligned(x, 16) && aligned(weight, 16) && (out_dtype == dtype || out_dtype == KEEP_F32),
+                 "tiles of %lld routes need x and weight 16-byte aligned, and an output of x's dtype or float32",
+                 (long long)tile);
+    DenseGemmArgs g{};
+    g.x = x; g.x_rows = x_rows; g.x_div = a.x_div; g.lhs = lhs; g.w = weight;
+    g.E = num_experts; g.ni = N; g.nk = K; g.routes = routes;
+    g.order = order; g.offsets = offsets; g.counts = counts;
+    g.te = tile_expert; g.to = tile_offset; g.tc = tile_count; g.n_tiles = valid_tiles; g.max_tiles = n_tiles;
+    g.out = out; g.odt = out_dtype; g.wide = N % 8 == 0 && aligned(out, 16);
+    return dense_gemm_rows(g, dtype, transposed, tile, (hipStream_t)stream);
+  }
   const int64_t v = 16 / size;
   const bool vec = K % v == 0 && (!transposed || N % v == 0) && aligned(x, 16) && aligned(weight, 16) &&
                    aligned(out, 16);
@@ -352,6 +375,15 @@ extern "C" int keep_gather_mm_grad_weight(const void* x, int dtype, int64_t x_ro
   KEEP_REQUIRE(offsets && counts && dw && (routes == 0 || (x && dy && order && x_rows > 0)), "null pointer argument");
   const int64_t size = dtype_size(dtype);
   KEEP_REQUIRE(aligned(x, size) && aligned(dy, size) && aligned(dw, size), "misaligned pointer");
+  if (dtype != KEEP_F32 && N % 8 == 0 && K % 8 == 0 && aligned(x, 16) && aligned(dy, 16) && aligned(dw, 16)) {
+    KEEP_REQUIRE(num_experts <= 0x7ffffff0LL / (((N + 63) / 64) * ((K + 63) / 64)), "too many outputs");
+    DenseGemmArgs g{};
+    g.x = x; g.x_rows = x_rows; g.x_div = x_div; g.w = dy;
+    g.E = num_experts; g.ni = K; g.nj = N; g.routes = routes;
+    g.order = order; g.offsets = offsets; g.counts = counts;
+    g.out = dw; g.odt = dtype; g.wide = 1;
+    return dense_gemm_weight(g, dtype, (hipStream_t)stream);
+  }
   OuterArgs a{};
   a.i = x; a.i_rows = x_rows; a.i_div = x_div; a.i_dim = K;
   a.j = dy; a.j_ld = N; a.j_dim = N;

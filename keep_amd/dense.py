@@ -38,12 +38,12 @@ class _Plan:
         self.tile_expert = self.offsets + 4 * groups
         self.tile_offset = self.tile_expert + 4 * room
         self.tile_count = self.tile_offset + 4 * room
-        n_tiles = self.tile_count + 4 * room
+        self.valid_tiles = self.tile_count + 4 * room
         self.n_tiles = n  # descriptors that can hold routes: those come first
         self.tile = tile
         _lib.call("keep_route_plan", rhs.data_ptr() if R else None, R, groups, tile, self.order if R else None,
                   inverse if R else None, self.counts, self.offsets, self.tile_expert, self.tile_offset,
-                  self.tile_count, room, n_tiles, ops._stream(rhs.device))
+                  self.tile_count, room, self.valid_tiles, ops._stream(rhs.device))
 
 
 def _weight_layout(weight: torch.Tensor) -> tuple[torch.Tensor, bool]:
@@ -58,12 +58,30 @@ def _weight_layout(weight: torch.Tensor) -> tuple[torch.Tensor, bool]:
 
 def _launch(x, weight, transposed: bool, rhs, lhs, routes: int, x_div: int, N: int, K: int, plan: _Plan | None,
             out) -> torch.Tensor:
-    pl = plan
+    if plan is None:
+        tiles = (None,) * 7 + (0, 0)
+    else:
+        tile = plan.tile
+        if tile != ROUTE_TILE and not _gemm_takes(x, weight, transposed, N, K, tile):
+            plan = _Plan(rhs, weight.shape[0], ROUTE_TILE)
+        tiles = (plan.order, plan.offsets, plan.counts, plan.tile_expert, plan.tile_offset, plan.tile_count,
+                 plan.valid_tiles, plan.n_tiles, plan.tile)
     _lib.call("keep_gather_mm", x.data_ptr(), ops._DT[x.dtype], x.shape[0], weight.data_ptr(), int(transposed),
-              rhs.data_ptr(), ops._ptr(lhs), routes, x_div, weight.shape[0], N, K, pl and pl.order,
-              pl and pl.tile_expert, pl and pl.tile_offset, pl and pl.tile_count, pl.n_tiles if pl else 0,
-              out.data_ptr(), ops._DT[out.dtype], ops._stream(x.device))
+              rhs.data_ptr(), ops._ptr(lhs), routes, x_div, weight.shape[0], N, K, *tiles, out.data_ptr(),
+              ops._DT[out.dtype], ops._stream(x.device))
     return out
+
+
+def _gemm_takes(x, weight, transposed: bool, N: int, K: int, tile: int) -> bool:
+    return (x.data_ptr() % 16 == 0 and weight.data_ptr() % 16 == 0
+            and bool(_lib.load().keep_gather_mm_tile_supported(ops._DT[x.dtype], int(transposed), N, K, tile)))
+
+
+def _tile(routes: int, experts: int) -> int:
+    """Routes per tile of the plan."""
+
+    mean = routes / experts
+    return 16 if mean < 8 else 64 if mean < 96 else 128 if mean < 256 else 256
 
 
 def _forward(x: torch.Tensor, weight: torch.Tensor, rhs: torch.Tensor, lhs: torch.Tensor | None, x_div: int):
@@ -75,7 +93,7 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, rhs: torch.Tensor, lhs: torc
     if R == 0:
         return out, None
     w, transposed = _weight_layout(weight)
-    plan = _Plan(rhs, E, ROUTE_TILE) if R > WINDOW_ROUTES and E <= ops.PLAN_EXPERTS else None
+    plan = _Plan(rhs, E, _tile(R, E)) if R > WINDOW_ROUTES and E <= ops.PLAN_EXPERTS else None
     return _launch(x, w, transposed, rhs, lhs, R, x_div, N, K, plan, out), plan
 
 
@@ -101,7 +119,7 @@ def _backward(x, weight, rhs, plan, k: int, dy, needs):
     R = rhs.numel()
     dx = dw = None
     if plan is None and R and E <= ops.PLAN_EXPERTS and (needs[1] or R > WINDOW_ROUTES):
-        plan = _Plan(rhs, E, ROUTE_TILE)
+        plan = _Plan(rhs, E, _tile(R, E))
     if needs[0]:
         if R == 0:
             dx = torch.zeros_like(x)

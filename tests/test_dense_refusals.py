@@ -11,9 +11,13 @@ def _lib_call(name, **args):
     return getattr(_lib.load(), name)(*args.values())
 
 
+PLAN = dict(order=16, offsets=16, counts=16, te=16, to=16, tc=16, valid=16)
+
+
 def _gather(**over):
     args = dict(x=16, dtype=1, x_rows=4, w=16, transposed=0, rhs=16, lhs=None, routes=4, x_div=1, E=2, N=8, K=16,
-                order=None, te=None, to=None, tc=None, n_tiles=0, out=16, odt=1, stream=None)
+                order=None, offsets=None, counts=None, te=None, to=None, tc=None, valid=None, n_tiles=0, tile=0, out=16,
+                odt=1, stream=None)
     assert not set(over) - set(args)
     return _lib_call("keep_gather_mm", **{**args, **over})
 
@@ -31,8 +35,15 @@ def _gather(**over):
     (dict(x=17), "misaligned"),
     (dict(w=1), "misaligned"),
     (dict(out=3), "misaligned"),
-    (dict(order=16), "all three"),
-    (dict(order=16, te=16, to=16, tc=16), "n_tiles"),
+    (dict(order=16), "all of its arrays"),
+    (dict(te=16), "all of its arrays"),
+    (dict(**PLAN, n_tiles=0), "n_tiles"),
+    (dict(**PLAN, n_tiles=3, tile=64, dtype=0, odt=0), "16-bit rows"),
+    (dict(**PLAN, n_tiles=3, tile=64, K=20), "16-bit rows"),
+    (dict(**PLAN, n_tiles=3, tile=64, transposed=1, N=12), "16-bit rows"),
+    (dict(**PLAN, n_tiles=3, tile=32), "16-bit rows"),
+    (dict(**PLAN, n_tiles=3, tile=64, x=18), "16-byte aligned"),
+    (dict(**PLAN, n_tiles=3, tile=64, odt=2), "16-byte aligned"),
     (dict(routes=1 << 30, N=1 << 20), "too many"),
 ])
 def test_gather_mm_entry_refuses(over, msg):

@@ -53,6 +53,10 @@ SHAPES = [
     (300, 24, 4, 160, 264),
     (1100, 3, 1, 130, 72),    # hundreds of rows per expert
     (700, 2, 2, 264, 520),
+    (500, 5, 2, 136, 200),    # the product through LDS, tiles of 128 routes
+    (900, 3, 2, 512, 320),
+    (61, 5, 8, 1024, 64),
+    (2000, 40, 1, 64, 1032),
 ]
 
 
