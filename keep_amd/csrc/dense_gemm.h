@@ -15,6 +15,8 @@ struct DenseGemmArgs {
   int64_t max_tiles;
   void* out;
   int odt, wide;
+  int far;                      // an operand of 4 GiB or more (set at the launch)
+  uint32_t div_mul, div_shift;  // x_div as a multiplication (set at the launch)
 };
 
 bool dense_gemm_tile(int64_t tile);  // tiles of a plan that dense_gemm_rows takes

@@ -63,11 +63,21 @@ __device__ __forceinline__ uint4 dg_frag_t(const char* s, int ct, int ks, int la
   return f.v;
 }
 
-// 16 bytes per lane from g to lds_wave_base + 16 lane. Written out, since the compiler waits for every copy in flight
-// before any LDS read that follows the builtin: here the reads are of the other buffer, and the loop's own wait and
-// barrier stand between a copy and its readers. (No register is written, so none can be reused early.)
+// r / x_div for 0 <= r < 2^31: (2 r m) >> (32 + l) with l = ceil(log2 x_div), m = ceil(2^(31 + l) / x_div), exact since
+// m x_div - 2^(31 + l) < x_div <= 2^l.
+__device__ __forceinline__ int64_t dg_row(const DenseGemmArgs& a, int r) {
+  return (int64_t)(__umulhi(2u * (uint32_t)r, a.div_mul) >> a.div_shift);
+}
+
+// 16 bytes per lane to lds_wave_base + 16 lane, from an address per lane, or from one offset per lane off a common
+// base. Written out, since the compiler waits for every copy in flight before any LDS read that follows the builtin: here
+// the reads are of the other buffer, and the loop's own wait and barrier stand between a copy and its readers. (No
+// register is written, so none can be reused early.)
 __device__ __forceinline__ void dg_dma(const void* g, uint32_t lds_wave_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_wave_base), "v"(g)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_wave_base), "v"(g) : "memory");
+}
+__device__ __forceinline__ void dg_dma(const void* base, uint32_t off, uint32_t lds_wave_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_wave_base), "v"(off), "s"(base)
                : "memory");
 }
 
@@ -109,8 +119,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
       off = a.offsets[e];
       count = (int)min((int64_t)a.counts[e], a.routes - off);
     } else {
-      jt = item / nib;
-      ib = item - jt * nib;
+      // groups of up to 8 row tiles, within a group column block by column block: the 32 items that an XCD's CUs work on
+      // share 8 + 4 operand blocks where N is wide
+      const int64_t tiles = total / nib, group = item / (8 * nib), in = item - group * (8 * nib);
+      const int64_t rows = min((int64_t)8, tiles - group * 8);
+      ib = in / rows;
+      jt = group * 8 + in - ib * rows;
       e = a.te[jt];
       count = min(a.tc[jt], BJ);
       off = a.to[jt];
@@ -122,29 +136,44 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
   const int64_t kn = MODE == DG_WEIGHT ? count : a.nk;
   const int steps = e < 0 ? 0 : (int)((kn + DG_K - 1) / DG_K);
 
-  // ---- the copies of a step
+  // ---- the copies of a step. Common case: 32-bit offsets off a base that moves on with the steps. The last step of a
+  // summed index that is no multiple of 64, and operands of 4 GiB and more, take an address per lane, past the end that of
+  // a zero. Columns past the output's are copies of its last ones: their results are not stored.
   const T* wbase = (const T*)a.w + (MODE == DG_WEIGHT || e < 0 ? 0 : e * a.ni * a.nk);
-  const char* pi[TRI ? 1 : LI];  // FORWARD: this thread's rows of W
-  const char* pj[TRJ ? 1 : LJ];  // FORWARD, TRANS: this thread's rows of x
-  if constexpr (!TRI) {
-#pragma unroll
-    for (int i = 0; i < LI; ++i) {
-      const int L = tid + i * NT, row = L >> 3, s = (L & 7) ^ dg_swz_i(row);
-      pi[i] = (const char*)(wbase + min(i0 + row, a.ni - 1) * a.nk + s * 8);
-    }
-  }
-  if constexpr (!TRJ) {
-#pragma unroll
-    for (int i = 0; i < LJ; ++i) {
-      const int L = tid + i * NT, row = L >> 3, s = (L & 7) ^ dg_swz_j(row);
-      const int64_t r = a.order[off + min(row, count - 1)];
-      int64_t xr = a.lhs ? (int64_t)a.lhs[r] : (int64_t)((uint32_t)r / (uint32_t)a.x_div);
-      if (xr < 0 || xr >= a.x_rows) xr = 0;
-      pj[i] = (const char*)((const T*)a.x + xr * a.nk + s * 8);
-    }
-  }
-  // WEIGHT: the routes of this thread's copies in the next step (-1: past the expert's last)
   constexpr int RI = BI / 8, RJ = BJ / 8;  // 16-byte slots of a transposed row
+  auto col_t = [&](int i, bool jside) -> int64_t {  // first column of copy i of a transposed operand
+    const int L = tid + i * NT, R = jside ? RJ : RI, row = L / R, sl = L % R;
+    const int swz = jside ? dg_swz_t<BJ>(row) : dg_swz_t<BI>(row);
+    return (((sl >> 1) ^ swz) * 2 + (sl & 1)) * 8;
+  };
+  uint32_t oi[LI], oj[LJ];  // offsets in bytes (WEIGHT: of the columns alone)
+  int64_t xrow[TRJ ? 1 : LJ];
+#pragma unroll
+  for (int i = 0; i < LI; ++i) {
+    const int L = tid + i * NT;
+    if constexpr (!TRI) {
+      const int row = L >> 3;
+      oi[i] = (uint32_t)((min(i0 + row, a.ni - 1) - i0) * a.nk + ((L & 7) ^ dg_swz_i(row)) * 8) * 2u;
+    } else {
+      const int64_t col = min(i0 + col_t(i, false), a.ni - 8);
+      oi[i] = (uint32_t)((MODE == DG_TRANS ? (int64_t)(L / RI) * a.ni : 0) + col) * 2u;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < LJ; ++i) {
+    const int L = tid + i * NT;
+    if constexpr (!TRJ) {
+      const int row = L >> 3;
+      const int64_t r = a.order[off + min(row, count - 1)];
+      int64_t xr = a.lhs ? (int64_t)a.lhs[r] : dg_row(a, (int)r);
+      if (xr < 0 || xr >= a.x_rows) xr = 0;
+      xrow[i] = xr;
+      oj[i] = (uint32_t)(xr * a.nk + ((L & 7) ^ dg_swz_j(row)) * 8) * 2u;
+    } else {
+      oj[i] = (uint32_t)min(j0 + col_t(i, true), a.nj - 8) * 2u;
+    }
+  }
+  // WEIGHT: the routes of this thread's copies in a step to come (-1: past the expert's last)
   int ri[TRJ ? LI : 1], rj[TRJ ? LJ : 1];
   auto fetch = [&](int step) {
     if constexpr (TRJ) {
@@ -161,86 +190,123 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
     }
   };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wv * 1024;
-  auto issue = [&](int step, int buf) {
-    const uint32_t bi = lds0 + buf * (SI + SJ), bj = bi + SI;
-    const bool tail = (step + 1) * (int64_t)DG_K > kn;
-#pragma unroll
-    for (int i = 0; i < LI; ++i) {
+  const T* ibase = MODE == DG_FORWARD ? wbase + i0 * a.nk : MODE == DG_TRANS ? wbase : (const T*)a.x;
+  const T* jbase = MODE == DG_WEIGHT ? (const T*)a.w : (const T*)a.x;
+  const int64_t istep = MODE == DG_FORWARD ? DG_K : MODE == DG_TRANS ? DG_K * a.ni : 0;
+  const int64_t jstep = MODE == DG_WEIGHT ? 0 : DG_K;
+  // copy i of the step (the I side's first)
+  auto copy = [&](int i, int step) {
+    const uint32_t to = lds0 + (step & 1) * (SI + SJ) + i * (NT * 16);
+    const bool plain = !a.far && (step + 1) * (int64_t)DG_K <= kn;
+    if (i < LI) {
       const int L = tid + i * NT;
-      const void* g;
-      if constexpr (!TRI) {
-        const int s = (L & 7) ^ dg_swz_i(L >> 3);
-        g = tail && step * (int64_t)DG_K + s * 8 >= a.nk ? (const void*)&g_zero16 : pi[i] + (int64_t)step * (DG_K * 2);
-      } else {
-        const int row = L / RI, sl = L % RI;
-        const int64_t col = i0 + (((sl >> 1) ^ dg_swz_t<BI>(row)) * 2 + (sl & 1)) * 8;
-        if constexpr (MODE == DG_TRANS) {
-          const int64_t k = (int64_t)step * DG_K + row;
-          g = col < a.ni && k < a.nk ? (const void*)(wbase + k * a.ni + col) : (const void*)&g_zero16;
-        } else {
-          const int64_t xr = (uint32_t)ri[i] / (uint32_t)a.x_div;
-          g = col < a.ni && ri[i] >= 0 && xr < a.x_rows ? (const void*)((const T*)a.x + xr * a.ni + col)
-                                                        : (const void*)&g_zero16;
+      if (plain) {
+        uint32_t o = oi[i];
+        if constexpr (MODE == DG_WEIGHT) {
+          const int64_t xr = dg_row(a, ri[i]);
+          o += (uint32_t)min(xr, a.x_rows - 1) * (uint32_t)(a.ni * 2);
         }
-      }
-      dg_dma(g, bi + i * (NT * 16));
-    }
-#pragma unroll
-    for (int i = 0; i < LJ; ++i) {
-      const int L = tid + i * NT;
-      const void* g;
-      if constexpr (!TRJ) {
-        const int s = (L & 7) ^ dg_swz_j(L >> 3);
-        g = tail && step * (int64_t)DG_K + s * 8 >= a.nk ? (const void*)&g_zero16 : pj[i] + (int64_t)step * (DG_K * 2);
+        dg_dma(ibase + step * istep, o, to);
       } else {
-        const int row = L / RJ, sl = L % RJ;
-        const int64_t col = j0 + (((sl >> 1) ^ dg_swz_t<BJ>(row)) * 2 + (sl & 1)) * 8;
-        g = col < a.nj && rj[i] >= 0 && rj[i] < a.routes ? (const void*)((const T*)a.w + (int64_t)rj[i] * a.nj + col)
-                                                        : (const void*)&g_zero16;
+        const void* g;
+        if constexpr (MODE == DG_FORWARD) {
+          const int row = L >> 3;
+          const int64_t k = step * (int64_t)DG_K + ((L & 7) ^ dg_swz_i(row)) * 8;
+          g = k < a.nk ? (const void*)(wbase + min(i0 + row, a.ni - 1) * a.nk + k) : (const void*)&g_zero16;
+        } else if constexpr (MODE == DG_TRANS) {
+          const int64_t k = step * (int64_t)DG_K + L / RI, col = min(i0 + col_t(i, false), a.ni - 8);
+          g = k < a.nk ? (const void*)(wbase + k * a.ni + col) : (const void*)&g_zero16;
+        } else {
+          const int64_t xr = dg_row(a, ri[i]), col = min(i0 + col_t(i, false), a.ni - 8);
+          g = ri[i] >= 0 && xr < a.x_rows ? (const void*)((const T*)a.x + xr * a.ni + col) : (const void*)&g_zero16;
+        }
+        dg_dma(g, to);
       }
-      dg_dma(g, bj + i * (NT * 16));
+    } else {
+      i -= LI;
+      const int L = tid + i * NT;
+      if (plain) {
+        uint32_t o = oj[i];
+        if constexpr (MODE == DG_WEIGHT) o += min((uint32_t)rj[i], (uint32_t)(a.routes - 1)) * (uint32_t)(a.nj * 2);
+        dg_dma(jbase + step * jstep, o, to);
+      } else {
+        const void* g;
+        if constexpr (MODE != DG_WEIGHT) {
+          const int64_t k = step * (int64_t)DG_K + ((L & 7) ^ dg_swz_j(L >> 3)) * 8;
+          g = k < a.nk ? (const void*)((const T*)a.x + xrow[i] * a.nk + k) : (const void*)&g_zero16;
+        } else {
+          const int64_t col = min(j0 + col_t(i, true), a.nj - 8);
+          g = rj[i] >= 0 && rj[i] < a.routes ? (const void*)((const T*)a.w + (int64_t)rj[i] * a.nj + col) : (const void*)&g_zero16;
+        }
+        dg_dma(g, to);
+      }
     }
   };
 
+  // ---- products, half a step (32 of the summed index) at a time; the next half's fragments are read while this one's
+  // products run, and the copies of the step after next start with the second half
   f4 acc[FJ][FI];
 #pragma unroll
   for (int j = 0; j < FJ; ++j)
 #pragma unroll
     for (int i = 0; i < FI; ++i) acc[j][i] = f4{0.f, 0.f, 0.f, 0.f};
-  if (steps > 0) {
-    fetch(0);
-    issue(0, 0);
-    fetch(1);
-  }
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this step's copies
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();        // everybody's, and nobody reads the other buffer any more
-    asm volatile("" ::: "memory");
-    if (s + 1 < steps) {
-      issue(s + 1, (s + 1) & 1);
-      fetch(s + 2);
-    }
-    const char* bi = smem + (s & 1) * (SI + SJ);
+  struct Half {
+    uint4 f[FI + FJ];
+  };
+  auto read = [&](Half& h, int n, int step, int ks) {  // fragment n, the I side's first
+    const char* bi = smem + (step & 1) * (SI + SJ);
     const char* bj = bi + SI;
+    if (n < FI) {
+      // results of fragments 4 g + u are columns 64 g + 16 q + 4 u + v
+      if constexpr (TRI) h.f[n] = dg_frag_t<BI>(bi, wi * FI + n, ks, lane);
+      else h.f[n] = dg_frag<1>(bi, wi * TI + (n >> 2) * 64 + (c >> 2) * 16 + (n & 3) * 4 + (c & 3), ks, q);
+    } else {
+      if constexpr (TRJ) h.f[n] = dg_frag_t<BJ>(bj, wj * FJ + n - FI, ks, lane);
+      else h.f[n] = dg_frag<0>(bj, wj * TJ + (n - FI) * 16 + c, ks, q);
+    }
+  };
+  constexpr int NR = FI + FJ, NC = LI + LJ;
+  constexpr int CC = (NC * 2 + FJ - 1) / FJ;  // copies per group of products: all in the first half of the groups
+  auto half = [&](const Half& use, Half& next, int nstep, int nks, bool copies, int cstep) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      uint4 fi[FI], fj[FJ];
+    for (int j = 0; j < FJ; ++j) {
+      if (copies) {
 #pragma unroll
-      for (int i = 0; i < FI; ++i) {
-        // results of fragments 4 g + u are columns 64 g + 16 q + 4 u + v
-        if constexpr (TRI) fi[i] = dg_frag_t<BI>(bi, wi * FI + i, ks, lane);
-        else fi[i] = dg_frag<1>(bi, wi * TI + (i >> 2) * 64 + (c >> 2) * 16 + (i & 3) * 4 + (c & 3), ks, q);
+        for (int i = j * CC; i < (j + 1) * CC && i < NC; ++i) copy(i, cstep);
       }
 #pragma unroll
-      for (int j = 0; j < FJ; ++j) {
-        if constexpr (TRJ) fj[j] = dg_frag_t<BJ>(bj, wj * FJ + j, ks, lane);
-        else fj[j] = dg_frag<0>(bj, wj * TJ + j * 16 + c, ks, q);
-      }
+      for (int n = j * NR / FJ; n < (j + 1) * NR / FJ; ++n) read(next, n, nstep, nks);
 #pragma unroll
-      for (int j = 0; j < FJ; ++j)
+      for (int i = 0; i < FI; ++i) acc[j][i] = dense_mfma<T>(use.f[i], use.f[FI + j], acc[j][i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto landed = [&]() {  // this wave's reads are done and its copies landed, then everybody's
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  if (steps > 0) {
+    Half h0, h1;
+    fetch(0);
 #pragma unroll
-        for (int i = 0; i < FI; ++i) acc[j][i] = dense_mfma<T>(fi[i], fj[j], acc[j][i]);
+    for (int i = 0; i < NC; ++i) copy(i, 0);
+    fetch(1);
+    landed();
+    if (steps > 1) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) copy(i, 1);
+      fetch(2);
+    }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) read(h0, n, 0, 0);
+    for (int s = 0; s < steps; ++s) {
+      half(h0, h1, s, 1, false, 0);
+      landed();  // step s is read by everybody, step s + 1 is there
+      // (after the last step h0 takes the buffer's old bytes, not used)
+      half(h1, h0, s + 1, 0, s + 2 < steps, s + 2);
+      if (s + 2 < steps) fetch(s + 3);
     }
   }
 
@@ -257,7 +323,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
     } else {
       if (row >= count) continue;
       const int64_t r = a.order[off + row];
-      const int64_t xr = a.lhs ? (int64_t)a.lhs[r] : (int64_t)((uint32_t)r / (uint32_t)a.x_div);
+      if (r < 0 || r >= a.routes) continue;
+      const int64_t xr = a.lhs ? (int64_t)a.lhs[r] : dg_row(a, (int)r);
       ok = e >= 0 && xr >= 0 && xr < a.x_rows;
       at = r * a.ni;
     }
@@ -290,7 +357,14 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
 }
 
 template <typename T, int BI, int BJ, int WI, int WJ, int MODE>
-static void dg_launch(const DenseGemmArgs& a, hipStream_t s) {
+static void dg_launch(DenseGemmArgs a, hipStream_t s) {
+  int l = 0;
+  while ((int64_t(1) << l) < a.x_div) ++l;
+  a.div_shift = l;
+  a.div_mul = (uint32_t)(((uint64_t(1) << (31 + l)) + a.x_div - 1) / a.x_div);
+  const int64_t most = int64_t(1) << 31;  // of 16-bit values (256 rows past a block's first too)
+  a.far = MODE == DG_WEIGHT ? a.x_rows * a.ni >= most || a.routes * a.nj >= most
+                            : a.x_rows * a.nk >= most || 256 * (MODE == DG_TRANS ? a.ni : a.nk) >= most;
   const int64_t nib = (a.ni + BI - 1) / BI;
   const int64_t items = MODE == DG_WEIGHT ? a.E * ((a.nj + BJ - 1) / BJ) * nib : a.max_tiles * nib;
   const dim3 grid((unsigned)((items + 7) / 8 * 8));
@@ -318,8 +392,14 @@ int dense_gemm_rows(const DenseGemmArgs& a, int dtype, bool transposed, int64_t 
 }
 
 int dense_gemm_weight(const DenseGemmArgs& a, int dtype, hipStream_t s) {
-  if (dtype == KEEP_F16) dg_launch<_Float16, 128, 128, 2, 2, DG_WEIGHT>(a, s);
-  else dg_launch<bf16s, 128, 128, 2, 2, DG_WEIGHT>(a, s);
+  const bool large = a.ni >= 192 && a.nj >= 192;
+  if (dtype == KEEP_F16) {
+    if (large) dg_launch<_Float16, 256, 256, 4, 2, DG_WEIGHT>(a, s);
+    else dg_launch<_Float16, 128, 128, 2, 2, DG_WEIGHT>(a, s);
+  } else {
+    if (large) dg_launch<bf16s, 256, 256, 4, 2, DG_WEIGHT>(a, s);
+    else dg_launch<bf16s, 128, 128, 2, 2, DG_WEIGHT>(a, s);
+  }
   return launch_status("keep_gather_mm_grad_weight");
 }
 
