@@ -18,6 +18,7 @@
 // loads (four rows of 16 columns a time), its 32-byte pairs permuted likewise.
 // Past an operand's end, lanes copy a zero instead.
 #include <algorithm>
+#include <type_traits>
 
 #include "dense_dev.h"
 #include "dense_gemm.h"
@@ -141,13 +142,17 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
   // a zero. Columns past the output's are copies of its last ones: their results are not stored.
   const T* wbase = (const T*)a.w + (MODE == DG_WEIGHT || e < 0 ? 0 : e * a.ni * a.nk);
   constexpr int RI = BI / 8, RJ = BJ / 8;  // 16-byte slots of a transposed row
-  auto col_t = [&](int i, bool jside) -> int64_t {  // first column of copy i of a transposed operand
-    const int L = tid + i * NT, R = jside ? RJ : RI, row = L / R, sl = L % R;
+  auto col_t = [&](int L, bool jside) -> int64_t {  // first column of slot L of a transposed operand
+    const int R = jside ? RJ : RI, row = L / R, sl = L % R;
     const int swz = jside ? dg_swz_t<BJ>(row) : dg_swz_t<BI>(row);
     return (((sl >> 1) ^ swz) * 2 + (sl & 1)) * 8;
   };
+  auto x_row = [&](int row) -> int64_t {  // of the tile's row; rows past the last repeat it
+    const int64_t r = a.order[off + min(row, count - 1)];
+    const int64_t xr = a.lhs ? (int64_t)a.lhs[r] : dg_row(a, (int)r);
+    return xr < 0 || xr >= a.x_rows ? 0 : xr;
+  };
   uint32_t oi[LI], oj[LJ];  // offsets in bytes (WEIGHT: of the columns alone)
-  int64_t xrow[TRJ ? 1 : LJ];
 #pragma unroll
   for (int i = 0; i < LI; ++i) {
     const int L = tid + i * NT;
@@ -155,7 +160,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
       const int row = L >> 3;
       oi[i] = (uint32_t)((min(i0 + row, a.ni - 1) - i0) * a.nk + ((L & 7) ^ dg_swz_i(row)) * 8) * 2u;
     } else {
-      const int64_t col = min(i0 + col_t(i, false), a.ni - 8);
+      const int64_t col = min(i0 + col_t(L, false), a.ni - 8);
       oi[i] = (uint32_t)((MODE == DG_TRANS ? (int64_t)(L / RI) * a.ni : 0) + col) * 2u;
     }
   }
@@ -164,13 +169,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
     const int L = tid + i * NT;
     if constexpr (!TRJ) {
       const int row = L >> 3;
-      const int64_t r = a.order[off + min(row, count - 1)];
-      int64_t xr = a.lhs ? (int64_t)a.lhs[r] : dg_row(a, (int)r);
-      if (xr < 0 || xr >= a.x_rows) xr = 0;
-      xrow[i] = xr;
-      oj[i] = (uint32_t)(xr * a.nk + ((L & 7) ^ dg_swz_j(row)) * 8) * 2u;
+      oj[i] = (uint32_t)(x_row(row) * a.nk + ((L & 7) ^ dg_swz_j(row)) * 8) * 2u;
     } else {
-      oj[i] = (uint32_t)min(j0 + col_t(i, true), a.nj - 8) * 2u;
+      oj[i] = (uint32_t)min(j0 + col_t(L, true), a.nj - 8) * 2u;
     }
   }
   // WEIGHT: the routes of this thread's copies in a step to come (-1: past the expert's last)
@@ -195,11 +196,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
   const int64_t istep = MODE == DG_FORWARD ? DG_K : MODE == DG_TRANS ? DG_K * a.ni : 0;
   const int64_t jstep = MODE == DG_WEIGHT ? 0 : DG_K;
   // copy i of the step (the I side's first)
-  auto copy = [&](int i, int step) {
+  auto copy = [&](int i, int step, bool part) {
     const uint32_t to = lds0 + (step & 1) * (SI + SJ) + i * (NT * 16);
     const bool plain = !a.far && (step + 1) * (int64_t)DG_K <= kn;
     if (i < LI) {
-      const int L = tid + i * NT;
       if (plain) {
         uint32_t o = oi[i];
         if constexpr (MODE == DG_WEIGHT) {
@@ -208,34 +208,38 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
         }
         dg_dma(ibase + step * istep, o, to);
       } else {
+        int L = tid + i * NT;
+        asm volatile("" : "+v"(L));  // the addresses are made here, not kept over the loop
         const void* g;
         if constexpr (MODE == DG_FORWARD) {
           const int row = L >> 3;
           const int64_t k = step * (int64_t)DG_K + ((L & 7) ^ dg_swz_i(row)) * 8;
           g = k < a.nk ? (const void*)(wbase + min(i0 + row, a.ni - 1) * a.nk + k) : (const void*)&g_zero16;
         } else if constexpr (MODE == DG_TRANS) {
-          const int64_t k = step * (int64_t)DG_K + L / RI, col = min(i0 + col_t(i, false), a.ni - 8);
+          const int64_t k = step * (int64_t)DG_K + L / RI, col = min(i0 + col_t(L, false), a.ni - 8);
           g = k < a.nk ? (const void*)(wbase + k * a.ni + col) : (const void*)&g_zero16;
         } else {
-          const int64_t xr = dg_row(a, ri[i]), col = min(i0 + col_t(i, false), a.ni - 8);
+          const int64_t xr = dg_row(a, ri[i]), col = min(i0 + col_t(L, false), a.ni - 8);
           g = ri[i] >= 0 && xr < a.x_rows ? (const void*)((const T*)a.x + xr * a.ni + col) : (const void*)&g_zero16;
         }
         dg_dma(g, to);
       }
     } else {
       i -= LI;
-      const int L = tid + i * NT;
+      if (part && (wv * 64 + i * NT) / 8 >= count) return;  // eight rows past the tile's last: their results are not stored
       if (plain) {
         uint32_t o = oj[i];
         if constexpr (MODE == DG_WEIGHT) o += min((uint32_t)rj[i], (uint32_t)(a.routes - 1)) * (uint32_t)(a.nj * 2);
         dg_dma(jbase + step * jstep, o, to);
       } else {
+        int L = tid + i * NT;
+        asm volatile("" : "+v"(L));  // the addresses are made here, not kept over the loop
         const void* g;
         if constexpr (MODE != DG_WEIGHT) {
           const int64_t k = step * (int64_t)DG_K + ((L & 7) ^ dg_swz_j(L >> 3)) * 8;
-          g = k < a.nk ? (const void*)((const T*)a.x + xrow[i] * a.nk + k) : (const void*)&g_zero16;
+          g = k < a.nk ? (const void*)((const T*)a.x + x_row(L >> 3) * a.nk + k) : (const void*)&g_zero16;
         } else {
-          const int64_t col = min(j0 + col_t(i, true), a.nj - 8);
+          const int64_t col = min(j0 + col_t(L, true), a.nj - 8);
           g = rj[i] >= 0 && rj[i] < a.routes ? (const void*)((const T*)a.w + (int64_t)rj[i] * a.nj + col) : (const void*)&g_zero16;
         }
         dg_dma(g, to);
@@ -266,18 +270,21 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
     }
   };
   constexpr int NR = FI + FJ, NC = LI + LJ;
+  // this wave's fragments that hold rows
+  const int live = max(0, min(FJ, (count - wj * TJ + 15) / 16));
   constexpr int CC = (NC * 2 + FJ - 1) / FJ;  // copies per group of products: all in the first half of the groups
-  auto half = [&](const Half& use, Half& next, int nstep, int nks, bool copies, int cstep) {
+  auto half = [&](const Half& use, Half& next, int nstep, int nks, bool copies, int cstep, bool part) {
 #pragma unroll
     for (int j = 0; j < FJ; ++j) {
       if (copies) {
 #pragma unroll
-        for (int i = j * CC; i < (j + 1) * CC && i < NC; ++i) copy(i, cstep);
+        for (int i = j * CC; i < (j + 1) * CC && i < NC; ++i) copy(i, cstep, part);
       }
 #pragma unroll
       for (int n = j * NR / FJ; n < (j + 1) * NR / FJ; ++n) read(next, n, nstep, nks);
+      if (!part || j < live)
 #pragma unroll
-      for (int i = 0; i < FI; ++i) acc[j][i] = dense_mfma<T>(use.f[i], use.f[FI + j], acc[j][i]);
+        for (int i = 0; i < FI; ++i) acc[j][i] = dense_mfma<T>(use.f[i], use.f[FI + j], acc[j][i]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -287,27 +294,33 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  if (steps > 0) {
+  // PART: a tile with fewer rows than BJ leaves out the copies and products of fragments without rows
+  auto sum = [&](auto part_c) {
+    constexpr bool PART = decltype(part_c)::value;
     Half h0, h1;
     fetch(0);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) copy(i, 0);
+    for (int i = 0; i < NC; ++i) copy(i, 0, PART);
     fetch(1);
     landed();
     if (steps > 1) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) copy(i, 1);
+      for (int i = 0; i < NC; ++i) copy(i, 1, PART);
       fetch(2);
     }
 #pragma unroll
     for (int n = 0; n < NR; ++n) read(h0, n, 0, 0);
     for (int s = 0; s < steps; ++s) {
-      half(h0, h1, s, 1, false, 0);
+      half(h0, h1, s, 1, false, 0, PART);
       landed();  // step s is read by everybody, step s + 1 is there
       // (after the last step h0 takes the buffer's old bytes, not used)
-      half(h1, h0, s + 1, 0, s + 2 < steps, s + 2);
+      half(h1, h0, s + 1, 0, s + 2 < steps, s + 2, PART);
       if (s + 2 < steps) fetch(s + 3);
     }
+  };
+  if (steps > 0) {
+    if (MODE == DG_WEIGHT || count == BJ) sum(std::false_type{});
+    else if constexpr (MODE != DG_WEIGHT) sum(std::true_type{});
   }
 
   // ---- results: row j (route or n) of this lane, columns as above (TRANS, WEIGHT: 16 i + 4 q + v)

@@ -81,7 +81,7 @@ def _tile(routes: int, experts: int) -> int:
     """Routes per tile of the plan."""
 
     mean = routes / experts
-    return 16 if mean < 8 else 64 if mean < 96 else 128 if mean < 256 else 256
+    return 16 if mean < 2 else 64 if mean < 48 else 128 if mean < 100 else 256
 
 
 def _forward(x: torch.Tensor, weight: torch.Tensor, rhs: torch.Tensor, lhs: torch.Tensor | None, x_div: int):
