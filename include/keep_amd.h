@@ -594,10 +594,11 @@ int keep_gather_mm_grad_weight(const void* x, int dtype, int64_t x_rows, const v
 
 /* Low-rank adapters of many requests: out[r] = base[r] + scales[a] (x[r / x_div] A[a]^T) B[a]^T with a = idx[r].
  * x [x_rows, K], A [adapters, rank, K] and B [adapters, N, rank] of one dtype, rank in 1..128; scales fp32 [adapters]
- * or NULL (ones); base [routes, N] or NULL (zeros). idx < 0: no adapter; idx >= adapters: a NaN row. order (or NULL): a
+ * or NULL (ones); base [routes, N] of out's dtype or NULL (zeros); out of x's
+ * dtype or float32. idx < 0: no adapter; idx >= adapters: a NaN row. order (or NULL): a
  * permutation of the routes that brings those of one adapter together (keep_route_plan's). t_out (or NULL): the scaled
  * low-rank rows, fp32 [routes, keep_lora_rank_stride(rank)], zeros without an adapter. The workspace holds
- * keep_lora_workspace_bytes, 16-byte aligned. x = dy, A = B^T [adapters, rank, N], B = A^T [adapters, K, rank] gives the
+ * keep_lora_workspace_bytes, 16-byte aligned (t_out too). x = dy, A = B^T [adapters, rank, N], B = A^T [adapters, K, rank] gives the
  * gradient of x. */
 int keep_lora(const void* x, int dtype, int64_t x_rows, const void* a, const void* b, const float* scales,
               const int32_t* idx, const int32_t* order, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank,

@@ -50,10 +50,11 @@ __device__ __forceinline__ GatherTile gather_tile(const GatherArgs& a, int64_t t
     const int64_t p = (int64_t)a.to[tile] + c;
     if (c < t.count && p >= 0 && p < a.routes) t.route = a.order[p];
   } else {
-    const DenseTile d = dense_window_tile([&](int64_t p) { return a.rhs[p]; }, tile, a.routes, lane);
+    const DenseWindow w([&](int64_t p) { return a.rhs[p]; }, tile, a.routes, lane);
+    const DenseTile d = w.tile(tile, lane);
     t.count = d.count;
     if (t.count == 0) return t;
-    t.e = a.rhs[tile];
+    t.e = d.group;
     t.route = d.mine;
   }
   if (t.route >= a.routes) t.route = -1;
@@ -109,8 +110,8 @@ __global__ __launch_bounds__(64 * GF_WAVES) void k_gather_few(GatherArgs a) {
       for (int d = 0; d < UN; ++d) {
         const int64_t k = (s + d) * KS + q * V;
 #pragma unroll
-        for (int u = 0; u < NT; ++u) fi[d][u] = dense_ld<T, VEC>(wrow[u], k, INT64_MAX);
-        fj[d] = dense_ld<T, VEC>(xrow, k, INT64_MAX);
+        for (int u = 0; u < NT; ++u) fi[d][u] = dense_ld16(wrow[u], k);
+        fj[d] = dense_ld16(xrow, k);
       }
 #pragma unroll
       for (int d = 0; d < UN; ++d)
@@ -193,36 +194,51 @@ __global__ __launch_bounds__(64 * GT_WAVES) void k_gather_trans(GatherArgs a) {
 
 // ------------------------------------------------------------------ sums of outer products over a group's rows
 
-// Lane (c, q) of a step holds V neighbouring values of row 4 s + q of the wide side and one value per 16 of the narrow
-// side; product (u, b) takes value u. Four waves take every fourth step and are added in order through LDS.
-constexpr int RO_WAVES = 4, RO_NB = 2, RO_UN = 4;
+// Lane (c, q) of a step holds four neighbouring values of row 4 s + q of the wide side and one value per 16 of the narrow
+// side; product (u, b) takes value u. Eight waves take every eighth run of 32 routes, whose ids a lane each loads once, so
+// that a run's rows are all in flight together; the waves are added in order through LDS.
+constexpr int RO_WAVES = 8, RO_V = 4, RO_RUN = 32, RO_UN = RO_RUN / 4;
 
-template <typename TI, typename TJ, typename TO, bool VEC>
+template <typename T, bool VEC>
+__device__ __forceinline__ void ro_ld(const T* row, int64_t i, int64_t n, float (&f)[RO_V]) {
+  if constexpr (VEC && sizeof(T) == 2) {
+    const uint2 w = i < n ? *(const uint2*)(row + i) : make_uint2(0u, 0u);
+    f[0] = pair_lo<PairOf<T>::value>(w.x); f[1] = pair_hi<PairOf<T>::value>(w.x);
+    f[2] = pair_lo<PairOf<T>::value>(w.y); f[3] = pair_hi<PairOf<T>::value>(w.y);
+  } else if constexpr (VEC) {
+    const float4 w = i < n ? *(const float4*)(row + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
+  } else {
+#pragma unroll
+    for (int u = 0; u < RO_V; ++u) f[u] = i + u < n ? to_float(row[i + u]) : 0.f;
+  }
+}
+
+template <typename TI, typename TJ, typename TO, bool VEC, int NB>
 __global__ __launch_bounds__(64 * RO_WAVES) void k_rows_outer(OuterArgs a) {
-  constexpr int V = Dense<TI>::V;
-  __shared__ float4 red[RO_WAVES][V * RO_NB][64];
+  __shared__ float4 red[RO_WAVES][RO_V * NB][64];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int64_t i0 = (int64_t)blockIdx.x * (16 * V), j0 = (int64_t)blockIdx.y * (16 * RO_NB), g = blockIdx.z;
+  const int64_t i0 = (int64_t)blockIdx.x * (16 * RO_V), j0 = (int64_t)blockIdx.y * (16 * NB), g = blockIdx.z;
   const int64_t p0 = a.offsets[g], p1 = min(p0 + a.counts[g], a.routes);
-  f4 acc[V][RO_NB];
+  f4 acc[RO_V][NB];
 #pragma unroll
-  for (int u = 0; u < V; ++u)
+  for (int u = 0; u < RO_V; ++u)
 #pragma unroll
-    for (int b = 0; b < RO_NB; ++b) acc[u][b] = f4{0.f, 0.f, 0.f, 0.f};
-  const int64_t i = i0 + c * V;
-  for (int64_t p = p0 + 4 * wv; p < p1; p += 4 * RO_WAVES * RO_UN) {
-    uint4 fi[RO_UN];
-    float fj[RO_UN][RO_NB];
+    for (int b = 0; b < NB; ++b) acc[u][b] = f4{0.f, 0.f, 0.f, 0.f};
+  const int64_t i = i0 + c * RO_V;
+  for (int64_t p = p0 + RO_RUN * wv; p < p1; p += RO_RUN * RO_WAVES) {
+    const int64_t at = p + (lane & (RO_RUN - 1));
+    const int id = at < p1 ? a.order[at] : -1;
+    float fi[RO_UN][RO_V], fj[RO_UN][NB];
 #pragma unroll
     for (int d = 0; d < RO_UN; ++d) {
-      const int64_t at = p + 4 * RO_WAVES * d + q;
-      const int64_t r = at < p1 ? (int64_t)a.order[at] : -1;
-      const int64_t ir = r >= 0 && r < a.routes ? r / a.i_div : -1;
+      const int r = __shfl(id, 4 * d + q, 64);
+      const int64_t ir = r >= 0 && r < a.routes ? (int64_t)((uint32_t)r / (uint32_t)a.i_div) : -1;
       const bool ok = ir >= 0 && ir < a.i_rows;
-      fi[d] = ok ? dense_ld<TI, VEC>((const TI*)a.i + ir * a.i_dim, i, a.i_dim) : make_uint4(0u, 0u, 0u, 0u);
+      ro_ld<TI, VEC>((const TI*)a.i + (ok ? ir : 0) * a.i_dim, ok ? i : a.i_dim, a.i_dim, fi[d]);
 #pragma unroll
-      for (int b = 0; b < RO_NB; ++b) {
+      for (int b = 0; b < NB; ++b) {
         const int64_t j = j0 + 16 * b + c;
         fj[d][b] = ok && j < a.j_dim ? to_float(((const TJ*)a.j)[r * a.j_ld + j]) : 0.f;
       }
@@ -230,54 +246,60 @@ __global__ __launch_bounds__(64 * RO_WAVES) void k_rows_outer(OuterArgs a) {
 #pragma unroll
     for (int d = 0; d < RO_UN; ++d)
 #pragma unroll
-      for (int u = 0; u < V; ++u)
+      for (int u = 0; u < RO_V; ++u)
 #pragma unroll
-        for (int b = 0; b < RO_NB; ++b)
-          acc[u][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(dense_at<TI>(fi[d], u), fj[d][b], acc[u][b], 0, 0, 0);
+        for (int b = 0; b < NB; ++b)
+          acc[u][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fi[d][u], fj[d][b], acc[u][b], 0, 0, 0);
   }
 #pragma unroll
-  for (int u = 0; u < V; ++u)
+  for (int u = 0; u < RO_V; ++u)
 #pragma unroll
-    for (int b = 0; b < RO_NB; ++b)
-      red[wv][u * RO_NB + b][lane] = make_float4(acc[u][b][0], acc[u][b][1], acc[u][b][2], acc[u][b][3]);
+    for (int b = 0; b < NB; ++b)
+      red[wv][u * NB + b][lane] = make_float4(acc[u][b][0], acc[u][b][1], acc[u][b][2], acc[u][b][3]);
   __syncthreads();
-  // wave v: the results i0 + V (4 q + v) + u of column j0 + 16 b + c
-  const int64_t io = i0 + (4 * q + wv) * V;
+  // a quarter of the waves per v: the results i0 + 4 (4 q + v) + u of column j0 + 16 b + c
+  const int v = wv & 3;
+  const int64_t io = i0 + (4 * q + v) * RO_V;
   if (io >= a.i_dim) return;
   TO* out = (TO*)a.out + g * a.i_dim * a.j_dim;
 #pragma unroll
-  for (int b = 0; b < RO_NB; ++b) {
+  for (int b = 0; b < NB; ++b) {
+    if ((wv >> 2) != (b & 1)) continue;
     const int64_t j = j0 + 16 * b + c;
     if (j >= a.j_dim) continue;
-    float f[V];
+    float f[RO_V];
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
+    for (int u = 0; u < RO_V; ++u) {
       f[u] = 0.f;
 #pragma unroll
-      for (int w = 0; w < RO_WAVES; ++w) f[u] += ((const float*)&red[w][u * RO_NB + b][lane])[wv];
+      for (int w = 0; w < RO_WAVES; ++w) f[u] += ((const float*)&red[w][u * NB + b][lane])[v];
     }
     if (a.j_inner) {
 #pragma unroll
-      for (int u = 0; u < V; ++u)
+      for (int u = 0; u < RO_V; ++u)
         if (io + u < a.i_dim) out[(io + u) * a.j_dim + j] = from_float<TO>(f[u]);
     } else {
-      dense_st<TO, V>(out + j * a.i_dim + io, a.i_dim - io, f, VEC);
+      dense_st<TO, RO_V>(out + j * a.i_dim + io, a.i_dim - io, f, VEC);
     }
   }
+}
+
+template <typename TI, typename TJ, typename TO, int NB>
+static void outer_launch(const OuterArgs& a, int64_t groups, bool vec, hipStream_t s) {
+  const dim3 grid((unsigned)((a.i_dim + 16 * RO_V - 1) / (16 * RO_V)), (unsigned)((a.j_dim + 16 * NB - 1) / (16 * NB)),
+                  (unsigned)groups);
+  if (vec) hipLaunchKernelGGL((k_rows_outer<TI, TJ, TO, true, NB>), grid, dim3(64 * RO_WAVES), 0, s, a);
+  else hipLaunchKernelGGL((k_rows_outer<TI, TJ, TO, false, NB>), grid, dim3(64 * RO_WAVES), 0, s, a);
 }
 
 template <typename TI, typename TJ, typename TO>
 static void outer_launch(const OuterArgs& a, int64_t groups, bool vec, hipStream_t s) {
-  constexpr int V = Dense<TI>::V;
-  const dim3 grid((unsigned)((a.i_dim + 16 * V - 1) / (16 * V)), (unsigned)((a.j_dim + 16 * RO_NB - 1) / (16 * RO_NB)),
-                  (unsigned)groups);
-  if (vec) hipLaunchKernelGGL((k_rows_outer<TI, TJ, TO, true>), grid, dim3(64 * RO_WAVES), 0, s, a);
-  else hipLaunchKernelGGL((k_rows_outer<TI, TJ, TO, false>), grid, dim3(64 * RO_WAVES), 0, s, a);
+  if (a.j_dim <= 16) outer_launch<TI, TJ, TO, 1>(a, groups, vec, s);
+  else outer_launch<TI, TJ, TO, 2>(a, groups, vec, s);
 }
 
 int rows_outer(const OuterArgs& a, int dtype, bool j_float, int64_t groups, hipStream_t s, const char* what) {
-  const int64_t v = dtype == KEEP_F32 ? 4 : 8;
-  const bool vec = a.i_dim % v == 0 && aligned(a.i, 16) && aligned(a.out, 16);
+  const bool vec = a.i_dim % RO_V == 0 && aligned(a.i, 16) && aligned(a.out, 16);
   if (dtype == KEEP_F32) outer_launch<float, float, float>(a, groups, vec, s);
   else if (dtype == KEEP_F16 && j_float) outer_launch<_Float16, float, _Float16>(a, groups, vec, s);
   else if (dtype == KEEP_F16) outer_launch<_Float16, _Float16, _Float16>(a, groups, vec, s);

@@ -39,23 +39,27 @@ __device__ __forceinline__ f4 dense_mfma(const uint4& i, const uint4& j, f4 acc)
   }
 }
 
-// Values k .. k + V of a row of n values, zeros past its end (row = null: zeros). VEC: rows hold whole 16-byte
-// fragments at aligned addresses.
+// Values k .. k + V of a row, all there, at an aligned address.
+template <typename T>
+__device__ __forceinline__ uint4 dense_ld16(const T* row, int64_t k) {
+  typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+  const v4u v = *(const __attribute__((address_space(1))) v4u*)(row + k);
+  return uint4{v.x, v.y, v.z, v.w};
+}
+
+// Values k .. k + V of a row of n values, zeros past its end. VEC: rows hold whole 16-byte fragments at aligned addresses.
 template <typename T, bool VEC>
 __device__ __forceinline__ uint4 dense_ld(const T* row, int64_t k, int64_t n) {
-  uint4 r = make_uint4(0u, 0u, 0u, 0u);
-  if (!row || k >= n) return r;
   if constexpr (VEC) {
-    typedef unsigned int v4u __attribute__((ext_vector_type(4)));
-    const v4u v = *(const __attribute__((address_space(1))) v4u*)(row + k);
-    return uint4{v.x, v.y, v.z, v.w};
+    return k < n ? dense_ld16(row, k) : make_uint4(0u, 0u, 0u, 0u);
   } else {
     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < Dense<T>::V; ++i) {
-      if (k + i >= n) break;
-      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(row[k + i]);
-      else w[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[k + i]) << (16 * (i & 1));
+      if (k + i < n) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(row[k + i]);
+        else w[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[k + i]) << (16 * (i & 1));
+      }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -99,52 +103,64 @@ __device__ __forceinline__ void dense_st(T* p, int64_t n, const float (&f)[V], b
 }
 
 // The routes of a tile of up to 16, grouped without a plan: position r of a window of 128 positions heads a tile if a
-// multiple of 16 earlier positions of the window share its group; the tile is those of the next 16 that do. A wave
-// finds them with two ballots. group(p): the group of position p.
+// multiple of 16 earlier positions of the window share its group; the tile is those of the next 16 that do. A wave keeps
+// the window's groups in two registers and finds a tile with two ballots.
 constexpr int DENSE_WINDOW = 128;
 struct DenseTile {
-  int count;     // routes of the tile (0: r heads none)
+  int group;
+  int count;     // routes of the tile (0: the position heads none)
   int64_t mine;  // position of the tile's row c = lane % 16 (-1: none)
 };
 
-template <typename Group>
-__device__ __forceinline__ DenseTile dense_window_tile(Group group, int64_t r, int64_t routes, int lane) {
-  const int64_t base = r / DENSE_WINDOW * DENSE_WINDOW;
-  const int at = (int)(r - base);
-  const int g = group(r);
-  const bool h0 = base + lane < routes && group(base + lane) == g;
-  const bool h1 = base + 64 + lane < routes && group(base + 64 + lane) == g;
-  const uint64_t m0 = __ballot(h0), m1 = __ballot(h1);
-  const int below = at < 64 ? __popcll(m0 & ((1ull << at) - 1ull))
-                            : __popcll(m0) + __popcll(m1 & ((1ull << (at - 64)) - 1ull));
-  DenseTile t{0, -1};
-  if (below & 15) return t;
-  const int all = __popcll(m0) + __popcll(m1);
-  t.count = min(16, all - below);
-  const int c = lane & 15;
-  if (c < t.count) {  // the (below + c)-th set bit
-    int k = below + c;
-    uint64_t m = m0;
-    int off = 0;
-    if (k >= __popcll(m0)) {
-      k -= __popcll(m0);
-      m = m1;
-      off = 64;
-    }
-    // halving: the k-th set bit of m
-    int pos = 0;
-#pragma unroll
-    for (int w = 32; w >= 1; w >>= 1) {
-      const uint64_t low = (m >> pos) & ((1ull << w) - 1ull);
-      const int n = __popcll(low);
-      if (k >= n) {
-        k -= n;
-        pos += w;
-      }
-    }
-    t.mine = base + off + pos;
+struct DenseWindow {
+  int64_t base;
+  int g0, g1;     // groups of positions base + lane and base + 64 + lane
+  uint64_t v0, v1;
+
+  template <typename Group>
+  __device__ __forceinline__ DenseWindow(Group group, int64_t r, int64_t routes, int lane) {
+    base = r / DENSE_WINDOW * DENSE_WINDOW;
+    const bool h0 = base + lane < routes, h1 = base + 64 + lane < routes;
+    g0 = h0 ? group(base + lane) : 0;
+    g1 = h1 ? group(base + 64 + lane) : 0;
+    v0 = __ballot(h0);
+    v1 = __ballot(h1);
   }
-  return t;
-}
+
+  // r: a position of this window, the same in every lane
+  __device__ __forceinline__ DenseTile tile(int64_t r, int lane) const {
+    const int at = __builtin_amdgcn_readfirstlane((int)(r - base));
+    DenseTile t;
+    t.group = at < 64 ? __builtin_amdgcn_readlane(g0, at) : __builtin_amdgcn_readlane(g1, at - 64);
+    t.count = 0;
+    t.mine = -1;
+    const uint64_t m0 = __ballot(g0 == t.group) & v0, m1 = __ballot(g1 == t.group) & v1;
+    const int n0 = __popcll(m0);
+    const int below = at < 64 ? __popcll(m0 & ((1ull << at) - 1ull)) : n0 + __popcll(m1 & ((1ull << (at - 64)) - 1ull));
+    if (below & 15) return t;
+    t.count = min(16, n0 + __popcll(m1) - below);
+    const int c = lane & 15;
+    if (c < t.count) {  // the (below + c)-th set bit, by halving
+      int k = below + c, pos = 0;
+      uint64_t m = m0;
+      if (k >= n0) {
+        k -= n0;
+        m = m1;
+        pos = 64;
+      }
+      int at2 = 0;
+#pragma unroll
+      for (int w = 32; w >= 1; w >>= 1) {
+        const int n = __popcll((m >> at2) & ((1ull << w) - 1ull));
+        if (k >= n) {
+          k -= n;
+          at2 += w;
+        }
+      }
+      t.mine = base + pos + at2;
+    }
+    return t;
+  }
+};
 
 }  // namespace keep

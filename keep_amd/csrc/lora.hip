@@ -2,30 +2,39 @@
 //
 //   out[r] = base[r] + s[a] (x[row_r] A[a]^T) B[a]^T,   a = idx[r]   (A [n][R][K], B [n][N][R])
 //
-// a < 0: no adapter (out = base, or zeros); a >= n: a NaN row. Two launches:
+// a < 0: no adapter (out = base, or zeros); a >= n: a NaN row. Two launches over
+// the same tiles of up to 32 neighbouring routes of one adapter:
 //
-// k_lora_shrink: t = x A^T. A block takes a tile of up to 16 routes of one
-// adapter and a slice of K; its four waves split the slice, are added in order
-// through LDS, and the slice's partial t goes to the workspace in fp32.
+// k_lora_shrink: t = x A^T. Blocks along K take a slice each; a block's waves
+// share the slice and are added in order through LDS, and the slice's partial t
+// goes to the workspace in fp32.
 // k_lora_expand: adds the slices in order, times s, and streams B's rows of the
 // block's columns: out = base + t B^T.
 //
-// Tiles need no plan: rows of one adapter are found with two ballots over a
-// window of 128 positions (dense_window_tile), since rows of a request lie
-// together in a batch, or, of many requests, are few.
+// Tiles need no plan: a wave finds the runs of one adapter in a window of 128
+// positions with two ballots (LoraWindow), since rows of a request lie together
+// in a batch. Routes of several experts do not: those come with a plan's order.
+// One launch that repeats t in every block of columns took 1.1 to 1.6 times as
+// long at every size (one CU reads A, where the slices read it on many).
+//
+// Bound: the dependent loads at a block's start (window, partial sums, rows).
+// One row, r = 16, 4096 -> 4096: 9.3 us of which two empty launches take about
+// 5; 4093 rows in runs of about 100, r = 32: 48 us, the bytes alone 21.
 //
 // t enters the second product in the rows' 16-bit type (one rounding, half a
 // step of that type relative to the row's largest t), each row times a power of
 // two that brings its largest value to [1, 2): fp16 then holds every row
 // whatever its range. float rows stay float throughout.
 #include <algorithm>
+#include <type_traits>
 
 #include "dense_dev.h"
 #include "dense_outer.h"
 
 namespace keep {
 
-constexpr int LR_WAVES = 4;
+constexpr int LS_WAVES = 8, LE_WAVES = 8;
+constexpr int LORA_ROWS = 32;  // of a tile
 
 struct LoraArgs {
   const void* x;
@@ -35,206 +44,318 @@ struct LoraArgs {
   const int32_t *idx, *order;
   int64_t routes, x_div;
   int64_t n, R, K, N;
-  int cand;       // candidate positions per block
-  int64_t split;  // shrink: slices of K; expand: blocks along N
+  int heads;      // blocks per window: each takes every heads-th tile
+  int64_t split;  // slices of K; blocks along N
   int64_t slices;
   float* ws;  // [slices][routes][16 RT]
   float* t_out;
-  const void* base;
-  int bdt;
+  const void* base;  // null: zeros
   void* out;
-  int odt;
-  int wide;  // rows of base and out hold whole 16-byte pieces at aligned addresses
 };
 
-__device__ __forceinline__ int lora_group(const LoraArgs& a, int64_t p) {
-  const int g = a.idx[a.order ? (int64_t)a.order[p] : p];
-  return g < 0 ? -1 : g >= a.n ? (int)a.n : g;
+struct LoraTile {
+  int g, count;   // adapter (-1: none, n: out of range), routes (0: no tile)
+  int64_t first;  // their first position
+  bool has;
+};
+
+// The tiles of 128 positions: runs of one adapter, cut after LORA_ROWS rows.
+struct LoraWindow {
+  int64_t base;
+  int g0, g1, valid;
+  uint64_t h0, h1;  // positions that start a tile
+
+  __device__ __forceinline__ LoraWindow(const LoraArgs& a, int64_t window, int lane) {
+    base = window * 128;
+    valid = (int)min((int64_t)128, a.routes - base);
+    auto group = [&](int64_t p) {
+      const int g = a.idx[a.order ? (int64_t)a.order[p] : p];
+      return g < 0 ? -1 : g >= a.n ? (int)a.n : g;
+    };
+    g0 = lane < valid ? group(base + lane) : -2;
+    g1 = lane + 64 < valid ? group(base + 64 + lane) : -2;
+    const int p0 = __shfl_up(g0, 1, 64), p1 = __shfl_up(g1, 1, 64), last = __builtin_amdgcn_readlane(g0, 63);
+    const uint64_t f0 = __ballot(lane < valid && (lane == 0 || g0 != p0));
+    const uint64_t f1 = __ballot(lane + 64 < valid && g1 != (lane == 0 ? last : p1));
+    // from its run's start on, every LORA_ROWS-th position starts a tile
+    const uint64_t upto = (2ull << lane) - 1ull;
+    const int s0 = 63 - __clzll(f0 & upto), s1 = f1 & upto ? 127 - __clzll(f1 & upto) : 63 - __clzll(f0);
+    h0 = __ballot(lane < valid && ((lane - s0) & (LORA_ROWS - 1)) == 0);
+    h1 = __ballot(lane + 64 < valid && ((lane + 64 - s1) & (LORA_ROWS - 1)) == 0);
+  }
+
+  __device__ __forceinline__ int tiles() const { return __popcll(h0) + __popcll(h1); }
+
+  __device__ __forceinline__ LoraTile tile(const LoraArgs& a, int k) const {
+    const int n0 = __popcll(h0);
+    uint64_t m = k < n0 ? h0 : h1;
+    int i = k < n0 ? k : k - n0, at = 0;
+#pragma unroll
+    for (int w = 32; w >= 1; w >>= 1) {  // the i-th set bit of m, by halving
+      const int n = __popcll((m >> at) & ((1ull << w) - 1ull));
+      if (i >= n) {
+        i -= n;
+        at += w;
+      }
+    }
+    m = at == 63 ? 0 : m >> (at + 1) << (at + 1);
+    const int pos = __builtin_amdgcn_readfirstlane(at + (k < n0 ? 0 : 64));
+    int end = m ? __ffsll((unsigned long long)m) - 1 + (pos & 64) : pos < 64 && h1 ? 63 + __ffsll((unsigned long long)h1) : valid;
+    LoraTile t;
+    t.g = pos < 64 ? __builtin_amdgcn_readlane(g0, pos) : __builtin_amdgcn_readlane(g1, pos - 64);
+    t.count = __builtin_amdgcn_readfirstlane(end - pos);
+    t.first = base + pos;
+    t.has = t.g >= 0 && t.g < a.n;
+    return t;
+  }
+};
+
+// Route of row `row` of a tile (-1: past its last).
+__device__ __forceinline__ int64_t lora_route(const LoraArgs& a, const LoraTile& t, int row) {
+  if (row >= t.count) return -1;
+  return a.order ? (int64_t)a.order[t.first + row] : t.first + row;
 }
 
-template <typename T, bool VEC, int RT>
-__global__ __launch_bounds__(64 * LR_WAVES) void k_lora_shrink(LoraArgs a) {
-  constexpr int V = Dense<T>::V, KS = Dense<T>::KS, UN = RT <= 2 ? 4 : RT == 4 ? 2 : 1;
-  __shared__ float4 red[LR_WAVES][RT][64];
-  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int64_t cb = blockIdx.x / a.split, slice = blockIdx.x - cb * a.split;
-  const int64_t steps = (a.K + KS - 1) / KS, shares = a.split * LR_WAVES, per = (steps + shares - 1) / shares;
-  const int64_t s0 = min(steps, (slice * LR_WAVES + wv) * per), s1 = min(steps, s0 + per);
+// NJ fragments of 16 rows over the steps s0 .. s1: rank 16 u + 4 q + v of row 16 j + c.
+template <typename T, bool VEC, int RT, int NJ>
+__device__ __forceinline__ void lora_dot(const LoraArgs& a, const LoraTile& t, int64_t s0, int64_t s1, int lane,
+                                         f4 (&acc)[NJ][RT]) {
+  constexpr int V = Dense<T>::V, KS = Dense<T>::KS, UN = RT + NJ <= 4 ? 4 : RT + NJ <= 8 ? 2 : 1;
+  const int c = lane & 15, q = lane >> 4;
+  const T *xrow[NJ], *arow[RT];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {  // rows past the tile's last: row 0's values, not stored
+    const int64_t route = lora_route(a, t, 16 * j + c);
+    const int64_t xr = route < 0 ? 0 : min((int64_t)((uint32_t)route / (uint32_t)a.x_div), a.x_rows - 1);
+    xrow[j] = (const T*)a.x + xr * a.K;
+#pragma unroll
+    for (int u = 0; u < RT; ++u) acc[j][u] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int u = 0; u < RT; ++u) arow[u] = (const T*)a.a + ((int64_t)t.g * a.R + min((int64_t)(16 * u + c), a.R - 1)) * a.K;
   const int64_t whole = VEC ? min(s1, a.K / KS) : s0;
-  for (int cc = 0; cc < a.cand; ++cc) {
-    const int64_t pos = cb * a.cand + cc;
-    if (pos >= a.routes) break;
-    const int g = lora_group(a, pos);
-    if (g < 0 || g >= a.n) continue;
-    const DenseTile d = dense_window_tile([&](int64_t p) { return lora_group(a, p); }, pos, a.routes, lane);
-    if (d.count == 0) continue;
-    const int64_t route = d.mine < 0 ? -1 : a.order ? (int64_t)a.order[d.mine] : d.mine;
-    const int64_t xr = route < 0 ? 0 : min(route / a.x_div, a.x_rows - 1);
-    const T* xrow = (const T*)a.x + xr * a.K;  // lanes without a route: row 0's, not stored
-    const T* arow[RT];
+  int64_t s = s0;
+  for (; s + UN <= whole; s += UN) {
+    uint4 fi[UN][RT], fj[UN][NJ];
 #pragma unroll
-    for (int u = 0; u < RT; ++u) arow[u] = (const T*)a.a + ((int64_t)g * a.R + min((int64_t)(16 * u + c), a.R - 1)) * a.K;
-    f4 acc[RT];
+    for (int i = 0; i < UN; ++i) {
+      const int64_t k = (s + i) * KS + q * V;
 #pragma unroll
-    for (int u = 0; u < RT; ++u) acc[u] = f4{0.f, 0.f, 0.f, 0.f};
-    int64_t s = s0;
-    for (; s + UN <= whole; s += UN) {
-      uint4 fi[UN][RT], fj[UN];
+      for (int j = 0; j < NJ; ++j) fj[i][j] = dense_ld16(xrow[j], k);
 #pragma unroll
-      for (int i = 0; i < UN; ++i) {
-        const int64_t k = (s + i) * KS + q * V;
-        fj[i] = dense_ld<T, VEC>(xrow, k, INT64_MAX);
-#pragma unroll
-        for (int u = 0; u < RT; ++u) fi[i][u] = dense_ld<T, VEC>(arow[u], k, INT64_MAX);
-      }
-#pragma unroll
-      for (int i = 0; i < UN; ++i)
-#pragma unroll
-        for (int u = 0; u < RT; ++u) acc[u] = dense_mfma<T>(fi[i][u], fj[i], acc[u]);
-    }
-    for (; s < s1; ++s) {
-      const int64_t k = s * KS + q * V;
-      const uint4 fj = dense_ld<T, VEC>(xrow, k, a.K);
-#pragma unroll
-      for (int u = 0; u < RT; ++u) acc[u] = dense_mfma<T>(dense_ld<T, VEC>(arow[u], k, a.K), fj, acc[u]);
+      for (int u = 0; u < RT; ++u) fi[i][u] = dense_ld16(arow[u], k);
     }
 #pragma unroll
-    for (int u = 0; u < RT; ++u) red[wv][u][lane] = make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
-    __syncthreads();
-    for (int u = wv; u < RT; u += LR_WAVES) {
-      float4 f = red[0][u][lane];
+    for (int i = 0; i < UN; ++i)
 #pragma unroll
-      for (int w = 1; w < LR_WAVES; ++w) {
-        const float4 p = red[w][u][lane];
-        f.x += p.x; f.y += p.y; f.z += p.z; f.w += p.w;
-      }
-      if (route >= 0) *(float4*)(a.ws + (slice * a.routes + route) * (16 * RT) + 16 * u + 4 * q) = f;
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int u = 0; u < RT; ++u) acc[j][u] = dense_mfma<T>(fi[i][u], fj[i][j], acc[j][u]);
+  }
+  for (; s < s1; ++s) {
+    const int64_t k = s * KS + q * V;
+    uint4 fi[RT];
+#pragma unroll
+    for (int u = 0; u < RT; ++u) fi[u] = dense_ld<T, VEC>(arow[u], k, a.K);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const uint4 fj = dense_ld<T, VEC>(xrow[j], k, a.K);
+#pragma unroll
+      for (int u = 0; u < RT; ++u) acc[j][u] = dense_mfma<T>(fi[u], fj, acc[j][u]);
     }
-    __syncthreads();  // red is written again
   }
 }
 
-__device__ __forceinline__ float lora_ld(const void* p, int dt, int64_t i) {
-  if (dt == KEEP_F32) return ((const float*)p)[i];
-  if (dt == KEEP_BF16) return to_float(((const bf16s*)p)[i]);
-  return to_float(((const _Float16*)p)[i]);
+template <typename T, bool VEC, int RT>
+__global__ __launch_bounds__(64 * LS_WAVES) void k_lora_shrink(LoraArgs a) {
+  constexpr int KS = Dense<T>::KS;
+  __shared__ float4 red[LS_WAVES][RT][64];
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int64_t cb = blockIdx.x / a.split, slice = blockIdx.x - cb * a.split;
+  const int64_t window = cb / a.heads;
+  const LoraWindow w(a, window, lane);
+  const int64_t steps = (a.K + KS - 1) / KS, shares = a.split * LS_WAVES, per = (steps + shares - 1) / shares;
+  const int64_t s0 = min(steps, (slice * LS_WAVES + wv) * per), s1 = min(steps, s0 + per);
+  const int tiles = w.tiles();
+  for (int k = (int)(cb - window * a.heads); k < tiles; k += a.heads) {
+    const LoraTile t = w.tile(a, k);
+    if (!t.has) continue;
+    auto rows = [&](auto nj_c) {
+      constexpr int NJ = decltype(nj_c)::value;
+      f4 acc[NJ][RT];
+      lora_dot<T, VEC, RT, NJ>(a, t, s0, s1, lane, acc);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+        for (int u = 0; u < RT; ++u) red[wv][u][lane] = make_float4(acc[j][u][0], acc[j][u][1], acc[j][u][2], acc[j][u][3]);
+        __syncthreads();
+        const int64_t route = lora_route(a, t, 16 * j + c);
+        for (int u = wv; u < RT; u += LS_WAVES) {
+          float4 p[LS_WAVES];
+#pragma unroll
+          for (int i = 0; i < LS_WAVES; ++i) p[i] = red[i][u][lane];
+          float4 f = p[0];
+#pragma unroll
+          for (int i = 1; i < LS_WAVES; ++i) {
+            f.x += p[i].x; f.y += p[i].y; f.z += p[i].z; f.w += p[i].w;
+          }
+          if (route >= 0) *(float4*)(a.ws + (slice * a.routes + route) * (16 * RT) + 16 * u + 4 * q) = f;
+        }
+        __syncthreads();  // red is written again
+      }
+    };
+    if (t.count <= 16) rows(std::integral_constant<int, 1>{});
+    else rows(std::integral_constant<int, 2>{});
+  }
 }
 
-// A block's four waves take groups of 64 columns in turn. Lane (c, q) of product u holds B row 16 (c / 4) + 4 u + c % 4
-// of the group, so that the lane's results over the four products are 16 neighbouring columns of route c.
-template <typename T, bool VEC, int RT>
-__global__ __launch_bounds__(64 * LR_WAVES) void k_lora_expand(LoraArgs a) {
+// A wave takes 64 columns of a tile. Lane (c, q) of product u holds B row 32 (u / 2) + 8 (c / 4) + 4 (u % 2) + c % 4 of
+// them, so that the lane's results over two products are 8 neighbouring columns of route c, and a row's four lanes make
+// 64 bytes of each load and store. (No loop over columns: loads of a second turn would wait for the first one's stores.)
+// OT: base's and out's type. VEC: rows of B, base and out hold whole 16-byte pieces at aligned addresses.
+template <typename T, typename OT, bool VEC, int RT>
+__global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
   constexpr int V = Dense<T>::V, KS = Dense<T>::KS, RP = 16 * RT, NK = (RP + KS - 1) / KS;
-  __shared__ float ts[16][NK * KS + 4];
-  __shared__ float inv[16];
+  __shared__ float ts[LORA_ROWS][NK * KS + 4];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int64_t cb = blockIdx.x / a.split, nb = blockIdx.x - cb * a.split;
-  for (int cc = 0; cc < a.cand; ++cc) {
-    const int64_t pos = cb * a.cand + cc;
-    if (pos >= a.routes) break;
-    const DenseTile d = dense_window_tile([&](int64_t p) { return lora_group(a, p); }, pos, a.routes, lane);
-    if (d.count == 0) continue;
-    const int g = lora_group(a, pos);
-    const bool has = g >= 0 && g < a.n;
-    const int64_t route = d.mine < 0 ? -1 : a.order ? (int64_t)a.order[d.mine] : d.mine;
-    uint4 fj[NK];
-    if (has) {
-      const float sc = a.scales ? a.scales[g] : 1.f;
-      // 16 threads per row: thread k of row tid / 16 adds the slices of ranks k, k + 16, ...
-      const int row = threadIdx.x >> 4, k0 = threadIdx.x & 15;
-      const int64_t tr = __shfl(route, row, 64);  // lane row holds route row
-      float mx = 0.f;
-#pragma unroll
-      for (int u = 0; u < NK * KS / 16; ++u) {
-        const int k = 16 * u + k0;
-        float v = 0.f;
-        if (tr >= 0 && k < a.R) {
-          for (int64_t s = 0; s < a.slices; ++s) v += a.ws[(s * a.routes + tr) * RP + k];
-          v *= sc;
-        }
-        if (a.t_out && nb == 0 && tr >= 0 && k < RP) a.t_out[tr * RP + k] = v;
-        ts[row][k] = v;
-        mx = fmaxf(mx, fabsf(v));
+  const int64_t window = cb / a.heads;
+  const LoraWindow w(a, window, lane);
+  const int64_t n0 = (nb * LE_WAVES + wv) * 64;
+  const int tiles = w.tiles();
+  for (int k = (int)(cb - window * a.heads); k < tiles; k += a.heads) {
+    const LoraTile t = w.tile(a, k);
+    if (!t.has) {  // base as it is, zeros, or NaN
+      for (int64_t i = threadIdx.x; a.t_out && nb == 0 && i < t.count * RP; i += 64 * LE_WAVES)
+        a.t_out[lora_route(a, t, (int)(i / RP)) * RP + i % RP] = 0.f;
+      const int64_t n = n0 + lane;
+      for (int row = 0; row < t.count && n < a.N; ++row) {
+        const int64_t at = lora_route(a, t, row) * a.N + n;
+        ((OT*)a.out)[at] = t.g >= 0 ? from_float<OT>(__builtin_nanf("")) : a.base ? ((const OT*)a.base)[at] : from_float<OT>(0.f);
       }
+      continue;
+    }
+    auto rows = [&](auto nj_c) {
+      constexpr int NJ = decltype(nj_c)::value, OV = 16 / sizeof(OT);
+      int64_t at[NJ];  // of the row in base and out (-1: none)
 #pragma unroll
-      for (int m = 8; m >= 1; m >>= 1) mx = fmaxf(mx, __shfl_xor(mx, m, 64));
-      // 2^e <= mx: the factor 2^-e (1 for rows of zeros, subnormals, infinities; NaN does not reach mx)
-      const int e = (int)(__float_as_uint(mx) >> 23) - 127;
-      const bool use = sizeof(T) == 2 && e > -127 && e < 127;
-      if (k0 == 0) inv[row] = use ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
-      const float fac = use ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+      for (int j = 0; j < NJ; ++j) {
+        const int64_t r = lora_route(a, t, 16 * j + c);
+        at[j] = r < 0 ? -1 : r * a.N;
+      }
+      // B's rows and base are read before t is there
+      uint4 fi[NK][4], base[NJ][2][8 / OV];
+      const T* bb = (const T*)a.b + (int64_t)t.g * a.N * a.R;
 #pragma unroll
-      for (int u = 0; u < NK * KS / 16; ++u) ts[row][16 * u + k0] *= fac;
+      for (int i = 0; i < NK; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int64_t n = min(n0 + (u >> 1) * 32 + (c >> 2) * 8 + (u & 1) * 4 + (c & 3), a.N - 1);
+          const int r = i * KS + q * V;
+          if constexpr (VEC) {  // past the rank: zeros, loaded from the row's first values
+            fi[i][u] = dense_ld16(bb + n * a.R, r < a.R ? r : 0);
+            if (r >= a.R) fi[i][u] = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            fi[i][u] = dense_ld<T, VEC>(bb + n * a.R, r, a.R);
+          }
+        }
+      if (VEC && a.base) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int h = 0; h < 8 / OV; ++h)
+              base[j][p][h] = dense_ld16((const OT*)a.base + max(at[j], (int64_t)0), min(n0 + p * 32 + q * 8, a.N - 8) + h * OV);
+      }
+      const float sc = a.scales ? a.scales[t.g] : 1.f;
+      for (int i = threadIdx.x; i < NJ * 16 * RP / 4; i += 64 * LE_WAVES) {
+        const int row = i / (RP / 4), k4 = (i - row * (RP / 4)) * 4;
+        const int64_t tr = lora_route(a, t, row);
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tr >= 0) {
+          for (int64_t sl = 0; sl < a.slices; ++sl) {
+            const float4 p = *(const float4*)(a.ws + (sl * a.routes + tr) * RP + k4);
+            f.x += p.x; f.y += p.y; f.z += p.z; f.w += p.w;
+          }
+          f.x = k4 < a.R ? f.x * sc : 0.f;
+          f.y = k4 + 1 < a.R ? f.y * sc : 0.f;
+          f.z = k4 + 2 < a.R ? f.z * sc : 0.f;
+          f.w = k4 + 3 < a.R ? f.w * sc : 0.f;
+          if (a.t_out && nb == 0) *(float4*)(a.t_out + tr * RP + k4) = f;
+        }
+        *(float4*)&ts[row][k4] = f;
+        if (NK * KS > RP) *(float4*)&ts[row][RP + k4] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
       __syncthreads();
+      f4 acc[NJ][4];
+      float back[NJ];
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const float* p = &ts[c][i * KS + q * V];
+      for (int j = 0; j < NJ; ++j) {
+        float f[NK][V], mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            const float4 p = *(const float4*)&ts[16 * j + c][i * KS + q * V + e];
+            f[i][e] = p.x; f[i][e + 1] = p.y; f[i][e + 2] = p.z; f[i][e + 3] = p.w;
+            mx = fmaxf(fmaxf(fmaxf(mx, fabsf(p.x)), fabsf(p.y)), fmaxf(fabsf(p.z), fabsf(p.w)));
+          }
+        uint4 fj[NK];
         if constexpr (sizeof(T) == 4) {
-          fj[i] = make_uint4(__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3]));
+#pragma unroll
+          for (int i = 0; i < NK; ++i)
+            fj[i] = make_uint4(__float_as_uint(f[i][0]), __float_as_uint(f[i][1]), __float_as_uint(f[i][2]),
+                               __float_as_uint(f[i][3]));
+          back[j] = 1.f;
         } else {
-          uint32_t w[4];
+          mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          // 2^e <= mx: the factor 2^-e (1 for rows of zeros, subnormals, infinities; NaN does not reach mx)
+          const int e = (int)(__float_as_uint(mx) >> 23) - 127;
+          const bool use = e > -127 && e < 127;
+          const float fac = use ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+          back[j] = use ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
 #pragma unroll
-          for (int h = 0; h < 4; ++h)
-            w[h] = (uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(p[2 * h])) |
-                   ((uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(p[2 * h + 1])) << 16);
-          fj[i] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-    } else if (a.t_out && nb == 0 && d.mine >= 0) {
-      for (int k = wv * 4 + q; k < RP; k += 16) a.t_out[route * RP + k] = 0.f;
-    }
-    const float back = has ? inv[c] : 0.f;
-    const int64_t groups = (a.N + 63) / 64;
-    for (int64_t gi = nb * LR_WAVES + wv; gi < groups; gi += a.split * LR_WAVES) {
-      const int64_t n0 = gi * 64;
-      f4 acc[4];
+          for (int i = 0; i < NK; ++i) {
+            uint32_t v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) acc[u] = f4{0.f, 0.f, 0.f, 0.f};
-      if (has) {
-        const T* bb = (const T*)a.b + (int64_t)g * a.N * a.R;
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          uint4 fi[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int64_t n = min(n0 + (c >> 2) * 16 + u * 4 + (c & 3), a.N - 1);
-            fi[u] = dense_ld<T, VEC>(bb + n * a.R, i * KS + q * V, a.R);
+            for (int p = 0; p < 4; ++p)
+              v[p] = (uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(f[i][2 * p] * fac)) |
+                     ((uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(f[i][2 * p + 1] * fac)) << 16);
+            fj[i] = make_uint4(v[0], v[1], v[2], v[3]);
           }
+        }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) acc[u] = dense_mfma<T>(fi[u], fj[i], acc[u]);
+        for (int u = 0; u < 4; ++u) {
+          acc[j][u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < NK; ++i) acc[j][u] = dense_mfma<T>(fi[i][u], fj[i], acc[j][u]);
         }
       }
-      const int64_t n = n0 + q * 16;
-      if (route < 0 || n >= a.N) continue;
-      const int64_t at = route * a.N + n, left = a.N - n;
-      float f[16];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) f[4 * u + v] = has ? acc[u][v] * back : g >= 0 ? __builtin_nanf("") : 0.f;
-      const bool whole = left >= 16 && a.wide;
-      if (a.base) {
-        if (whole && a.bdt != KEEP_F32) {
+        for (int p = 0; p < 2; ++p) {
+          const int64_t n = n0 + p * 32 + q * 8;
+          if (at[j] < 0 || n >= a.N) continue;
+          float f[8];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint4 w = *(const uint4*)((const uint16_t*)a.base + at + 8 * h);
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-              f[8 * h + u] += a.bdt == KEEP_BF16 ? dense_at<bf16s>(w, u) : dense_at<_Float16>(w, u);
+          for (int u = 0; u < 8; ++u) {
+            f[u] = acc[j][2 * p + (u >> 2)][u & 3] * back[j];
+            if (a.base) {
+              if constexpr (VEC) f[u] += dense_at<OT>(base[j][p][u / OV], u % OV);
+              else f[u] += n + u < a.N ? to_float(((const OT*)a.base)[at[j] + n + u]) : 0.f;
+            }
           }
-        } else {
-#pragma unroll
-          for (int u = 0; u < 16; ++u)
-            if (u < left) f[u] += lora_ld(a.base, a.bdt, at + u);
+          dense_st<OT, 8>((OT*)a.out + at[j] + n, a.N - n, f, VEC);
         }
-      }
-      if (a.odt == KEEP_F32) dense_st<float, 16>((float*)a.out + at, left, f, whole);
-      else if (a.odt == KEEP_BF16) dense_st<bf16s, 16>((bf16s*)a.out + at, left, f, whole);
-      else dense_st<_Float16, 16>((_Float16*)a.out + at, left, f, whole);
-    }
-    __syncthreads();  // ts and inv are written again
+      __syncthreads();  // ts is written again
+    };
+    if (t.count <= 16) rows(std::integral_constant<int, 1>{});
+    else rows(std::integral_constant<int, 2>{});
   }
 }
 
@@ -242,27 +363,31 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_lora_expand(LoraArgs a) {
 
 static int lora_rt(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }
 
-// Positions per block: one while every position may be an adapter of its own, else 16 (about one tile's).
-static int lora_cand(int64_t routes) { return routes <= 256 ? 1 : 16; }
+// Blocks per window: one per position while every row may be a request of its own, else about as many as a window of
+// long runs has tiles.
+static int64_t lora_heads(int64_t routes) { return routes <= 256 ? std::min<int64_t>(routes, 128) : 6; }
+static int64_t lora_blocks(int64_t routes) { return (routes + 127) / 128 * lora_heads(routes); }
 
+// Slices of K: 48 KiB of A each (one row, r = 16 of 4096: 4 slices 9.3 us, 1 12.0; r = 128 of 8192: 16 slices 20, 4 28),
+// while the tiles leave CUs free (64 requests of r = 64: 4 slices 16.4 us, 8 19.4; 4093 rows of r = 32: 4 slices 48, 16
+// 68). Each wave takes at least one step of 64 bytes of a row.
 static int64_t lora_slices(int64_t routes, int64_t R, int64_t K, int size) {
-  const int64_t steps = (K * size + 63) / 64;                 // of 64 bytes of a row
-  const int64_t tiles = (routes + 15) / 16;
-  const int64_t want = std::max<int64_t>(1, 1024 / tiles);    // about four blocks per CU
-  return std::max<int64_t>(1, std::min<int64_t>({want, 16, (steps + 15) / 16}));
+  const int64_t steps = (K * size + 63) / 64, want = R * K * size / (48 << 10) + 1;
+  const int64_t room = routes <= 256 ? 256 / routes : 640 * 20 / routes;
+  return std::max<int64_t>(1, std::min<int64_t>({want, room, 16, steps / LS_WAVES}));
 }
 
-template <typename T, bool VECK, bool VECR>
-static void lora_launch(LoraArgs a, int64_t nsplit, hipStream_t s) {
-  const int64_t cbs = (a.routes + a.cand - 1) / a.cand;
-  const int rt = lora_rt(a.R);
+template <typename T, typename OT, bool VECK, bool VECR>
+static void lora_launch(LoraArgs a, hipStream_t s) {
+  const int64_t blocks = lora_blocks(a.routes), groups = (a.N + 64 * LE_WAVES - 1) / (64 * LE_WAVES);
   auto go = [&](auto c) {
     constexpr int RT = decltype(c)::value;
     a.split = a.slices;
-    hipLaunchKernelGGL((k_lora_shrink<T, VECK, RT>), dim3((unsigned)(cbs * a.slices)), dim3(64 * LR_WAVES), 0, s, a);
-    a.split = nsplit;
-    hipLaunchKernelGGL((k_lora_expand<T, VECR, RT>), dim3((unsigned)(cbs * nsplit)), dim3(64 * LR_WAVES), 0, s, a);
+    hipLaunchKernelGGL((k_lora_shrink<T, VECK, RT>), dim3((unsigned)(blocks * a.split)), dim3(64 * LS_WAVES), 0, s, a);
+    a.split = groups;
+    hipLaunchKernelGGL((k_lora_expand<T, OT, VECR, RT>), dim3((unsigned)(blocks * a.split)), dim3(64 * LE_WAVES), 0, s, a);
   };
+  const int rt = lora_rt(a.R);
   if (rt == 1) go(std::integral_constant<int, 1>{});
   else if (rt == 2) go(std::integral_constant<int, 2>{});
   else if (rt == 4) go(std::integral_constant<int, 4>{});
@@ -270,11 +395,16 @@ static void lora_launch(LoraArgs a, int64_t nsplit, hipStream_t s) {
 }
 
 template <typename T>
-static void lora_pick(const LoraArgs& a, int64_t nsplit, bool vk, bool vr, hipStream_t s) {
-  if (vk && vr) lora_launch<T, true, true>(a, nsplit, s);
-  else if (vk) lora_launch<T, true, false>(a, nsplit, s);
-  else if (vr) lora_launch<T, false, true>(a, nsplit, s);
-  else lora_launch<T, false, false>(a, nsplit, s);
+static void lora_pick(const LoraArgs& a, bool out_float, bool vk, bool vr, hipStream_t s) {
+  auto go = [&](auto ot) {
+    typedef decltype(ot) OT;
+    if (vk && vr) lora_launch<T, OT, true, true>(a, s);
+    else if (vk) lora_launch<T, OT, true, false>(a, s);
+    else if (vr) lora_launch<T, OT, false, true>(a, s);
+    else lora_launch<T, OT, false, false>(a, s);
+  };
+  if (out_float) go(float{});
+  else go(T{});
 }
 
 }  // namespace keep
@@ -285,6 +415,7 @@ extern "C" int64_t keep_lora_rank_stride(int64_t rank) { return rank >= 1 && ran
 
 extern "C" int64_t keep_lora_workspace_bytes(int dtype, int64_t routes, int64_t rank, int64_t K) {
   if (!dtype_ok(dtype) || !dims_ok({routes, rank, K}) || rank < 1 || rank > 128) return 0;
+  if (routes == 0) return 0;
   return lora_slices(routes, rank, K, dtype_size(dtype)) * routes * 16 * lora_rt(rank) * 4;
 }
 
@@ -293,16 +424,19 @@ extern "C" int keep_lora(const void* x, int dtype, int64_t x_rows, const void* a
                          int64_t rank, int64_t K, int64_t N, const void* base, int base_dtype, float* t_out,
                          void* workspace, int64_t workspace_bytes, void* out, int out_dtype, void* stream) {
   KEEP_REQUIRE_DIMS(x_rows, routes, x_div, adapters, rank, K, N);
-  KEEP_REQUIRE(dtype_ok(dtype) && dtype_ok(out_dtype) && (!base || dtype_ok(base_dtype)), "bad dtype enum");
+  KEEP_REQUIRE(dtype_ok(dtype) && dtype_ok(out_dtype), "bad dtype enum");
+  KEEP_REQUIRE((out_dtype == dtype || out_dtype == KEEP_F32) && (!base || base_dtype == out_dtype),
+               "out must have x's dtype or float32, and base out's");
   KEEP_REQUIRE(rank >= 1 && rank <= 128, "rank must be in 1..128");
   KEEP_REQUIRE(adapters > 0 && K > 0 && N > 0 && x_div > 0, "adapters, K, N and x_div must be positive");
   if (routes == 0) return KEEP_OK;
   KEEP_REQUIRE(x && a && b && idx && out && workspace && x_rows > 0, "null pointer argument");
+  KEEP_REQUIRE(lora_blocks(routes) <= 0x7fffffffLL / std::max<int64_t>(16, (N + 511) / 512), "too many outputs");
   KEEP_REQUIRE((routes - 1) / x_div < x_rows, "x holds %lld rows, %lld routes need more", (long long)x_rows,
                (long long)routes);
   const int64_t size = dtype_size(dtype);
   KEEP_REQUIRE(aligned(x, size) && aligned(a, size) && aligned(b, size) && aligned(out, dtype_size(out_dtype)) &&
-                   aligned(workspace, 16) && aligned(t_out, 4),
+                   aligned(workspace, 16) && aligned(t_out, 16),
                "misaligned pointer");
   const int64_t need = keep_lora_workspace_bytes(dtype, routes, rank, K);
   KEEP_REQUIRE(workspace_bytes >= need, "workspace needs %lld bytes, has %lld", (long long)need,
@@ -310,22 +444,18 @@ extern "C" int keep_lora(const void* x, int dtype, int64_t x_rows, const void* a
   LoraArgs p{};
   p.x = x; p.x_rows = x_rows; p.a = a; p.b = b; p.scales = scales; p.idx = idx; p.order = order;
   p.routes = routes; p.x_div = x_div; p.n = adapters; p.R = rank; p.K = K; p.N = N;
-  p.cand = lora_cand(routes);
+  p.heads = (int)lora_heads(routes);
   p.slices = lora_slices(routes, rank, K, (int)size);
   p.ws = (float*)workspace; p.t_out = t_out;
-  p.base = base; p.bdt = base ? base_dtype : KEEP_F32;
-  p.out = out; p.odt = out_dtype;
-  const int64_t cbs = (routes + p.cand - 1) / p.cand, groups = (N + 255) / 256;  // 256 columns a block and turn
-  const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(groups, 2048 / std::max<int64_t>(1, (routes + 15) / 16)));
-  KEEP_REQUIRE(cbs <= 0x7fffffffLL / std::max(nsplit, p.slices), "too many routes");
+  p.base = base; p.out = out;
   const int64_t v = 16 / size;
   const bool vk = K % v == 0 && aligned(x, 16) && aligned(a, 16);
-  const bool vr = rank % v == 0 && aligned(b, 16);
-  p.wide = N % 8 == 0 && aligned(base, 16) && aligned(out, 16);
+  const bool vr = rank % v == 0 && N % 8 == 0 && aligned(b, 16) && aligned(base, 16) && aligned(out, 16);
+  const bool f = out_dtype == KEEP_F32;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == KEEP_F32) lora_pick<float>(p, nsplit, vk, vr, s);
-  else if (dtype == KEEP_F16) lora_pick<_Float16>(p, nsplit, vk, vr, s);
-  else lora_pick<bf16s>(p, nsplit, vk, vr, s);
+  if (dtype == KEEP_F32) lora_pick<float>(p, f, vk, vr, s);
+  else if (dtype == KEEP_F16) lora_pick<_Float16>(p, f, vk, vr, s);
+  else lora_pick<bf16s>(p, f, vk, vr, s);
   return launch_status("keep_lora");
 }
 

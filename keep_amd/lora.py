@@ -3,7 +3,8 @@
 ``gather_lora`` adds each row's own adapter to the projection's output,
 ``out[r] = base[r] + s[a] (x[r] A[a]^T) B[a]^T`` with ``a = indices[r]`` (negative:
 no adapter; past the end: a NaN row), in two launches whatever the mix of
-requests (``keep_lora``). It is differentiable in ``x``, ``A``, ``B`` and
+requests (``keep_lora``). Rows of one adapter lie together in a batch of requests;
+scattered ones are right too, but read its factors once each. It is differentiable in ``x``, ``A``, ``B`` and
 ``base``. ``LoraAdapters`` holds the adapters of a layer: a dense projection
 (``QuantizedVQLinear``) or routed experts, one adapter per expert
 (``SwitchLinear``, ``QuantizedVQSwitchLinear``). Adapters of a lower rank than
@@ -27,11 +28,11 @@ PLANNED_ROUTES = 512
 def _launch(x, a, b, scales, idx, order, x_div: int, base, out, t_out) -> torch.Tensor:
     n, rank, K = a.shape
     R = idx.numel()
-    lib = _lib.load()
-    ws = torch.empty(lib.keep_lora_workspace_bytes(ops._DT[x.dtype], R, rank, K), dtype=torch.uint8, device=x.device)
+    need = _lib.load().keep_lora_workspace_bytes(ops._DT[x.dtype], R, rank, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
     _lib.call("keep_lora", x.data_ptr(), ops._DT[x.dtype], x.shape[0], a.data_ptr(), b.data_ptr(), ops._ptr(scales),
               idx.data_ptr(), order, R, x_div, n, rank, K, b.shape[1], ops._ptr(base),
-              ops._DT[base.dtype] if base is not None else 0, ops._ptr(t_out), ws.data_ptr(), ws.numel(),
+              ops._DT[base.dtype] if base is not None else 0, ops._ptr(t_out), ws.data_ptr(), need,
               out.data_ptr(), ops._DT[out.dtype], ops._stream(x.device))
     return out
 
@@ -130,8 +131,8 @@ def gather_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, ind
         raise ValueError(f"indices must be [{x.shape[0]}] or [{x.shape[0]}, top_k], found {tuple(idx.shape)}")
     x_div = idx.shape[1] if idx.ndim == 2 else 1
     shape = (*idx.shape, N)
-    if base is not None and (tuple(base.shape) != shape or base.dtype not in ops._DT):
-        raise ValueError(f"base must have shape {shape} in float32, float16 or bfloat16, found {tuple(base.shape)} "
+    if base is not None and (tuple(base.shape) != shape or base.dtype not in (x.dtype, torch.float32)):
+        raise ValueError(f"base must have shape {shape} in {x.dtype} or float32, found {tuple(base.shape)} "
                          f"in {base.dtype}")
     if scales is not None:
         if torch.is_grad_enabled() and scales.requires_grad:

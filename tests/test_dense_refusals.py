@@ -83,7 +83,8 @@ def _lora(**over):
 
 @pytest.mark.parametrize("over, msg", [
     (dict(dtype=5), "dtype"),
-    (dict(base=16, bdt=9), "dtype"),
+    (dict(base=16, bdt=0), "base out's"),
+    (dict(odt=2), "x's dtype or float32"),
     (dict(rank=0), "rank"),
     (dict(rank=129), "rank"),
     (dict(n=0), "positive"),
@@ -105,7 +106,7 @@ def test_lora_sizes():
     lib = _lib.load()
     assert [lib.keep_lora_rank_stride(r) for r in (0, 1, 16, 17, 64, 65, 128, 129)] == [0, 16, 16, 32, 64, 128, 128, 0]
     assert lib.keep_lora_workspace_bytes(1, -1, 16, 64) == 0 and lib.keep_lora_workspace_bytes(9, 1, 16, 64) == 0
-    assert lib.keep_lora_workspace_bytes(1, 1, 16, 4096) % (16 * 4) == 0 < lib.keep_lora_workspace_bytes(1, 1, 16, 64)
+    assert lib.keep_lora_workspace_bytes(1, 0, 16, 64) == 0 < lib.keep_lora_workspace_bytes(1, 1, 16, 64)
 
 
 @pytest.mark.parametrize("over, msg", [
