@@ -594,25 +594,28 @@ int keep_gather_mm_grad_weight(const void* x, int dtype, int64_t x_rows, const v
 
 /* Low-rank adapters of many requests: out[r] = base[r] + scales[a] (x[r / x_div] A[a]^T) B[a]^T with a = idx[r].
  * x [x_rows, K], A [adapters, rank, K] and B [adapters, N, rank] of one dtype, rank in 1..128; scales fp32 [adapters]
- * or NULL (ones); base [routes, N] of out's dtype or NULL (zeros); out of x's
- * dtype or float32. idx < 0: no adapter; idx >= adapters: a NaN row. order (or NULL): a
- * permutation of the routes that brings those of one adapter together (keep_route_plan's). t_out (or NULL): the scaled
- * low-rank rows, fp32 [routes, keep_lora_rank_stride(rank)], zeros without an adapter. The workspace holds
- * keep_lora_workspace_bytes, 16-byte aligned (t_out too). x = dy, A = B^T [adapters, rank, N], B = A^T [adapters, K, rank] gives the
- * gradient of x. */
+ * or NULL (ones); base [routes, N] of out's dtype or NULL (zeros); out of x's dtype or float32. idx < 0: no adapter;
+ * idx >= adapters: a NaN row. grouped (at most 1024 adapters): a route plan brings the routes of one adapter together
+ * first (without, runs of one adapter are found where they lie). t_out (or NULL): the scaled low-rank rows, fp32 [routes,
+ * keep_lora_rank_stride(rank)], zeros without an adapter. The workspace holds keep_lora_workspace_bytes, 16-byte aligned
+ * (t_out too). */
 int keep_lora(const void* x, int dtype, int64_t x_rows, const void* a, const void* b, const float* scales,
-              const int32_t* idx, const int32_t* order, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank,
-              int64_t K, int64_t N, const void* base, int base_dtype, float* t_out, void* workspace,
-              int64_t workspace_bytes, void* out, int out_dtype, void* stream);
-int64_t keep_lora_workspace_bytes(int dtype, int64_t routes, int64_t rank, int64_t K);
+              const int32_t* idx, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank, int64_t K, int64_t N,
+              const void* base, int base_dtype, float* t_out, int grouped, void* workspace, int64_t workspace_bytes,
+              void* out, int out_dtype, void* stream);
+int64_t keep_lora_workspace_bytes(int dtype, int64_t routes, int64_t adapters, int64_t rank, int64_t K, int grouped);
 int64_t keep_lora_rank_stride(int64_t rank);
 
-/* Gradient of one adapter factor: the sum over the routes r of each adapter of t[r]^T rows[r / x_div], [adapters, rank,
- * dim], or with rank_inner [adapters, dim, rank]. t fp32 [routes, t_stride] (keep_lora's t_out; for A that of the call
- * that gives the gradient of x); order, offsets and counts from keep_route_plan over idx. */
-int keep_lora_grad(const void* rows, int dtype, int64_t n_rows, int64_t x_div, int64_t dim, const float* t,
-                   int64_t t_stride, int64_t rank, int rank_inner, int64_t routes, int64_t adapters,
-                   const int32_t* order, const int32_t* offsets, const int32_t* counts, void* out, void* stream);
+/* Its gradients, from dy [routes, N] of x's dtype and the forward's t_out: dx [x_rows, K] (a row's routes added in fp32),
+ * da [adapters, rank, K], db [adapters, N, rank], each or NULL; routes = x_rows x_div. planned: with a route plan, which
+ * da and db need (at most 1024 adapters). base's gradient is dy. The workspace holds keep_lora_backward_workspace_bytes
+ * (dx, planned as in the call), 256-byte aligned. */
+int keep_lora_backward(const void* x, int dtype, int64_t x_rows, const void* a, const void* b, const float* scales,
+                       const int32_t* idx, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank, int64_t K,
+                       int64_t N, const float* t, const void* dy, void* dx, void* da, void* db, int planned,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+int64_t keep_lora_backward_workspace_bytes(int dtype, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank,
+                                           int64_t K, int64_t N, int dx, int planned);
 
 /* Random-sign Walsh-Hadamard transform of T rows of n activations (16 <= n <= 8192,
  * a power of two): forward y = FWHT(x * signs) / sqrt(n), inverse (inverse != 0)

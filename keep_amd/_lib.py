@@ -59,12 +59,13 @@ _SIGS = {
     "keep_gather_mm_tile_supported": [c_int, c_int, c_int64, c_int64, c_int64],
     "keep_gather_mm_grad_weight": [_P, c_int, c_int64, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P, _P,
                                    _P],
-    "keep_lora": [_P, c_int, c_int64, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P,
-                  c_int, _P, _P, c_int64, _P, c_int, _P],
-    "keep_lora_workspace_bytes": [c_int, c_int64, c_int64, c_int64],
+    "keep_lora": [_P, c_int, c_int64, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int,
+                  _P, c_int, _P, c_int64, _P, c_int, _P],
+    "keep_lora_workspace_bytes": [c_int, c_int64, c_int64, c_int64, c_int64, c_int],
     "keep_lora_rank_stride": [c_int64],
-    "keep_lora_grad": [_P, c_int, c_int64, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int64, c_int64, _P, _P, _P,
-                       _P, _P],
+    "keep_lora_backward": [_P, c_int, c_int64, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P,
+                           _P, _P, _P, _P, c_int, _P, c_int64, _P],
+    "keep_lora_backward_workspace_bytes": [c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int],
     "keep_rht": [_P, c_int, _P, c_int, c_int64, c_int64, _P, c_int, _P],
     "keep_rmsnorm_quant_rht": [_P, c_int, c_int64, c_int64, _P, c_int, c_float, c_int64, c_int, _P, _P, _P, c_int, _P],
     "keep_moe_combine_add": [_P, _P, c_int, _P, c_int, c_int64, _P, c_int, _P],
@@ -122,7 +123,8 @@ _SIGS = {
 _RESTYPE = {"keep_last_error": c_char_p, "keep_moe_tiles_workspace_bytes": c_int64,
             "keep_moe_layer1_workspace_bytes": c_int64,
             "keep_vq_grouped_gemm_q8_workspace_bytes": c_int64,
-            "keep_lora_workspace_bytes": c_int64, "keep_lora_rank_stride": c_int64}
+            "keep_lora_workspace_bytes": c_int64, "keep_lora_rank_stride": c_int64,
+            "keep_lora_backward_workspace_bytes": c_int64}
 EXPORTED = tuple(_SIGS)
 
 _lib = None

@@ -81,8 +81,8 @@ def combine_add(routed: torch.Tensor, shared: torch.Tensor | None = None, residu
             raise ValueError(f"{name} must match routed's shape {tuple(routed.shape)} in a float dtype")
     od = out_dtype or (residual.dtype if residual is not None else torch.float32)
     if _grad.wanted(routed, shared, residual):
-        held = _grad.check_capture(routed, shared, residual)  # noqa: F841
-        return _CombineAdd.apply(routed, shared, residual, od)
+        _grad.check_capture(routed, shared, residual)
+        return _grad.mark(_CombineAdd.apply(routed, shared, residual, od))
     return _combine_add(routed, shared, residual, od)
 
 

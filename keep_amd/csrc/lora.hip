@@ -50,7 +50,7 @@ struct LoraArgs {
   float* ws;  // [slices][routes][16 RT]
   float* t_out;
   const void* base;  // null: zeros
-  void* out;
+  void* out;  // null: t_out alone
 };
 
 struct LoraTile {
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
   const int64_t cb = blockIdx.x / a.split, nb = blockIdx.x - cb * a.split;
   const int64_t window = cb / a.heads;
   const LoraWindow w(a, window, lane);
-  const int64_t n0 = (nb * LE_WAVES + wv) * 64;
+  const int64_t n0 = (nb * LE_WAVES + wv) * 64, ncol = a.out ? a.N : 0;
   const int tiles = w.tiles();
   for (int k = (int)(cb - window * a.heads); k < tiles; k += a.heads) {
     const LoraTile t = w.tile(a, k);
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
       for (int64_t i = threadIdx.x; a.t_out && nb == 0 && i < t.count * RP; i += 64 * LE_WAVES)
         a.t_out[lora_route(a, t, (int)(i / RP)) * RP + i % RP] = 0.f;
       const int64_t n = n0 + lane;
-      for (int row = 0; row < t.count && n < a.N; ++row) {
+      for (int row = 0; row < t.count && n < ncol; ++row) {
         const int64_t at = lora_route(a, t, row) * a.N + n;
         ((OT*)a.out)[at] = t.g >= 0 ? from_float<OT>(__builtin_nanf("")) : a.base ? ((const OT*)a.base)[at] : from_float<OT>(0.f);
       }
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           const int64_t n = n0 + p * 32 + q * 8;
-          if (at[j] < 0 || n >= a.N) continue;
+          if (at[j] < 0 || n >= ncol) continue;
           float f[8];
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
@@ -357,6 +357,34 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
     if (t.count <= 16) rows(std::integral_constant<int, 1>{});
     else rows(std::integral_constant<int, 2>{});
   }
+}
+
+// Both factors transposed for the backward pass: [n][P][Q] -> [n][Q][P], 64 x 64 tiles through LDS.
+struct TransposeArgs {
+  const void* from[2];
+  void* to[2];
+  int64_t P[2], Q[2], blocks[2];
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_lora_transpose(TransposeArgs a) {
+  __shared__ T tile[64][66];
+  const int m = blockIdx.x >= a.blocks[0] ? 1 : 0;
+  int64_t b = blockIdx.x - (m ? a.blocks[0] : 0);
+  const int64_t P = a.P[m], Q = a.Q[m], pb = (P + 63) / 64, qb = (Q + 63) / 64;
+  const int64_t n = b / (pb * qb);
+  b -= n * pb * qb;
+  const int64_t p0 = b / qb * 64, q0 = (b - b / qb * qb) * 64;
+  const T* from = (const T*)a.from[m] + n * P * Q;
+  T* to = (T*)a.to[m] + n * P * Q;
+  const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 64; i += 4)
+    if (p0 + i + r < P && q0 + c < Q) tile[i + r][c] = from[(p0 + i + r) * Q + q0 + c];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 64; i += 4)
+    if (q0 + i + r < Q && p0 + c < P) to[(q0 + i + r) * P + p0 + c] = tile[c][i + r];
 }
 
 // ------------------------------------------------------------------ host side
@@ -384,7 +412,7 @@ static void lora_launch(LoraArgs a, hipStream_t s) {
     constexpr int RT = decltype(c)::value;
     a.split = a.slices;
     hipLaunchKernelGGL((k_lora_shrink<T, VECK, RT>), dim3((unsigned)(blocks * a.split)), dim3(64 * LS_WAVES), 0, s, a);
-    a.split = groups;
+    a.split = a.out ? groups : 1;
     hipLaunchKernelGGL((k_lora_expand<T, OT, VECR, RT>), dim3((unsigned)(blocks * a.split)), dim3(64 * LE_WAVES), 0, s, a);
   };
   const int rt = lora_rt(a.R);
@@ -409,71 +437,181 @@ static void lora_pick(const LoraArgs& a, bool out_float, bool vk, bool vr, hipSt
 
 }  // namespace keep
 
+namespace keep {
+
+// A plan's arrays in a workspace.
+struct LoraPlan {
+  int32_t *order, *inverse, *counts, *offsets, *tiles;
+  int64_t room;
+  static int64_t bytes(int64_t routes, int64_t n) {
+    return (4 * (2 * routes + 2 * n + 3 * ((routes + 15) / 16 + n) + 1) + 255) / 256 * 256;
+  }
+  int make(void* ws, const int32_t* idx, int64_t routes, int64_t n, void* stream) {
+    order = (int32_t*)ws;
+    inverse = order + routes;
+    counts = inverse + routes;
+    offsets = counts + n;
+    tiles = offsets + n;
+    room = (routes + 15) / 16 + n;
+    return keep_route_plan(idx, routes, n, 16, order, inverse, counts, offsets, tiles, tiles + room, tiles + 2 * room,
+                           room, tiles + 3 * room, stream);
+  }
+};
+
+static int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
+
+static int64_t lora_partials(int dtype, int64_t routes, int64_t rank, int64_t K) {
+  return round256(lora_slices(routes, rank, K, dtype_size(dtype)) * routes * 16 * lora_rt(rank) * 4);
+}
+
+static void lora_run(LoraArgs p, int dtype, int out_dtype, hipStream_t s) {
+  const int64_t size = dtype_size(dtype), v = 16 / size;
+  p.heads = (int)lora_heads(p.routes);
+  p.slices = lora_slices(p.routes, p.R, p.K, (int)size);
+  const bool vk = p.K % v == 0 && aligned(p.x, 16) && aligned(p.a, 16);
+  const bool vr = p.R % v == 0 && p.N % 8 == 0 && aligned(p.b, 16) && aligned(p.base, 16) && aligned(p.out, 16);
+  const bool f = out_dtype == KEEP_F32;
+  if (dtype == KEEP_F32) lora_pick<float>(p, f, vk, vr, s);
+  else if (dtype == KEEP_F16) lora_pick<_Float16>(p, f, vk, vr, s);
+  else lora_pick<bf16s>(p, f, vk, vr, s);
+}
+
+static int lora_check(int dtype, int64_t x_rows, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank,
+                      int64_t K, int64_t N, int grouped) {
+  KEEP_REQUIRE_DIMS(x_rows, routes, x_div, adapters, rank, K, N);
+  KEEP_REQUIRE(dtype_ok(dtype), "bad dtype enum");
+  KEEP_REQUIRE(rank >= 1 && rank <= 128, "rank must be in 1..128");
+  KEEP_REQUIRE(adapters > 0 && K > 0 && N > 0 && x_div > 0, "adapters, K, N and x_div must be positive");
+  KEEP_REQUIRE(!grouped || adapters <= 1024, "a plan holds at most 1024 adapters");
+  KEEP_REQUIRE(routes == 0 || (routes - 1) / x_div < x_rows, "x holds %lld rows, %lld routes need more",
+               (long long)x_rows, (long long)routes);
+  KEEP_REQUIRE(routes == 0 || lora_blocks(routes) <= 0x7fffffffLL / std::max<int64_t>(16, (std::max(N, K) + 511) / 512),
+               "too many outputs");
+  return KEEP_OK;
+}
+
+}  // namespace keep
+
 using namespace keep;
 
 extern "C" int64_t keep_lora_rank_stride(int64_t rank) { return rank >= 1 && rank <= 128 ? 16 * lora_rt(rank) : 0; }
 
-extern "C" int64_t keep_lora_workspace_bytes(int dtype, int64_t routes, int64_t rank, int64_t K) {
-  if (!dtype_ok(dtype) || !dims_ok({routes, rank, K}) || rank < 1 || rank > 128) return 0;
-  if (routes == 0) return 0;
-  return lora_slices(routes, rank, K, dtype_size(dtype)) * routes * 16 * lora_rt(rank) * 4;
+extern "C" int64_t keep_lora_workspace_bytes(int dtype, int64_t routes, int64_t adapters, int64_t rank, int64_t K,
+                                             int grouped) {
+  if (!dtype_ok(dtype) || !dims_ok({routes, adapters, rank, K}) || rank < 1 || rank > 128 || routes == 0) return 0;
+  return lora_partials(dtype, routes, rank, K) + (grouped ? LoraPlan::bytes(routes, adapters) : 0);
 }
 
 extern "C" int keep_lora(const void* x, int dtype, int64_t x_rows, const void* a, const void* b, const float* scales,
-                         const int32_t* idx, const int32_t* order, int64_t routes, int64_t x_div, int64_t adapters,
-                         int64_t rank, int64_t K, int64_t N, const void* base, int base_dtype, float* t_out,
-                         void* workspace, int64_t workspace_bytes, void* out, int out_dtype, void* stream) {
-  KEEP_REQUIRE_DIMS(x_rows, routes, x_div, adapters, rank, K, N);
-  KEEP_REQUIRE(dtype_ok(dtype) && dtype_ok(out_dtype), "bad dtype enum");
+                         const int32_t* idx, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank, int64_t K,
+                         int64_t N, const void* base, int base_dtype, float* t_out, int grouped, void* workspace,
+                         int64_t workspace_bytes, void* out, int out_dtype, void* stream) {
+  if (int rc = lora_check(dtype, x_rows, routes, x_div, adapters, rank, K, N, grouped)) return rc;
   KEEP_REQUIRE((out_dtype == dtype || out_dtype == KEEP_F32) && (!base || base_dtype == out_dtype),
                "out must have x's dtype or float32, and base out's");
-  KEEP_REQUIRE(rank >= 1 && rank <= 128, "rank must be in 1..128");
-  KEEP_REQUIRE(adapters > 0 && K > 0 && N > 0 && x_div > 0, "adapters, K, N and x_div must be positive");
   if (routes == 0) return KEEP_OK;
   KEEP_REQUIRE(x && a && b && idx && out && workspace && x_rows > 0, "null pointer argument");
-  KEEP_REQUIRE(lora_blocks(routes) <= 0x7fffffffLL / std::max<int64_t>(16, (N + 511) / 512), "too many outputs");
-  KEEP_REQUIRE((routes - 1) / x_div < x_rows, "x holds %lld rows, %lld routes need more", (long long)x_rows,
-               (long long)routes);
   const int64_t size = dtype_size(dtype);
   KEEP_REQUIRE(aligned(x, size) && aligned(a, size) && aligned(b, size) && aligned(out, dtype_size(out_dtype)) &&
-                   aligned(workspace, 16) && aligned(t_out, 16),
+                   aligned(base, dtype_size(out_dtype)) && aligned(workspace, 16) && aligned(t_out, 16),
                "misaligned pointer");
-  const int64_t need = keep_lora_workspace_bytes(dtype, routes, rank, K);
+  const int64_t need = keep_lora_workspace_bytes(dtype, routes, adapters, rank, K, grouped);
   KEEP_REQUIRE(workspace_bytes >= need, "workspace needs %lld bytes, has %lld", (long long)need,
                (long long)workspace_bytes);
   LoraArgs p{};
-  p.x = x; p.x_rows = x_rows; p.a = a; p.b = b; p.scales = scales; p.idx = idx; p.order = order;
+  p.x = x; p.x_rows = x_rows; p.a = a; p.b = b; p.scales = scales; p.idx = idx;
   p.routes = routes; p.x_div = x_div; p.n = adapters; p.R = rank; p.K = K; p.N = N;
-  p.heads = (int)lora_heads(routes);
-  p.slices = lora_slices(routes, rank, K, (int)size);
-  p.ws = (float*)workspace; p.t_out = t_out;
-  p.base = base; p.out = out;
-  const int64_t v = 16 / size;
-  const bool vk = K % v == 0 && aligned(x, 16) && aligned(a, 16);
-  const bool vr = rank % v == 0 && N % 8 == 0 && aligned(b, 16) && aligned(base, 16) && aligned(out, 16);
-  const bool f = out_dtype == KEEP_F32;
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == KEEP_F32) lora_pick<float>(p, f, vk, vr, s);
-  else if (dtype == KEEP_F16) lora_pick<_Float16>(p, f, vk, vr, s);
-  else lora_pick<bf16s>(p, f, vk, vr, s);
+  p.ws = (float*)workspace; p.t_out = t_out; p.base = base; p.out = out;
+  if (grouped) {
+    LoraPlan plan;
+    if (int rc = plan.make((char*)workspace + lora_partials(dtype, routes, rank, K), idx, routes, adapters, stream)) return rc;
+    p.order = plan.order;
+  }
+  lora_run(p, dtype, out_dtype, (hipStream_t)stream);
   return launch_status("keep_lora");
 }
 
-extern "C" int keep_lora_grad(const void* rows, int dtype, int64_t n_rows, int64_t x_div, int64_t dim, const float* t,
-                              int64_t t_stride, int64_t rank, int rank_inner, int64_t routes, int64_t adapters,
-                              const int32_t* order, const int32_t* offsets, const int32_t* counts, void* out,
-                              void* stream) {
-  KEEP_REQUIRE_DIMS(n_rows, x_div, dim, t_stride, rank, routes, adapters);
-  KEEP_REQUIRE(dtype_ok(dtype), "bad dtype enum");
-  KEEP_REQUIRE(rank >= 1 && rank <= 128 && t_stride >= rank, "rank must be in 1..128 and t_stride at least it");
-  KEEP_REQUIRE(adapters > 0 && adapters <= 65535 && dim > 0 && x_div > 0, "adapters, dim and x_div must be positive");
-  KEEP_REQUIRE(offsets && counts && out && (routes == 0 || (rows && t && order && n_rows > 0)), "null pointer argument");
-  KEEP_REQUIRE(aligned(rows, dtype_size(dtype)) && aligned(out, dtype_size(dtype)) && aligned(t, 4),
+// The backward workspace: both factors transposed, partial sums, dt, the routes' dx in float32 (several routes a row), the
+// plan.
+namespace keep {
+struct LoraBackward {
+  int64_t bt, at, partials, dt, rows, plan, total;
+  LoraBackward(int dtype, int64_t routes, int64_t x_div, int64_t n, int64_t rank, int64_t K, int64_t N, bool dx, bool planned) {
+    const int64_t size = dtype_size(dtype);
+    bt = 0;
+    at = bt + round256(n * rank * N * size);
+    partials = at + round256(n * rank * K * size);
+    dt = partials + lora_partials(dtype, routes, rank, N);
+    rows = dt + round256(routes * 16 * lora_rt(rank) * 4);
+    plan = rows + (dx && x_div > 1 ? round256(routes * K * 4) : 0);
+    total = plan + (planned ? LoraPlan::bytes(routes, n) : 0);
+  }
+};
+}  // namespace keep
+
+extern "C" int64_t keep_lora_backward_workspace_bytes(int dtype, int64_t routes, int64_t x_div, int64_t adapters,
+                                                      int64_t rank, int64_t K, int64_t N, int dx, int planned) {
+  if (!dtype_ok(dtype) || !dims_ok({routes, x_div, adapters, rank, K, N}) || rank < 1 || rank > 128 || routes == 0) return 0;
+  return LoraBackward(dtype, routes, x_div, adapters, rank, K, N, dx, planned).total;
+}
+
+extern "C" int keep_lora_backward(const void* x, int dtype, int64_t x_rows, const void* a, const void* b,
+                                  const float* scales, const int32_t* idx, int64_t routes, int64_t x_div,
+                                  int64_t adapters, int64_t rank, int64_t K, int64_t N, const float* t, const void* dy,
+                                  void* dx, void* da, void* db, int planned, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
+  if (int rc = lora_check(dtype, x_rows, routes, x_div, adapters, rank, K, N, planned)) return rc;
+  KEEP_REQUIRE(planned || (!da && !db), "gradients of the factors need a plan");
+  KEEP_REQUIRE(x_rows * x_div == routes, "x holds %lld rows of %lld routes, not %lld", (long long)x_rows,
+               (long long)x_div, (long long)routes);
+  if (routes == 0) return KEEP_OK;
+  KEEP_REQUIRE(x && a && b && idx && dy && workspace && (t || !db), "null pointer argument");
+  const int64_t size = dtype_size(dtype);
+  KEEP_REQUIRE(aligned(x, size) && aligned(a, size) && aligned(b, size) && aligned(dy, size) && aligned(dx, size) &&
+                   aligned(da, size) && aligned(db, size) && aligned(t, 16) && aligned(workspace, 256),
                "misaligned pointer");
-  OuterArgs a{};
-  a.i = rows; a.i_rows = n_rows; a.i_div = x_div; a.i_dim = dim;
-  a.j = t; a.j_ld = t_stride; a.j_dim = rank;
-  a.order = order; a.offsets = offsets; a.counts = counts; a.routes = routes;
-  a.out = out; a.j_inner = rank_inner;
-  return rows_outer(a, dtype, true, adapters, (hipStream_t)stream, "keep_lora_grad");
+  const LoraBackward w(dtype, routes, x_div, adapters, rank, K, N, dx != nullptr, planned);
+  KEEP_REQUIRE(workspace_bytes >= w.total, "workspace needs %lld bytes, has %lld", (long long)w.total,
+               (long long)workspace_bytes);
+  char* ws = (char*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  LoraPlan plan{};
+  if (planned)
+    if (int rc = plan.make(ws + w.plan, idx, routes, adapters, stream)) return rc;
+  float* dt = (float*)(ws + w.dt);
+  const int64_t stride = 16 * lora_rt(rank);
+  if (dx || da) {  // dt = s dy B, dx = dt A: the forward's two products on the transposed factors
+    TransposeArgs tr{{b, a}, {ws + w.bt, ws + w.at}, {N, rank}, {rank, K}, {0, 0}};
+    for (int m = 0; m < 2; ++m) tr.blocks[m] = adapters * ((tr.P[m] + 63) / 64) * ((tr.Q[m] + 63) / 64);
+    if (!dx) tr.blocks[1] = 0;
+    KEEP_REQUIRE(tr.blocks[0] + tr.blocks[1] <= 0x7fffffffLL, "too many factors");
+    const dim3 grid((unsigned)(tr.blocks[0] + tr.blocks[1]));
+    if (size == 4) hipLaunchKernelGGL(k_lora_transpose<uint32_t>, grid, dim3(256), 0, s, tr);
+    else hipLaunchKernelGGL(k_lora_transpose<uint16_t>, grid, dim3(256), 0, s, tr);
+    LoraArgs p{};
+    p.x = dy; p.x_rows = routes; p.a = ws + w.bt; p.b = ws + w.at; p.scales = scales; p.idx = idx;
+    p.order = planned && x_div > 1 ? plan.order : nullptr;
+    p.routes = routes; p.x_div = 1; p.n = adapters; p.R = rank; p.K = N; p.N = K;
+    p.ws = (float*)(ws + w.partials); p.t_out = dt;
+    const bool apart = dx && x_div > 1;  // a row's routes are added in float32 and rounded once
+    p.out = apart ? ws + w.rows : dx;
+    lora_run(p, dtype, apart ? KEEP_F32 : dtype, s);
+    if (apart)
+      if (int rc = keep_route_combine_rows(ws + w.rows, KEEP_F32, nullptr, x_rows, x_div, K, dx, dtype, stream)) return rc;
+  }
+  OuterArgs o{};
+  o.order = plan.order; o.offsets = plan.offsets; o.counts = plan.counts; o.routes = routes;
+  if (da) {
+    o.i = x; o.i_rows = x_rows; o.i_div = x_div; o.i_dim = K;
+    o.j = dt; o.j_ld = stride; o.j_dim = rank;
+    o.out = da; o.j_inner = 0;
+    if (int rc = rows_outer(o, dtype, true, adapters, s, "keep_lora_backward")) return rc;
+  }
+  if (db) {
+    o.i = dy; o.i_rows = routes; o.i_div = 1; o.i_dim = N;
+    o.j = t; o.j_ld = stride; o.j_dim = rank;
+    o.out = db; o.j_inner = 1;
+    if (int rc = rows_outer(o, dtype, true, adapters, s, "keep_lora_backward")) return rc;
+  }
+  return launch_status("keep_lora_backward");
 }

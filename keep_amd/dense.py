@@ -184,8 +184,8 @@ def gather_mm(x: torch.Tensor, weight: torch.Tensor, rhs_indices, *, lhs_indices
             ops._host_check_indices("lhs_indices", lhs, x.shape[0])
     with ops._on(device):
         if not grad:
-            return _forward(x.detach().contiguous(), weight.detach(), rhs, lhs, max(k, 1))[0].view(shape)
+            return _forward(x.contiguous(), weight, rhs, lhs, max(k, 1))[0].view(shape)
         if weight.requires_grad and E > ops.PLAN_EXPERTS:
             raise ValueError(f"a gradient of weight needs at most {ops.PLAN_EXPERTS} experts, found {E}")
-        held = _grad.check_capture(x, weight)  # noqa: F841
-        return _GatherMM.apply(x, weight, rhs, max(k, 1)).view(shape)
+        _grad.check_capture(x, weight)
+        return _grad.mark(_GatherMM.apply(x, weight, rhs, max(k, 1))).view(shape)

@@ -17,7 +17,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from keep_amd import _grad, _lib, ops
-from keep_amd.dense import _Plan
 
 MAX_RANK = 128
 # Routes (2D indices) from which a plan brings the routes of one adapter together first: rows of a request lie together
@@ -25,40 +24,33 @@ MAX_RANK = 128
 PLANNED_ROUTES = 512
 
 
-def _launch(x, a, b, scales, idx, order, x_div: int, base, out, t_out) -> torch.Tensor:
+def _forward(x, a, b, scales, idx, x_div: int, base, out_dtype, t_out=None) -> torch.Tensor:
     n, rank, K = a.shape
-    R = idx.numel()
-    need = _lib.load().keep_lora_workspace_bytes(ops._DT[x.dtype], R, rank, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    _lib.call("keep_lora", x.data_ptr(), ops._DT[x.dtype], x.shape[0], a.data_ptr(), b.data_ptr(), ops._ptr(scales),
-              idx.data_ptr(), order, R, x_div, n, rank, K, b.shape[1], ops._ptr(base),
-              ops._DT[base.dtype] if base is not None else 0, ops._ptr(t_out), ws.data_ptr(), need,
-              out.data_ptr(), ops._DT[out.dtype], ops._stream(x.device))
-    return out
-
-
-def _forward(x, a, b, scales, idx, x_div: int, base, out_dtype, t_out=None, plan=None):
-    R, N = idx.numel(), b.shape[1]
-    out = torch.empty((R, N), dtype=out_dtype, device=x.device)
+    R, N, device = idx.numel(), b.shape[1], x.device
+    out = torch.empty((R, N), dtype=out_dtype, device=device)
     if R == 0:
         return out
-    if plan is None and idx.ndim == 2 and R >= PLANNED_ROUTES and a.shape[0] <= ops.PLAN_EXPERTS:
-        plan = _Plan(idx, a.shape[0], 16)
-    return _launch(x, a, b, scales, idx, plan and plan.order, x_div, base, out, t_out)
+    dt, od = ops._DT[x.dtype], ops._DT[out_dtype]
+    grouped = int(x_div > 1 and R >= PLANNED_ROUTES and n <= ops.PLAN_EXPERTS)
+    need = _lib.load().keep_lora_workspace_bytes(dt, R, n, rank, K, grouped)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    _lib.call("keep_lora", x.data_ptr(), dt, x.shape[0], a.data_ptr(), b.data_ptr(), ops._ptr(scales), idx.data_ptr(), R,
+              x_div, n, rank, K, N, ops._ptr(base), od, ops._ptr(t_out), grouped, ws.data_ptr(), need, out.data_ptr(), od,
+              ops._stream(device))
+    return out
 
 
 class _GatherLora(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, b, base, scales, idx, x_div, out_dtype):
-        xc, ac, bc = x.contiguous(), a.contiguous(), b.contiguous()
-        R, rank = idx.numel(), a.shape[1]
+        x, a, b = x.contiguous(), a.contiguous(), b.contiguous()
         # the scaled low-rank rows, for B's gradient
-        t = torch.empty((R, _lib.load().keep_lora_rank_stride(rank)), dtype=torch.float32, device=x.device)
-        plan = _Plan(idx, a.shape[0], 16) if R and a.shape[0] <= ops.PLAN_EXPERTS else None
-        out = _forward(xc, ac, bc, scales, idx, x_div, None if base is None else base.contiguous(), out_dtype, t,
-                       plan if idx.ndim == 2 else None)
-        ctx.save_for_backward(xc, ac, bc, scales, idx, t)
-        ctx.plan, ctx.x_div = plan, x_div
+        t = torch.empty((idx.numel(), _lib.load().keep_lora_rank_stride(a.shape[1])), dtype=torch.float32,
+                        device=x.device)
+        ctx.base_shape = None if base is None else base.shape
+        out = _forward(x, a, b, scales, idx, x_div, None if base is None else base.contiguous(), out_dtype, t)
+        ctx.save_for_backward(x, a, b, scales, idx, t)
+        ctx.x_div = x_div
         return out
 
     @staticmethod
@@ -66,36 +58,20 @@ class _GatherLora(torch.autograd.Function):
     def backward(ctx, dy):
         x, a, b, scales, idx, t = ctx.saved_tensors
         nx, na, nb, nbase = ctx.needs_input_grad[:4]
-        with ops._on(x.device):
-            dx, da, db = _backward(x, a, b, scales, idx, t, ctx.plan, ctx.x_div, dy, nx, na, nb)
-        return dx, da, db, dy if nbase else None, None, None, None, None
-
-
-def _backward(x, a, b, scales, idx, t, plan, x_div: int, dy, nx: bool, na: bool, nb: bool):
-    (n, rank, K), N, R = a.shape, b.shape[1], idx.numel()
-    if R == 0:
-        return (torch.zeros_like(x) if nx else None, torch.zeros_like(a) if na else None,
-                torch.zeros_like(b) if nb else None)
-    g = dy.to(x.dtype).contiguous()  # a float32 output over 16-bit rows: its gradient enters the products in 16 bits
-    dx = da = db = None
-    if nx or na:  # dt = s dy B, dx = dt A: the same two products on the transposed factors
-        dt = torch.empty_like(t)
-        k = x_div
-        rows = torch.empty((R, K), dtype=x.dtype if k == 1 else torch.float32, device=x.device)
-        _launch(g, b.transpose(1, 2).contiguous(), a.transpose(1, 2).contiguous(), scales, idx,
-                plan.order if plan is not None and idx.ndim == 2 else None, 1, None, rows, dt)
-        if nx:
-            dx = rows if k == 1 else ops._sum_routes(rows, k, x.dtype)
-        if na:
-            da = torch.empty_like(a)
-            _lib.call("keep_lora_grad", x.data_ptr(), ops._DT[x.dtype], x.shape[0], x_div, K, dt.data_ptr(),
-                      dt.shape[1], rank, 0, R, n, plan.order, plan.offsets, plan.counts, da.data_ptr(),
-                      ops._stream(x.device))
-    if nb:
-        db = torch.empty_like(b)
-        _lib.call("keep_lora_grad", g.data_ptr(), ops._DT[g.dtype], R, 1, N, t.data_ptr(), t.shape[1], rank, 1, R, n,
-                  plan.order, plan.offsets, plan.counts, db.data_ptr(), ops._stream(x.device))
-    return dx, da, db
+        (n, rank, K), N, R, device = a.shape, b.shape[1], idx.numel(), x.device
+        make = torch.empty_like if R else torch.zeros_like
+        dx, da, db = (make(t_) if need else None for t_, need in ((x, nx), (a, na), (b, nb)))
+        if R and (nx or na or nb):
+            # a float32 output over 16-bit rows: its gradient enters the products in their type
+            g, dt = dy.to(x.dtype).contiguous(), ops._DT[x.dtype]
+            planned = int(na or nb or (ctx.x_div > 1 and R >= PLANNED_ROUTES and n <= ops.PLAN_EXPERTS))
+            with ops._on(device):
+                need = _lib.load().keep_lora_backward_workspace_bytes(dt, R, ctx.x_div, n, rank, K, N, int(nx), planned)
+                ws = torch.empty(need, dtype=torch.uint8, device=device)
+                _lib.call("keep_lora_backward", x.data_ptr(), dt, x.shape[0], a.data_ptr(), b.data_ptr(),
+                          ops._ptr(scales), idx.data_ptr(), R, ctx.x_div, n, rank, K, N, t.data_ptr(), g.data_ptr(),
+                          ops._ptr(dx), ops._ptr(da), ops._ptr(db), planned, ws.data_ptr(), need, ops._stream(device))
+        return dx, da, db, dy.reshape(ctx.base_shape) if nbase else None, None, None, None, None
 
 
 def gather_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, indices, *,
@@ -145,13 +121,12 @@ def gather_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, ind
     od = x.dtype if base is None else base.dtype
     with ops._on(device):
         if not _grad.wanted(x, lora_a, lora_b, base):
-            return _forward(x.detach().contiguous(), lora_a.detach().contiguous(), lora_b.detach().contiguous(), scales,
-                            idx, max(x_div, 1), None if base is None else base.detach().contiguous(), od).view(shape)
+            return _forward(x.contiguous(), lora_a.contiguous(), lora_b.contiguous(), scales, idx, max(x_div, 1),
+                            None if base is None else base.contiguous(), od).view(shape)
         if (lora_a.requires_grad or lora_b.requires_grad) and n > ops.PLAN_EXPERTS:
             raise ValueError(f"gradients of the factors need at most {ops.PLAN_EXPERTS} adapters, found {n}")
-        held = _grad.check_capture(x, lora_a, lora_b, base)  # noqa: F841
-        flat = None if base is None else base.reshape(-1, N)
-        return _GatherLora.apply(x, lora_a, lora_b, flat, scales, idx, max(x_div, 1), od).view(shape)
+        _grad.check_capture(x, lora_a, lora_b, base)
+        return _grad.mark(_GatherLora.apply(x, lora_a, lora_b, base, scales, idx, max(x_div, 1), od)).view(shape)
 
 
 class LoraAdapters:

@@ -728,9 +728,9 @@ def route_combine(y: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype 
         _dense_device(y)
         if od not in _DT:
             raise ValueError(f"unsupported output dtype {od}")
-        held = _grad.check_capture(y, weight)  # noqa: F841
+        _grad.check_capture(y, weight)
         with _on(y.device):
-            return _RouteCombine.apply(y, weight, od)
+            return _grad.mark(_RouteCombine.apply(y, weight, od))
     return _combine_rows(y.contiguous(), weight.float().contiguous(), od)
 
 

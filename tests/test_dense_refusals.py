@@ -75,8 +75,8 @@ def test_grad_weight_entry_refuses(over, msg):
 
 
 def _lora(**over):
-    args = dict(x=16, dtype=1, x_rows=4, a=16, b=16, scales=None, idx=16, order=None, routes=4, x_div=1, n=2, rank=16,
-                K=32, N=8, base=None, bdt=0, t_out=None, ws=16, ws_bytes=1 << 30, out=16, odt=1, stream=None)
+    args = dict(x=16, dtype=1, x_rows=4, a=16, b=16, scales=None, idx=16, routes=4, x_div=1, n=2, rank=16, K=32, N=8,
+                base=None, bdt=0, t_out=None, grouped=0, ws=16, ws_bytes=1 << 30, out=16, odt=1, stream=None)
     assert not set(over) - set(args)
     return _lib_call("keep_lora", **{**args, **over})
 
@@ -96,6 +96,9 @@ def _lora(**over):
     (dict(a=17), "misaligned"),
     (dict(ws=8), "misaligned"),
     (dict(ws_bytes=10), "workspace needs"),
+    (dict(n=1025, grouped=1), "at most 1024"),
+    (dict(base=17, bdt=1), "misaligned"),
+    (dict(routes=1 << 30, x_rows=1 << 30, N=1 << 20), "too many"),
 ])
 def test_lora_entry_refuses(over, msg):
     assert _lora(**over) == _lib.KEEP_EINVAL
@@ -105,18 +108,25 @@ def test_lora_entry_refuses(over, msg):
 def test_lora_sizes():
     lib = _lib.load()
     assert [lib.keep_lora_rank_stride(r) for r in (0, 1, 16, 17, 64, 65, 128, 129)] == [0, 16, 16, 32, 64, 128, 128, 0]
-    assert lib.keep_lora_workspace_bytes(1, -1, 16, 64) == 0 and lib.keep_lora_workspace_bytes(9, 1, 16, 64) == 0
-    assert lib.keep_lora_workspace_bytes(1, 0, 16, 64) == 0 < lib.keep_lora_workspace_bytes(1, 1, 16, 64)
+    need = lib.keep_lora_workspace_bytes
+    assert need(1, -1, 4, 16, 64, 0) == need(9, 1, 4, 16, 64, 0) == need(1, 0, 4, 16, 64, 0) == 0
+    assert 0 < need(1, 1, 4, 16, 64, 0) < need(1, 1, 4, 16, 64, 1)
+    need = lib.keep_lora_backward_workspace_bytes
+    assert need(1, 0, 1, 4, 16, 64, 32, 1, 1) == need(1, 4, 1, 4, 200, 64, 32, 1, 1) == 0
+    assert 0 < need(1, 8, 2, 4, 16, 64, 32, 0, 0) < need(1, 8, 2, 4, 16, 64, 32, 1, 0) < need(1, 8, 2, 4, 16, 64, 32, 1, 1)
 
 
 @pytest.mark.parametrize("over, msg", [
-    (dict(dtype=5), "dtype"), (dict(rank=200), "rank"), (dict(stride=8), "t_stride"), (dict(n=0), "positive"),
-    (dict(t=None), "null"), (dict(t=18), "misaligned"),
+    (dict(dtype=5), "dtype"), (dict(rank=200), "rank"), (dict(n=0), "positive"), (dict(planned=0), "need a plan"),
+    (dict(n=2000), "at most 1024"), (dict(routes=3), "rows of"), (dict(routes=5), "need more"), (dict(t=None), "null"),
+    (dict(dy=None), "null"), (dict(da=17), "misaligned"), (dict(ws=16), "misaligned"),
+    (dict(ws_bytes=100), "workspace needs"),
 ])
-def test_lora_grad_entry_refuses(over, msg):
-    args = dict(rows=16, dtype=1, n_rows=4, x_div=1, dim=32, t=16, stride=16, rank=16, inner=0, routes=4, n=2, order=16,
-                offsets=16, counts=16, out=16, stream=None)
-    assert _lib_call("keep_lora_grad", **{**args, **over}) == _lib.KEEP_EINVAL
+def test_lora_backward_entry_refuses(over, msg):
+    args = dict(x=16, dtype=1, x_rows=4, a=16, b=16, scales=None, idx=16, routes=4, x_div=1, n=2, rank=16, K=32, N=8,
+                t=16, dy=16, dx=16, da=16, db=16, planned=1, ws=256, ws_bytes=1 << 30, stream=None)
+    assert not set(over) - set(args)
+    assert _lib_call("keep_lora_backward", **{**args, **over}) == _lib.KEEP_EINVAL
     assert msg in _lib.load().keep_last_error().decode()
 
 
@@ -240,14 +250,20 @@ def test_capture_check_marks_live_eager_graphs(monkeypatch):
     w = torch.zeros(3, requires_grad=True)
     capturing = [False]
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
-    _grad.check_capture(w)  # nothing holds the node: the mark goes with it
+    _grad.mark(w * 2)  # nothing holds the node: the mark goes with it
     capturing[0] = True
     _grad.check_capture(w)
     capturing[0] = False
-    held = w * 2
-    _grad.check_capture(w)
+    held = _grad.mark((w * 2) * w)  # (a leaf beside an inner node)
     capturing[0] = True
     with pytest.raises(RuntimeError, match="eager graph"):
         _grad.check_capture(w)
     del held
     _grad.check_capture(w)
+    capturing[0] = False
+    held = _grad.mark(w.view(3, 1) * 2)  # under a view
+    capturing[0] = True
+    with pytest.raises(RuntimeError, match="eager graph"):
+        _grad.check_capture(w.view(1, 3))
+    del held
+    _grad.check_capture(w.view(1, 3))
