@@ -318,6 +318,17 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
       if (s + 2 < steps) fetch(s + 3);
     }
   };
+  // the routes of this lane's rows, read before the sums: -1 none, -2 - r a NaN row
+  int ro[MODE == DG_WEIGHT ? 1 : FJ];
+  if constexpr (MODE != DG_WEIGHT) {
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      const int row = wj * TJ + j * 16 + c;
+      const int r = a.order[off + min(row, count - 1)];
+      const int64_t xr = a.lhs ? (int64_t)a.lhs[r] : dg_row(a, r);
+      ro[j] = row >= count || r < 0 || r >= a.routes ? -1 : e >= 0 && xr >= 0 && xr < a.x_rows ? r : -2 - r;
+    }
+  }
   if (steps > 0) {
     if (MODE == DG_WEIGHT || count == BJ) sum(std::false_type{});
     else if constexpr (MODE != DG_WEIGHT) sum(std::true_type{});
@@ -334,12 +345,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
       if (j0 + row >= a.nj) continue;
       at = (e * a.nj + j0 + row) * a.ni;
     } else {
-      if (row >= count) continue;
-      const int64_t r = a.order[off + row];
-      if (r < 0 || r >= a.routes) continue;
-      const int64_t xr = a.lhs ? (int64_t)a.lhs[r] : dg_row(a, (int)r);
-      ok = e >= 0 && xr >= 0 && xr < a.x_rows;
-      at = r * a.ni;
+      if (ro[j] == -1) continue;
+      ok = ro[j] >= 0;
+      at = (int64_t)(ok ? ro[j] : -2 - ro[j]) * a.ni;
     }
     if constexpr (!TRI) {
 #pragma unroll
