@@ -93,37 +93,34 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wv % WI, wj = wv / WI;
 
   // work item: (j tile or expert and row block, i block), dealt to the XCDs in contiguous runs
-  int64_t e, jt, ib;
+  int64_t e;
+  uint32_t jt, ib;
   int count = 0;
   int64_t off = 0;
   {
-    const int64_t nib = (a.ni + BI - 1) / BI;
-    int64_t total;
-    if constexpr (MODE == DG_WEIGHT) total = a.E * ((a.nj + BJ - 1) / BJ) * nib;
-    else {
-      int64_t tiles = a.n_tiles[0];  // tiles of valid experts; those of invalid routes follow
-      const int64_t valid = (int64_t)a.offsets[a.E - 1] + a.counts[a.E - 1];
-      tiles = min(tiles + (a.routes - valid + BJ - 1) / BJ, a.max_tiles);
-      total = tiles * nib;
-    }
-    const int64_t per = (total + 7) / 8;
-    const int64_t slot = blockIdx.x >> 3;
-    if (slot >= per) return;
-    const int64_t item = (blockIdx.x & 7) * per + slot;
-    if (item >= total) return;
+    const uint32_t nib = (uint32_t)((a.ni + BI - 1) / BI);
+    uint32_t total, ntiles = 0;
     if constexpr (MODE == DG_WEIGHT) {
-      const int64_t njb = (a.nj + BJ - 1) / BJ;
-      e = item / (njb * nib);
-      const int64_t r = item - e * (njb * nib);
+      total = (uint32_t)a.E * (uint32_t)((a.nj + BJ - 1) / BJ) * nib;
+    } else {
+      // tiles of valid experts; those of invalid routes follow
+      const int64_t valid = (int64_t)a.offsets[a.E - 1] + a.counts[a.E - 1];
+      ntiles = (uint32_t)min(a.n_tiles[0] + (a.routes - valid + BJ - 1) / BJ, a.max_tiles);
+      total = ntiles * nib;
+    }
+    const uint32_t per = (total + 7) / 8, slot = blockIdx.x >> 3, item = (blockIdx.x & 7) * per + slot;
+    if (slot >= per || item >= total) return;
+    if constexpr (MODE == DG_WEIGHT) {
+      const uint32_t njb = (uint32_t)((a.nj + BJ - 1) / BJ), ex = item / (njb * nib), r = item - ex * (njb * nib);
       jt = r / nib;
       ib = r - jt * nib;
-      off = a.offsets[e];
-      count = (int)min((int64_t)a.counts[e], a.routes - off);
+      e = ex;
+      off = a.offsets[ex];
+      count = (int)max((int64_t)0, min((int64_t)a.counts[ex], a.routes - off));
     } else {
       // groups of up to 8 row tiles, within a group column block by column block: the 32 items that an XCD's CUs work on
       // share 8 + 4 operand blocks where N is wide
-      const int64_t tiles = total / nib, group = item / (8 * nib), in = item - group * (8 * nib);
-      const int64_t rows = min((int64_t)8, tiles - group * 8);
+      const uint32_t group = item / (8 * nib), in = item - group * (8 * nib), rows = min(8u, ntiles - group * 8);
       ib = in / rows;
       jt = group * 8 + in - ib * rows;
       e = a.te[jt];
@@ -133,7 +130,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
       if (e < 0 || e >= a.E) e = -1;
     }
   }
-  const int64_t i0 = ib * BI, j0 = MODE == DG_WEIGHT ? jt * BJ : 0;
+  const int64_t i0 = (int64_t)ib * BI, j0 = MODE == DG_WEIGHT ? (int64_t)jt * BJ : 0;
   const int64_t kn = MODE == DG_WEIGHT ? count : a.nk;
   const int steps = e < 0 ? 0 : (int)((kn + DG_K - 1) / DG_K);
 
