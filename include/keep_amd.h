@@ -571,6 +571,14 @@ int keep_route_combine_rows(const void* y, int y_dtype, const float* w, int64_t 
 int keep_route_combine_grad(const void* y, int y_dtype, const float* w, const void* dout, int dout_dtype, int64_t T,
                             int64_t k, int64_t H, void* dy, float* dw, void* stream);
 
+/* keep_route_plan for many routes (R >= 1), over several workgroups: the same plan in three launches. The workspace holds
+ * keep_route_plan_blocks_workspace_bytes. */
+int keep_route_plan_blocks(const int32_t* rhs, int64_t R, int64_t E, int64_t tile, int32_t* order, int32_t* inverse,
+                           int32_t* counts, int32_t* offsets, int32_t* tile_expert, int32_t* tile_offset,
+                           int32_t* tile_count, int64_t max_tiles, int32_t* n_tiles_out, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+int64_t keep_route_plan_blocks_workspace_bytes(int64_t R, int64_t E);
+
 /* Routed product with dense expert weights: out[r] = W[rhs[r]] x[row_r] with row_r = lhs[r], or r / x_div without lhs.
  * x [x_rows, K] and weight of one dtype; weight [E, N, K], or with transposed [E, K, N]; out [routes, N]; fp32 sums. A
  * route whose expert or row is out of range gives a NaN row.

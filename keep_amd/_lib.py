@@ -54,6 +54,8 @@ _SIGS = {
     "keep_route_combine": [_P, _P, c_int64, c_int64, c_int64, _P, c_int, _P],
     "keep_route_combine_rows": [_P, c_int, _P, c_int64, c_int64, c_int64, _P, c_int, _P],
     "keep_route_combine_grad": [_P, c_int, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, _P],
+    "keep_route_plan_blocks": [_P, c_int64, c_int64, c_int64, _P, _P, _P, _P, _P, _P, _P, c_int64, _P, _P, c_int64, _P],
+    "keep_route_plan_blocks_workspace_bytes": [c_int64, c_int64],
     "keep_gather_mm": [_P, c_int, c_int64, _P, c_int, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P,
                        _P, _P, _P, _P, c_int64, c_int64, _P, c_int, _P],
     "keep_gather_mm_tile_supported": [c_int, c_int, c_int64, c_int64, c_int64],
@@ -124,7 +126,8 @@ _RESTYPE = {"keep_last_error": c_char_p, "keep_moe_tiles_workspace_bytes": c_int
             "keep_moe_layer1_workspace_bytes": c_int64,
             "keep_vq_grouped_gemm_q8_workspace_bytes": c_int64,
             "keep_lora_workspace_bytes": c_int64, "keep_lora_rank_stride": c_int64,
-            "keep_lora_backward_workspace_bytes": c_int64}
+            "keep_lora_backward_workspace_bytes": c_int64,
+            "keep_route_plan_blocks_workspace_bytes": c_int64}
 EXPORTED = tuple(_SIGS)
 
 _lib = None

@@ -21,6 +21,7 @@ from keep_amd import _grad, _lib, ops
 
 ROUTE_TILE = 16  # routes per tile of the planned kernel
 WINDOW_ROUTES = 128  # routes the kernel groups by itself
+PLAN_BLOCKS_ROUTES = 16384  # routes from which a plan takes several workgroups
 
 
 class _Plan:
@@ -30,7 +31,10 @@ class _Plan:
         R = rhs.numel()
         n = min((R + tile - 1) // tile + groups, R)
         room = (R + tile - 1) // tile + groups
-        self.buffer = torch.empty(2 * R + 2 * groups + 3 * room + 1, dtype=torch.int32, device=rhs.device)
+        lib = _lib.load()
+        blocks = R >= PLAN_BLOCKS_ROUTES
+        scratch = lib.keep_route_plan_blocks_workspace_bytes(R, groups) // 4 if blocks else 0
+        self.buffer = torch.empty(2 * R + 2 * groups + 3 * room + 1 + scratch, dtype=torch.int32, device=rhs.device)
         p = self.buffer.data_ptr()
         self.order, inverse = p, p + 4 * R
         self.counts = p + 8 * R
@@ -41,9 +45,12 @@ class _Plan:
         self.valid_tiles = self.tile_count + 4 * room
         self.n_tiles = n  # descriptors that can hold routes: those come first
         self.tile = tile
-        _lib.call("keep_route_plan", rhs.data_ptr() if R else None, R, groups, tile, self.order if R else None,
-                  inverse if R else None, self.counts, self.offsets, self.tile_expert, self.tile_offset,
-                  self.tile_count, room, self.valid_tiles, ops._stream(rhs.device))
+        args = (rhs.data_ptr(), R, groups, tile, self.order, inverse, self.counts, self.offsets, self.tile_expert,
+                self.tile_offset, self.tile_count, room, self.valid_tiles)
+        if blocks:
+            _lib.call("keep_route_plan_blocks", *args, self.valid_tiles + 4, 4 * scratch, ops._stream(rhs.device))
+        else:
+            _lib.call("keep_route_plan", *args, ops._stream(rhs.device))
 
 
 def _weight_layout(weight: torch.Tensor) -> tuple[torch.Tensor, bool]:

@@ -59,6 +59,17 @@ def test_no_routes_is_a_no_op():
     assert lib.keep_route_combine_grad(None, 0, None, None, 0, 0, 2, 8, None, None, None) == 0
 
 
+@pytest.mark.parametrize("over, msg", [
+    (dict(R=0), "route count"), (dict(E=1025), "E must be"), (dict(tile=0), "tile must be"),
+    (dict(max_tiles=3), "max_tiles"), (dict(ws=None), "null"), (dict(order=None), "null"), (dict(ws_bytes=10), "workspace"),
+])
+def test_plan_over_several_workgroups_refuses(over, msg):
+    args = dict(rhs=16, R=9000, E=4, tile=16, order=16, inverse=16, counts=16, offsets=16, te=16, to=16, tc=16,
+                max_tiles=1000, nt=16, ws=16, ws_bytes=1 << 20, stream=None)
+    assert _lib_call("keep_route_plan_blocks", **{**args, **over}) == _lib.KEEP_EINVAL
+    assert msg in _lib.load().keep_last_error().decode()
+
+
 def _grad_weight(**over):
     args = dict(x=16, dtype=1, x_rows=4, dy=16, routes=4, x_div=1, E=2, N=8, K=16, order=16, offsets=16, counts=16,
                 dw=16, stream=None)

@@ -57,6 +57,7 @@ SHAPES = [
     (900, 3, 2, 512, 320),
     (61, 5, 8, 1024, 64),
     (2000, 40, 1, 64, 1032),
+    (17000, 9, 1, 40, 72),    # a plan over several workgroups
 ]
 
 
@@ -74,6 +75,24 @@ def test_gather_mm_and_its_gradients(dev, dtype, shape):
     assert dx.dtype == dw.dtype == dtype
     want[1].check(dx, "dx")
     want[2].check(dw, "dw")
+
+
+@pytest.mark.parametrize("R, E, tile", [(1, 1, 16), (4096, 3, 64), (4097, 1024, 64), (20000, 7, 256), (70001, 384, 16),
+                                        (33000, 1, 128)])
+def test_plan_over_several_workgroups(dev, R, E, tile):
+    """The single workgroup's plan, array by array, routes out of range included."""
+    from keep_amd import _lib
+    g = torch.Generator(device=dev).manual_seed(R)
+    rhs = torch.randint(-1, E + 1, (R,), device=dev, generator=g, dtype=torch.int32)
+    want = ops.route_plan(rhs, E, tile)
+    got = [torch.full_like(t, -7) for t in want]
+    need = _lib.load().keep_route_plan_blocks_workspace_bytes(R, E)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    order, inverse, counts, offsets, te, to, tc, nt = got
+    _lib.call("keep_route_plan_blocks", rhs.data_ptr(), R, E, tile, *(t.data_ptr() for t in (order, inverse, counts,
+              offsets, te, to, tc)), te.numel(), nt.data_ptr(), ws.data_ptr(), need, ops._stream(dev))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
