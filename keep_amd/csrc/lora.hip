@@ -120,7 +120,7 @@ __device__ __forceinline__ int64_t lora_route(const LoraArgs& a, const LoraTile&
 template <typename T, bool VEC, int RT, int NJ>
 __device__ __forceinline__ void lora_dot(const LoraArgs& a, const LoraTile& t, int64_t s0, int64_t s1, int lane,
                                          f4 (&acc)[NJ][RT]) {
-  constexpr int V = Dense<T>::V, KS = Dense<T>::KS, UN = RT + NJ <= 4 ? 4 : RT + NJ <= 8 ? 2 : 1;
+  constexpr int V = Dense<T>::V, KS = Dense<T>::KS, UN = RT + NJ <= 4 ? 4 : 2;
   const int c = lane & 15, q = lane >> 4;
   const T *xrow[NJ], *arow[RT];
 #pragma unroll
@@ -133,17 +133,32 @@ __device__ __forceinline__ void lora_dot(const LoraArgs& a, const LoraTile& t, i
   }
 #pragma unroll
   for (int u = 0; u < RT; ++u) arow[u] = (const T*)a.a + ((int64_t)t.g * a.R + min((int64_t)(16 * u + c), a.R - 1)) * a.K;
-  const int64_t whole = VEC ? min(s1, a.K / KS) : s0;
-  int64_t s = s0;
-  for (; s + UN <= whole; s += UN) {
+  // UN steps' loads in flight together; past the share's last step, or K's end, zeros on both sides
+  for (int64_t s = s0; s < s1; s += UN) {
     uint4 fi[UN][RT], fj[UN][NJ];
 #pragma unroll
     for (int i = 0; i < UN; ++i) {
-      const int64_t k = (s + i) * KS + q * V;
+      const int64_t k = min(s + i, s1 - 1) * KS + q * V;
+      if constexpr (VEC) {
+        const int64_t kk = min(k, a.K - V);
+        const bool in = s + i < s1 && k < a.K;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) fj[i][j] = dense_ld16(xrow[j], k);
+        for (int j = 0; j < NJ; ++j) {
+          fj[i][j] = dense_ld16(xrow[j], kk);
+          if (!in) fj[i][j] = make_uint4(0u, 0u, 0u, 0u);
+        }
 #pragma unroll
-      for (int u = 0; u < RT; ++u) fi[i][u] = dense_ld16(arow[u], k);
+        for (int u = 0; u < RT; ++u) {
+          fi[i][u] = dense_ld16(arow[u], kk);
+          if (!in) fi[i][u] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      } else {
+        const int64_t n = s + i < s1 ? a.K : 0;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fj[i][j] = dense_ld<T, VEC>(xrow[j], k, n);
+#pragma unroll
+        for (int u = 0; u < RT; ++u) fi[i][u] = dense_ld<T, VEC>(arow[u], k, n);
+      }
     }
 #pragma unroll
     for (int i = 0; i < UN; ++i)
@@ -151,18 +166,6 @@ __device__ __forceinline__ void lora_dot(const LoraArgs& a, const LoraTile& t, i
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int u = 0; u < RT; ++u) acc[j][u] = dense_mfma<T>(fi[i][u], fj[i][j], acc[j][u]);
-  }
-  for (; s < s1; ++s) {
-    const int64_t k = s * KS + q * V;
-    uint4 fi[RT];
-#pragma unroll
-    for (int u = 0; u < RT; ++u) fi[u] = dense_ld<T, VEC>(arow[u], k, a.K);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const uint4 fj = dense_ld<T, VEC>(xrow[j], k, a.K);
-#pragma unroll
-      for (int u = 0; u < RT; ++u) acc[j][u] = dense_mfma<T>(fi[u], fj, acc[j][u]);
-    }
   }
 }
 
@@ -276,9 +279,16 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
         const int64_t tr = lora_route(a, t, row);
         float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
         if (tr >= 0) {
-          for (int64_t sl = 0; sl < a.slices; ++sl) {
-            const float4 p = *(const float4*)(a.ws + (sl * a.routes + tr) * RP + k4);
-            f.x += p.x; f.y += p.y; f.z += p.z; f.w += p.w;
+          for (int64_t sl = 0; sl < a.slices; sl += 4) {  // four loads in flight, added in order
+            float4 p[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+              p[d] = *(const float4*)(a.ws + (min(sl + d, a.slices - 1) * a.routes + tr) * RP + k4);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              if (sl + d >= a.slices) break;
+              f.x += p[d].x; f.y += p[d].y; f.z += p[d].z; f.w += p[d].w;
+            }
           }
           f.x = k4 < a.R ? f.x * sc : 0.f;
           f.y = k4 + 1 < a.R ? f.y * sc : 0.f;
@@ -396,13 +406,16 @@ static int lora_rt(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 :
 static int64_t lora_heads(int64_t routes) { return routes <= 256 ? std::min<int64_t>(routes, 128) : 6; }
 static int64_t lora_blocks(int64_t routes) { return (routes + 127) / 128 * lora_heads(routes); }
 
-// Slices of K: 48 KiB of A each (one row, r = 16 of 4096: 4 slices 9.3 us, 1 12.0; r = 128 of 8192: 16 slices 20, 4 28),
-// while the tiles leave CUs free (64 requests of r = 64: 4 slices 16.4 us, 8 19.4; 4093 rows of r = 32: 4 slices 48, 16
-// 68). Each wave takes at least one step of 64 bytes of a row.
+// Slices of K, a power of two (a wave's steps then come in whole batches): about 40 KiB of A each (one row, r = 16 of 4096:
+// 4 slices 9.3 us, 1 12.0; r = 128 of 8192: 16 slices 20, 4 28), while the tiles leave CUs free (64 requests of r = 64: 4
+// slices 16.4 us, 8 19.4; 4093 rows of r = 32: 4 slices 48, 16 68). Each wave takes at least a step of 64 bytes of a row.
 static int64_t lora_slices(int64_t routes, int64_t R, int64_t K, int size) {
-  const int64_t steps = (K * size + 63) / 64, want = R * K * size / (48 << 10) + 1;
-  const int64_t room = routes <= 256 ? 256 / routes : 640 * 20 / routes;
-  return std::max<int64_t>(1, std::min<int64_t>({want, room, 16, steps / LS_WAVES}));
+  const int64_t steps = (K * size + 63) / 64, want = R * K * size / (40 << 10) + 1;
+  const int64_t room = routes <= 256 ? 256 / routes : 20000 / routes;
+  const int64_t most = std::min<int64_t>({want, room, 16, steps / LS_WAVES});
+  int64_t n = 1;
+  while (2 * n <= most) n *= 2;
+  return n;
 }
 
 template <typename T, typename OT, bool VECK, bool VECR>
