@@ -216,8 +216,8 @@ __global__ __launch_bounds__(64 * LS_WAVES) void k_lora_shrink(LoraArgs a) {
 // A wave takes 64 columns of a tile. Lane (c, q) of product u holds B row 32 (u / 2) + 8 (c / 4) + 4 (u % 2) + c % 4 of
 // them, so that the lane's results over two products are 8 neighbouring columns of route c, and a row's four lanes make
 // 64 bytes of each load and store. (No loop over columns: loads of a second turn would wait for the first one's stores.)
-// OT: base's and out's type. VEC: rows of B, base and out hold whole 16-byte pieces at aligned addresses.
-template <typename T, typename OT, bool VEC, int RT>
+// OT: base's and out's type. VEC, WIDE: rows of B, and of base and out, hold whole 16-byte pieces at aligned addresses.
+template <typename T, typename OT, bool VEC, bool WIDE, int RT>
 __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
   constexpr int V = Dense<T>::V, KS = Dense<T>::KS, RP = 16 * RT, NK = (RP + KS - 1) / KS;
   __shared__ float ts[LORA_ROWS][NK * KS + 4];
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
             fi[i][u] = dense_ld<T, VEC>(bb + n * a.R, r, a.R);
           }
         }
-      if (VEC && a.base) {
+      if (WIDE && a.base) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -356,11 +356,11 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
           for (int u = 0; u < 8; ++u) {
             f[u] = acc[j][2 * p + (u >> 2)][u & 3] * back[j];
             if (a.base) {
-              if constexpr (VEC) f[u] += dense_at<OT>(base[j][p][u / OV], u % OV);
+              if constexpr (WIDE) f[u] += dense_at<OT>(base[j][p][u / OV], u % OV);
               else f[u] += n + u < a.N ? to_float(((const OT*)a.base)[at[j] + n + u]) : 0.f;
             }
           }
-          dense_st<OT, 8>((OT*)a.out + at[j] + n, a.N - n, f, VEC);
+          dense_st<OT, 8>((OT*)a.out + at[j] + n, a.N - n, f, WIDE);
         }
       __syncthreads();  // ts is written again
     };
@@ -401,9 +401,12 @@ __global__ __launch_bounds__(256) void k_lora_transpose(TransposeArgs a) {
 
 static int lora_rt(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }
 
-// Blocks per window: one per position while every row may be a request of its own, else about as many as a window of
-// long runs has tiles.
-static int64_t lora_heads(int64_t routes) { return routes <= 256 ? std::min<int64_t>(routes, 128) : 6; }
+// Blocks per window: one per position while every row may be a request of its own and the windows are few, down to about
+// as many as a window of long runs has tiles (4093 rows in runs of about 100: 6 blocks 48 us, 8 53).
+static int64_t lora_heads(int64_t routes) {
+  const int64_t windows = (routes + 127) / 128;
+  return std::min<int64_t>(std::min<int64_t>(routes, 128), windows <= 2 ? 128 : std::max<int64_t>(6, 192 / windows));
+}
 static int64_t lora_blocks(int64_t routes) { return (routes + 127) / 128 * lora_heads(routes); }
 
 // Slices of K, a power of two (a wave's steps then come in whole batches): about 40 KiB of A each (one row, r = 16 of 4096:
@@ -418,15 +421,17 @@ static int64_t lora_slices(int64_t routes, int64_t R, int64_t K, int size) {
   return n;
 }
 
-template <typename T, typename OT, bool VECK, bool VECR>
-static void lora_launch(LoraArgs a, hipStream_t s) {
+template <typename T, typename OT, bool VECR, bool WIDE>
+static void lora_launch(LoraArgs a, bool veck, hipStream_t s) {
   const int64_t blocks = lora_blocks(a.routes), groups = (a.N + 64 * LE_WAVES - 1) / (64 * LE_WAVES);
   auto go = [&](auto c) {
     constexpr int RT = decltype(c)::value;
     a.split = a.slices;
-    hipLaunchKernelGGL((k_lora_shrink<T, VECK, RT>), dim3((unsigned)(blocks * a.split)), dim3(64 * LS_WAVES), 0, s, a);
+    const dim3 shrink((unsigned)(blocks * a.split));
+    if (veck) hipLaunchKernelGGL((k_lora_shrink<T, true, RT>), shrink, dim3(64 * LS_WAVES), 0, s, a);
+    else hipLaunchKernelGGL((k_lora_shrink<T, false, RT>), shrink, dim3(64 * LS_WAVES), 0, s, a);
     a.split = a.out ? groups : 1;
-    hipLaunchKernelGGL((k_lora_expand<T, OT, VECR, RT>), dim3((unsigned)(blocks * a.split)), dim3(64 * LE_WAVES), 0, s, a);
+    hipLaunchKernelGGL((k_lora_expand<T, OT, VECR, WIDE, RT>), dim3((unsigned)(blocks * a.split)), dim3(64 * LE_WAVES), 0, s, a);
   };
   const int rt = lora_rt(a.R);
   if (rt == 1) go(std::integral_constant<int, 1>{});
@@ -436,13 +441,13 @@ static void lora_launch(LoraArgs a, hipStream_t s) {
 }
 
 template <typename T>
-static void lora_pick(const LoraArgs& a, bool out_float, bool vk, bool vr, hipStream_t s) {
+static void lora_pick(const LoraArgs& a, bool out_float, bool vk, bool vr, bool wide, hipStream_t s) {
   auto go = [&](auto ot) {
     typedef decltype(ot) OT;
-    if (vk && vr) lora_launch<T, OT, true, true>(a, s);
-    else if (vk) lora_launch<T, OT, true, false>(a, s);
-    else if (vr) lora_launch<T, OT, false, true>(a, s);
-    else lora_launch<T, OT, false, false>(a, s);
+    if (vr && wide) lora_launch<T, OT, true, true>(a, vk, s);
+    else if (vr) lora_launch<T, OT, true, false>(a, vk, s);
+    else if (wide) lora_launch<T, OT, false, true>(a, vk, s);
+    else lora_launch<T, OT, false, false>(a, vk, s);
   };
   if (out_float) go(float{});
   else go(T{});
@@ -473,6 +478,12 @@ struct LoraPlan {
 
 static int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
 
+// Whether every size in bytes that these sizes make fits 63 bits with room (dims_ok and the rank's range are checked first).
+static bool lora_sizes_ok(int64_t routes, int64_t n, int64_t rank, int64_t K, int64_t N) {
+  const int64_t most = int64_t(1) << 46, width = std::max<int64_t>({K, N, 1});
+  return n <= most / (rank * width) && routes <= most / width;
+}
+
 static int64_t lora_partials(int dtype, int64_t routes, int64_t rank, int64_t K) {
   return round256(lora_slices(routes, rank, K, dtype_size(dtype)) * routes * 16 * lora_rt(rank) * 4);
 }
@@ -482,11 +493,12 @@ static void lora_run(LoraArgs p, int dtype, int out_dtype, hipStream_t s) {
   p.heads = (int)lora_heads(p.routes);
   p.slices = lora_slices(p.routes, p.R, p.K, (int)size);
   const bool vk = p.K % v == 0 && aligned(p.x, 16) && aligned(p.a, 16);
-  const bool vr = p.R % v == 0 && p.N % 8 == 0 && aligned(p.b, 16) && aligned(p.base, 16) && aligned(p.out, 16);
+  const bool vr = p.R % v == 0 && aligned(p.b, 16);
+  const bool w = p.N % 8 == 0 && aligned(p.base, 16) && aligned(p.out, 16);
   const bool f = out_dtype == KEEP_F32;
-  if (dtype == KEEP_F32) lora_pick<float>(p, f, vk, vr, s);
-  else if (dtype == KEEP_F16) lora_pick<_Float16>(p, f, vk, vr, s);
-  else lora_pick<bf16s>(p, f, vk, vr, s);
+  if (dtype == KEEP_F32) lora_pick<float>(p, f, vk, vr, w, s);
+  else if (dtype == KEEP_F16) lora_pick<_Float16>(p, f, vk, vr, w, s);
+  else lora_pick<bf16s>(p, f, vk, vr, w, s);
 }
 
 static int lora_check(int dtype, int64_t x_rows, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank,
@@ -495,6 +507,7 @@ static int lora_check(int dtype, int64_t x_rows, int64_t routes, int64_t x_div, 
   KEEP_REQUIRE(dtype_ok(dtype), "bad dtype enum");
   KEEP_REQUIRE(rank >= 1 && rank <= 128, "rank must be in 1..128");
   KEEP_REQUIRE(adapters > 0 && K > 0 && N > 0 && x_div > 0, "adapters, K, N and x_div must be positive");
+  KEEP_REQUIRE(lora_sizes_ok(routes, adapters, rank, K, N), "too many values");
   KEEP_REQUIRE(!grouped || adapters <= 1024, "a plan holds at most 1024 adapters");
   KEEP_REQUIRE(routes == 0 || (routes - 1) / x_div < x_rows, "x holds %lld rows, %lld routes need more",
                (long long)x_rows, (long long)routes);
@@ -511,7 +524,9 @@ extern "C" int64_t keep_lora_rank_stride(int64_t rank) { return rank >= 1 && ran
 
 extern "C" int64_t keep_lora_workspace_bytes(int dtype, int64_t routes, int64_t adapters, int64_t rank, int64_t K,
                                              int grouped) {
-  if (!dtype_ok(dtype) || !dims_ok({routes, adapters, rank, K}) || rank < 1 || rank > 128 || routes == 0) return 0;
+  if (!dtype_ok(dtype) || !dims_ok({routes, adapters, rank, K}) || rank < 1 || rank > 128 || routes == 0 ||
+      !lora_sizes_ok(routes, adapters, rank, K, 1))
+    return 0;
   return lora_partials(dtype, routes, rank, K) + (grouped ? LoraPlan::bytes(routes, adapters) : 0);
 }
 
@@ -564,7 +579,9 @@ struct LoraBackward {
 
 extern "C" int64_t keep_lora_backward_workspace_bytes(int dtype, int64_t routes, int64_t x_div, int64_t adapters,
                                                       int64_t rank, int64_t K, int64_t N, int dx, int planned) {
-  if (!dtype_ok(dtype) || !dims_ok({routes, x_div, adapters, rank, K, N}) || rank < 1 || rank > 128 || routes == 0) return 0;
+  if (!dtype_ok(dtype) || !dims_ok({routes, x_div, adapters, rank, K, N}) || rank < 1 || rank > 128 ||
+      routes == 0 || !lora_sizes_ok(routes, adapters, rank, K, N))
+    return 0;
   return LoraBackward(dtype, routes, x_div, adapters, rank, K, N, dx, planned).total;
 }
 

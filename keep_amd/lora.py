@@ -21,7 +21,7 @@ from keep_amd import _grad, _lib, ops
 MAX_RANK = 128
 # Routes (2D indices) from which a plan brings the routes of one adapter together first: rows of a request lie together
 # as they are, its routes' experts do not.
-PLANNED_ROUTES = 512
+PLANNED_ROUTES = 256
 
 
 def _forward(x, a, b, scales, idx, x_div: int, base, out_dtype, t_out=None) -> torch.Tensor:
