@@ -57,6 +57,7 @@ SHAPES = [
     (900, 3, 2, 512, 320),
     (61, 5, 8, 1024, 64),
     (2000, 40, 1, 64, 1032),
+    (400, 3, 2, 8, 8),        # less than one step of the summed index
     (17000, 9, 1, 40, 72),    # a plan over several workgroups
 ]
 
@@ -228,6 +229,27 @@ def test_gather_mm_beyond_32_bit_offsets(dev):
     want[1].check(dx)
     want[2].check(dw[-1:])
     assert (dw[:-1].abs().amax(dim=(1, 2)) == 0).all()
+
+
+def test_gather_mm_rows_of_more_than_4_gib(dev):
+    """x past 2^31 values: the products through LDS leave their 32-bit offsets."""
+    T, K, N = 262_200, 8192, 64
+    x = torch.zeros(T, K, device=dev, dtype=torch.bfloat16)
+    last, w, idx, dy = _case(dev, torch.bfloat16, 40, 2, 1, N, K, seed=4)
+    x[-40:] = last
+    want = _expected(last, w, idx, dy)
+    full = torch.zeros(T, 1, device=dev, dtype=torch.int32)
+    full[-40:] = idx
+    x.requires_grad_(True), w.requires_grad_(True)
+    out = keep_amd.gather_mm(x, w, full)
+    want[0].check(out[-40:], "out")
+    assert (out[:1000] == 0).all()
+    g = torch.zeros(T, 1, N, device=dev, dtype=torch.bfloat16)
+    g[-40:] = dy
+    dx, dw = torch.autograd.grad(out, (x, w), g)
+    want[1].check(dx[-40:], "dx")
+    assert (dx[:1000] == 0).all()
+    want[2].check(dw, "dw")
 
 
 def _replays(fn, inputs, others):
