@@ -28,10 +28,15 @@ struct GatherArgs {
   int64_t routes, x_div;
   int64_t E, N, K;
   const int32_t *order, *te, *to, *tc;  // tiles of a route plan (null: grouped here, in windows)
-  int64_t strips;
+  int64_t tiles;
   void* out;
   int odt;
 };
+
+// A block's tile: strips of outputs along x, tiles along y and z (a launch holds 2^32 threads along x, 65535 blocks along
+// y and z).
+constexpr int64_t GATHER_Y = 32768;
+__device__ __forceinline__ int64_t gather_block() { return (int64_t)blockIdx.z * GATHER_Y + blockIdx.y; }
 
 // The routes of a block's tile: lane c's route (-1: none), its x row (0 where there is none), whether its row is valid.
 struct GatherTile {
@@ -42,6 +47,7 @@ struct GatherTile {
 
 __device__ __forceinline__ GatherTile gather_tile(const GatherArgs& a, int64_t tile, int lane) {
   GatherTile t{0, -1, -1, 0, false};
+  if (tile >= a.tiles) return t;
   const int c = lane & 15;
   if (a.te) {
     t.count = min(16, a.tc[tile]);
@@ -74,68 +80,59 @@ __device__ __forceinline__ void gather_store(const GatherArgs& a, int64_t at, in
   else dense_st<_Float16, 4>((_Float16*)a.out + at, left, f, vec);
 }
 
-// Eight waves share a tile's rows against 16 NT rows of W: wave s takes the s-th share of K and the shares are added in
-// order through LDS. Lane (c, q) of product u holds W row n0 + 4 NT (c / 4) + 4 u + c % 4, so that its results are
-// outputs n0 + 4 NT q + 4 u + v of route c.
+// Eight waves share a tile's rows against 16 rows of W: wave s takes the s-th share of K and the shares are added in order
+// through LDS. Lane (c, q) holds W row n0 + c, so that its results are outputs n0 + 4 q + v of route c.
+//
+// Bound by the bytes of W of the experts that are hit (a byte of W serves at most 16 routes, far below the matrix cores'
+// rate): one token of 6 experts, fp16 4096 -> 2048, 101 MB in 18.7 us, 5.4 TB/s; eight tokens, bf16, 743 MB of
+// weights in 124 us, 6.0 TB/s. Eight loads per wave are in flight; the fine strips (16 outputs) are what
+// fills 256 CUs with a token's few tiles.
 constexpr int GF_WAVES = 8;
 
-template <typename T, bool VEC, int NT>
+template <typename T, bool VEC>
 __global__ __launch_bounds__(64 * GF_WAVES) void k_gather_few(GatherArgs a) {
-  constexpr int V = Dense<T>::V, KS = Dense<T>::KS, UN = NT == 1 ? 8 : 4;
-  __shared__ float4 red[GF_WAVES][NT][64];
+  constexpr int V = Dense<T>::V, KS = Dense<T>::KS, UN = 8;
+  __shared__ float4 red[GF_WAVES][64];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int64_t tile = blockIdx.x / a.strips, strip = blockIdx.x - tile * a.strips;
-  const GatherTile t = gather_tile(a, tile, lane);
+  const GatherTile t = gather_tile(a, gather_block(), lane);
   if (t.count == 0) return;
-  const int64_t n0 = strip * (16 * NT);
-  f4 acc[NT];
-#pragma unroll
-  for (int u = 0; u < NT; ++u) acc[u] = f4{0.f, 0.f, 0.f, 0.f};
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  f4 acc{0.f, 0.f, 0.f, 0.f};
   if (t.e >= 0) {
     const T* xrow = (const T*)a.x + t.xr * a.K;  // lanes without a route read row 0's: their results are not stored
-    const T* wrow[NT];
-#pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int64_t n = min(n0 + (c >> 2) * (4 * NT) + u * 4 + (c & 3), a.N - 1);
-      wrow[u] = (const T*)a.w + (t.e * a.N + n) * a.K;
-    }
+    const T* wrow = (const T*)a.w + (t.e * a.N + min(n0 + c, a.N - 1)) * a.K;
     const int64_t steps = (a.K + KS - 1) / KS, per = (steps + GF_WAVES - 1) / GF_WAVES;
     const int64_t s0 = min(steps, wv * per), s1 = min(steps, s0 + per);
     int64_t s = s0;
     const int64_t whole = VEC ? min(s1, a.K / KS) : s0;  // steps with no end inside
     for (; s + UN <= whole; s += UN) {
-      uint4 fi[UN][NT], fj[UN];
+      uint4 fi[UN], fj[UN];
 #pragma unroll
       for (int d = 0; d < UN; ++d) {
         const int64_t k = (s + d) * KS + q * V;
-#pragma unroll
-        for (int u = 0; u < NT; ++u) fi[d][u] = dense_ld16(wrow[u], k);
+        fi[d] = dense_ld16(wrow, k);
         fj[d] = dense_ld16(xrow, k);
       }
 #pragma unroll
-      for (int d = 0; d < UN; ++d)
-#pragma unroll
-        for (int u = 0; u < NT; ++u) acc[u] = dense_mfma<T>(fi[d][u], fj[d], acc[u]);
+      for (int d = 0; d < UN; ++d) acc = dense_mfma<T>(fi[d], fj[d], acc);
     }
     for (; s < s1; ++s) {
       const int64_t k = s * KS + q * V;
       const uint4 fj = dense_ld<T, VEC>(xrow, k, a.K);
-#pragma unroll
-      for (int u = 0; u < NT; ++u) acc[u] = dense_mfma<T>(dense_ld<T, VEC>(wrow[u], k, a.K), fj, acc[u]);
+      acc = dense_mfma<T>(dense_ld<T, VEC>(wrow, k, a.K), fj, acc);
     }
   }
-#pragma unroll
-  for (int u = 0; u < NT; ++u) red[wv][u][lane] = make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
+  red[wv][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
-  if (wv >= NT) return;
+  if (wv > 0) return;
   float f[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int w = 0; w < GF_WAVES; ++w) {
-    const float4 p = red[w][wv][lane];
+    const float4 p = red[w][lane];
     f[0] += p.x; f[1] += p.y; f[2] += p.z; f[3] += p.w;
   }
-  const int64_t n = n0 + q * (4 * NT) + wv * 4;
+  const int64_t n = n0 + q * 4;
   if (t.route < 0 || n >= a.N) return;
   if (!t.ok)
 #pragma unroll
@@ -152,9 +149,8 @@ __global__ __launch_bounds__(64 * GT_WAVES) void k_gather_trans(GatherArgs a) {
   constexpr int V = Dense<T>::V, KS = Dense<T>::KS;
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int64_t tile = blockIdx.x / a.strips, strip = blockIdx.x - tile * a.strips;
-  const GatherTile t = gather_tile(a, tile, lane);
-  const int64_t n0 = (strip * GT_WAVES + wv) * (16 * V);
+  const GatherTile t = gather_tile(a, gather_block(), lane);
+  const int64_t n0 = ((int64_t)blockIdx.x * GT_WAVES + wv) * (16 * V);
   if (t.count == 0 || n0 >= a.N) return;
   f4 acc[V];
 #pragma unroll
@@ -311,19 +307,18 @@ int rows_outer(const OuterArgs& a, int dtype, bool j_float, int64_t groups, hipS
 // ------------------------------------------------------------------ host side
 
 template <typename T>
-static void gather_launch(GatherArgs a, int64_t tiles, bool transposed, bool vec, hipStream_t s) {
+static void gather_launch(const GatherArgs& a, bool transposed, bool vec, hipStream_t s) {
   constexpr int V = Dense<T>::V;
+  const int64_t strip = transposed ? 16 * V * GT_WAVES : 16;
+  const dim3 grid((unsigned)((a.N + strip - 1) / strip), (unsigned)std::min(a.tiles, GATHER_Y),
+                  (unsigned)((a.tiles + GATHER_Y - 1) / GATHER_Y));
   if (transposed) {
-    a.strips = (a.N + 16 * V * GT_WAVES - 1) / (16 * V * GT_WAVES);
-    const dim3 grid((unsigned)(tiles * a.strips));
     if (vec) hipLaunchKernelGGL((k_gather_trans<T, true>), grid, dim3(64 * GT_WAVES), 0, s, a);
     else hipLaunchKernelGGL((k_gather_trans<T, false>), grid, dim3(64 * GT_WAVES), 0, s, a);
     return;
   }
-  a.strips = (a.N + 15) / 16;
-  const dim3 grid((unsigned)(tiles * a.strips));
-  if (vec) hipLaunchKernelGGL((k_gather_few<T, true, 1>), grid, dim3(64 * GF_WAVES), 0, s, a);
-  else hipLaunchKernelGGL((k_gather_few<T, false, 1>), grid, dim3(64 * GF_WAVES), 0, s, a);
+  if (vec) hipLaunchKernelGGL((k_gather_few<T, true>), grid, dim3(64 * GF_WAVES), 0, s, a);
+  else hipLaunchKernelGGL((k_gather_few<T, false>), grid, dim3(64 * GF_WAVES), 0, s, a);
 }
 
 }  // namespace keep
@@ -362,8 +357,8 @@ extern "C" int keep_gather_mm(const void* x, int dtype, int64_t x_rows, const vo
   a.E = num_experts; a.N = N; a.K = K;
   a.order = order; a.te = tile_expert; a.to = tile_offset; a.tc = tile_count;
   a.out = out; a.odt = out_dtype;
-  const int64_t tiles = order ? n_tiles : routes;
-  KEEP_REQUIRE(tiles <= 0x7ffffff0LL / ((N + 15) / 16), "too many outputs");
+  a.tiles = order ? n_tiles : routes;
+  KEEP_REQUIRE(a.tiles <= 65535 * GATHER_Y && (N + 15) / 16 <= 0xffffffffLL / (64 * GF_WAVES), "too many outputs");
   if (gemm) {
     KEEP_REQUIRE(aligned(x, 16) && aligned(weight, 16) && (out_dtype == dtype || out_dtype == KEEP_F32),
                  "tiles of %lld routes need x and weight 16-byte aligned, and an output of x's dtype or float32",
@@ -380,9 +375,9 @@ extern "C" int keep_gather_mm(const void* x, int dtype, int64_t x_rows, const vo
   const bool vec = K % v == 0 && (!transposed || N % v == 0) && aligned(x, 16) && aligned(weight, 16) &&
                    aligned(out, 16);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == KEEP_F32) gather_launch<float>(a, tiles, transposed, vec, s);
-  else if (dtype == KEEP_F16) gather_launch<_Float16>(a, tiles, transposed, vec, s);
-  else gather_launch<bf16s>(a, tiles, transposed, vec, s);
+  if (dtype == KEEP_F32) gather_launch<float>(a, transposed, vec, s);
+  else if (dtype == KEEP_F16) gather_launch<_Float16>(a, transposed, vec, s);
+  else gather_launch<bf16s>(a, transposed, vec, s);
   return launch_status("keep_gather_mm");
 }
 

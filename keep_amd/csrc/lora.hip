@@ -35,6 +35,7 @@ namespace keep {
 
 constexpr int LS_WAVES = 8, LE_WAVES = 8;
 constexpr int LORA_ROWS = 32;  // of a tile
+constexpr int64_t LORA_BLOCKS = 0xffffffffLL / (64 * LS_WAVES);  // a launch holds 2^32 threads
 
 struct LoraArgs {
   const void* x;
@@ -511,7 +512,7 @@ static int lora_check(int dtype, int64_t x_rows, int64_t routes, int64_t x_div, 
   KEEP_REQUIRE(!grouped || adapters <= 1024, "a plan holds at most 1024 adapters");
   KEEP_REQUIRE(routes == 0 || (routes - 1) / x_div < x_rows, "x holds %lld rows, %lld routes need more",
                (long long)x_rows, (long long)routes);
-  KEEP_REQUIRE(routes == 0 || lora_blocks(routes) <= 0x7fffffffLL / std::max<int64_t>(16, (std::max(N, K) + 511) / 512),
+  KEEP_REQUIRE(routes == 0 || lora_blocks(routes) <= LORA_BLOCKS / std::max<int64_t>(16, (std::max(N, K) + 511) / 512),
                "too many outputs");
   return KEEP_OK;
 }
@@ -614,7 +615,7 @@ extern "C" int keep_lora_backward(const void* x, int dtype, int64_t x_rows, cons
     TransposeArgs tr{{b, a}, {ws + w.bt, ws + w.at}, {N, rank}, {rank, K}, {0, 0}};
     for (int m = 0; m < 2; ++m) tr.blocks[m] = adapters * ((tr.P[m] + 63) / 64) * ((tr.Q[m] + 63) / 64);
     if (!dx) tr.blocks[1] = 0;
-    KEEP_REQUIRE(tr.blocks[0] + tr.blocks[1] <= 0x7fffffffLL, "too many factors");
+    KEEP_REQUIRE(tr.blocks[0] + tr.blocks[1] <= 2 * LORA_BLOCKS, "too many factors");
     const dim3 grid((unsigned)(tr.blocks[0] + tr.blocks[1]));
     if (size == 4) hipLaunchKernelGGL(k_lora_transpose<uint32_t>, grid, dim3(256), 0, s, tr);
     else hipLaunchKernelGGL(k_lora_transpose<uint16_t>, grid, dim3(256), 0, s, tr);
