@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 _EAGER = "keep_amd: eager graph"
-_VIEWS = {n + "Backward0" for n in ("View", "UnsafeView", "ReshapeAlias", "Transpose", "Permute", "Select", "Slice")}
+_STEPS = 6  # views, casts and the like between a leaf and a call's argument
 
 
 def wanted(*tensors) -> bool:
@@ -18,20 +18,33 @@ def wanted(*tensors) -> bool:
     return False
 
 
+def _leaf_node(node):
+    """The gradient node of the leaf that ``node``'s graph reads alone (a parameter, its view or cast), or None."""
+
+    for _ in range(_STEPS):
+        if node is None or hasattr(node, "variable"):
+            return node
+        following = [f for f, _ in node.next_functions if f is not None]
+        if len(following) != 1:
+            return None
+        node = following[0]
+    return None
+
+
 def check_capture(*tensors) -> None:
     """Refuse to record a graph capture of a call on leaves that a live eager graph of these operators holds.
 
     A leaf has one gradient node at a time, bound to the stream that made it. While an eager graph is alive, a
     backward pass under capture would make that other stream wait on the capturing one, which ends the process. Eager
-    calls leave a mark on the node (``mark``), which lives as long as some graph holds it."""
+    calls leave a mark on the node (``mark``), which lives as long as some graph holds it. Leaves are found through
+    views, casts and other steps of one input."""
 
     if not torch.cuda.is_current_stream_capturing():
         return
     for t in tensors:
-        if t is not None and t.requires_grad and not t.is_leaf and t._is_view():
-            t = t._base
-        if t is not None and t.requires_grad and t.is_leaf:
-            if _EAGER in torch.autograd.graph.get_gradient_edge(t).node.metadata:
+        if t is not None and t.requires_grad:
+            node = _leaf_node(torch.autograd.graph.get_gradient_edge(t).node)
+            if node is not None and _EAGER in node.metadata:
                 raise RuntimeError("graph capture of a differentiable call on a leaf that an eager graph still holds: "
                                    "drop that graph's outputs first, or capture on leaves of its own")
 
@@ -41,8 +54,7 @@ def mark(out: torch.Tensor) -> torch.Tensor:
 
     if not torch.cuda.is_current_stream_capturing():
         for node, _ in out.grad_fn.next_functions:
-            while node is not None and node.name() in _VIEWS:
-                node = node.next_functions[0][0]
-            if node is not None and hasattr(node, "variable"):  # a leaf's
+            node = _leaf_node(node)
+            if node is not None:
                 node.metadata[_EAGER] = True
     return out

@@ -431,3 +431,17 @@ def test_switch_linear_layouts_and_bias(dev, dtype):
         assert torch.equal(lin(x, idx[..., i]), y[:, :, i])
     flat = keep_amd.gather_mm(x.reshape(6, 32), w, idx.reshape(6, 2)).view(2, 3, 2, 24)
     assert torch.equal(y, flat + b[idx.long()])
+
+
+@pytest.mark.parametrize("between", [lambda w: w.bfloat16(), lambda w: (w * 2).bfloat16().transpose(1, 2).contiguous().mT])
+def test_capture_is_refused_through_a_cast_too(dev, between):
+    x, w, idx, _ = _case(dev, torch.float32, 6, 6, 2, 48, 64)
+    x, master = x.bfloat16(), w.requires_grad_(True)
+    held = keep_amd.gather_mm(x, between(master), idx)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(g):
+            torch.zeros(1, device=dev)
+            keep_amd.gather_mm(x, between(master), idx)
+    del held
+    assert torch.isfinite(keep_amd.gather_mm(x, between(master), idx)).all()
