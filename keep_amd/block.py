@@ -72,7 +72,7 @@ def combine_add(routed: torch.Tensor, shared: torch.Tensor | None = None, residu
     term's gradient is the output's, in its dtype."""
 
     from keep_amd import _grad
-    from keep_amd.ops import _DT
+    from keep_amd.ops import _DT, _on
 
     if routed.dtype != torch.float32 or not routed.is_cuda:
         raise ValueError("routed must be a float32 device tensor")
@@ -80,10 +80,11 @@ def combine_add(routed: torch.Tensor, shared: torch.Tensor | None = None, residu
         if t is not None and (tuple(t.shape) != tuple(routed.shape) or t.dtype not in _DT):
             raise ValueError(f"{name} must match routed's shape {tuple(routed.shape)} in a float dtype")
     od = out_dtype or (residual.dtype if residual is not None else torch.float32)
-    if _grad.wanted(routed, shared, residual):
+    with _on(routed.device):
+        if not _grad.wanted(routed, shared, residual):
+            return _combine_add(routed, shared, residual, od)
         _grad.check_capture(routed, shared, residual)
         return _grad.mark(_CombineAdd.apply(routed, shared, residual, od))
-    return _combine_add(routed, shared, residual, od)
 
 
 def _combine_add(routed, shared, residual, od: torch.dtype) -> torch.Tensor:

@@ -724,14 +724,13 @@ def route_combine(y: torch.Tensor, weight: torch.Tensor, out_dtype: torch.dtype 
     if weight.device != y.device:
         raise ValueError(f"tensors must be on one device, found {y.device} and {weight.device}")
     weight = weight.reshape(T, k)
-    if _grad.wanted(y, weight):
-        _dense_device(y)
+    with _on(_dense_device(y)):
+        if not _grad.wanted(y, weight):
+            return _combine_rows(y.contiguous(), weight.float().contiguous(), od)
         if od not in _DT:
             raise ValueError(f"unsupported output dtype {od}")
         _grad.check_capture(y, weight)
-        with _on(y.device):
-            return _grad.mark(_RouteCombine.apply(y, weight, od))
-    return _combine_rows(y.contiguous(), weight.float().contiguous(), od)
+        return _grad.mark(_RouteCombine.apply(y, weight, od))
 
 
 def gemm_eligible(*, code_bits: int, x_dtype: torch.dtype, input_dims: int, group_size: int) -> bool:
