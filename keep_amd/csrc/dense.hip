@@ -192,7 +192,9 @@ __global__ __launch_bounds__(64 * GT_WAVES) void k_gather_trans(GatherArgs a) {
 
 // Lane (c, q) of a step holds four neighbouring values of row 4 s + q of the wide side and one value per 16 of the narrow
 // side; product (u, b) takes value u. Eight waves take every eighth run of 32 routes, whose ids a lane each loads once, so
-// that a run's rows are all in flight together; the waves are added in order through LDS.
+// that a run's rows are all in flight together; the waves are added in order through LDS. NB: 16-wide pieces of the narrow
+// side, one where a second would be empty. Bound by the wait for a run's rows: 2048 routes of 8 adapters, r = 16, 8.3 to
+// 11.7 us a factor (4096 or 2048 wide, bf16), 37 with one wave a block and a route id per step.
 constexpr int RO_WAVES = 8, RO_V = 4, RO_RUN = 32, RO_UN = RO_RUN / 4;
 
 template <typename T, bool VEC>
@@ -358,7 +360,9 @@ extern "C" int keep_gather_mm(const void* x, int dtype, int64_t x_rows, const vo
   a.order = order; a.te = tile_expert; a.to = tile_offset; a.tc = tile_count;
   a.out = out; a.odt = out_dtype;
   a.tiles = order ? n_tiles : routes;
-  KEEP_REQUIRE(a.tiles <= 65535 * GATHER_Y && (N + 15) / 16 <= 0xffffffffLL / (64 * GF_WAVES), "too many outputs");
+  KEEP_REQUIRE(a.tiles <= 65535 * GATHER_Y && (N + 15) / 16 <= 0xffffffffLL / (64 * GF_WAVES) &&
+                   routes <= (int64_t(1) << 40) / N,  // (a value each of 2^40: more than a GPU holds)
+               "too many outputs");
   if (gemm) {
     KEEP_REQUIRE(aligned(x, 16) && aligned(weight, 16) && (out_dtype == dtype || out_dtype == KEEP_F32),
                  "tiles of %lld routes need x and weight 16-byte aligned, and an output of x's dtype or float32",

@@ -19,7 +19,8 @@
 //
 // Bound: the dependent loads at a block's start (window, partial sums, rows).
 // One row, r = 16, 4096 -> 4096: 9.3 us of which two empty launches take about
-// 5; 4093 rows in runs of about 100, r = 32: 48 us, the bytes alone 21.
+// 5; 64 requests of r = 64, 4096 -> 2048: 17 us, the bytes alone 7; 4093 rows in
+// runs of about 100, r = 32, 4096 -> 4096: 48 us (17 + 31), the bytes alone 21.
 //
 // t enters the second product in the rows' 16-bit type (one rounding, half a
 // step of that type relative to the row's largest t), each row times a power of

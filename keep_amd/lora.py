@@ -20,7 +20,9 @@ from keep_amd import _grad, _lib, ops
 
 MAX_RANK = 128
 # Routes (2D indices) from which a plan brings the routes of one adapter together first: rows of a request lie together
-# as they are, its routes' experts do not.
+# as they are, its routes' experts do not. Microseconds without and with one, routes of random adapters, bf16: 32 adapters of
+# r = 16, 2048 -> 1024: 128 routes 10 / 15, 256 12 / 19, 512 25 / 19, 4096 126 / 28; 64 of r = 32, 4096 -> 2048: 128 routes
+# 15 / 18, 256 27 / 25, 512 53 / 27, 4096 303 / 50.
 PLANNED_ROUTES = 256
 
 
@@ -131,7 +133,8 @@ def gather_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, ind
 
 class LoraAdapters:
     """The adapters of one layer, a row of factors per adapter: ``a [n, r, K]``, ``b [n, N, r]`` for a dense
-    projection; ``a [n, E, r, K]``, ``b [n, E, N, r]`` for routed experts. ``scales [n]`` (e.g. alpha / r)."""
+    projection; ``a [n, E, r, K]``, ``b [n, E, N, r]`` for routed experts. ``scales [n]`` (e.g. alpha / r);
+    routed experts' are copied here, once."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor | None = None):
         if a.ndim not in (3, 4) or b.ndim != a.ndim or a.shape[:-2] != b.shape[:-2] or a.shape[-2] != b.shape[-1]:
