@@ -17,6 +17,19 @@
 // as it is too, rows of the tile's width, and read with the transposing LDS
 // loads (four rows of 16 columns a time), its 32-byte pairs permuted likewise.
 // Past an operand's end, lanes copy a zero instead.
+//
+// Bound by the matrix cores: a step of a 256 x 256 tile reads 64 KiB of LDS
+// copies for 2^23 multiply-adds, and its waves read each fragment from LDS two
+// (I) or four (J) times, half a step ahead of its products (no bank conflicts by
+// the counter). Measured, bf16: 8192 x 8192 x 8192 forward 854 to 880 us
+// (1250 to 1290 TFLOP/s), dx 1219 to 1275 TFLOP/s, dW about 1100; 65536 routes
+// of 32 experts, 4096 -> 2048, 1045 us (1052). Of a tile of 4096 summed values about 11 us are
+// its first copies and its stores; the last round of tiles fills part of the CUs.
+// Eight waves of 64 x 128 results each and four of 128 x 128 hold the same tile:
+// the eight hide each other's waits. Tiles in turn on a resident workgroup, the
+// next one's copies under the stores, took 66 to 86 registers more than there are.
+// Below about 48 routes an expert the weights' bytes bound it: 256 x 64 tiles
+// stream 384 experts of 4096 -> 2048 (6.4 GB) in 1.1 to 1.23 ms, 5.3 to 5.8 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -82,17 +95,24 @@ __device__ __forceinline__ void dg_dma(const void* base, uint32_t off, uint32_t 
                : "memory");
 }
 
+// Row tiles that an XCD takes in turn (0: a contiguous run of all items). With few routes an expert most tiles read weights
+// of their own, and an XCD whose run has experts of several tiles is done early: 384 experts of 4096 -> 2048, 8192 routes
+// 1213 us in runs, 1110 in turns of 2 (1, 4: the same); 12288 routes of Zipf popularity 1293 against 1226; 64 experts of
+// 2048 -> 768 38.5 against 40. Large tiles share operands with their neighbours instead.
+constexpr int dg_turn(int bj) { return bj == 64 ? 2 : 0; }
+
 template <typename T, int BI, int BJ, int WI, int WJ, int MODE>
 __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
   constexpr int NT = 64 * WI * WJ, TI = BI / WI, TJ = BJ / WJ, FI = TI / 16, FJ = TJ / 16;
   constexpr int LI = BI * 8 / NT, LJ = BJ * 8 / NT;  // 16-byte copies per thread and step
   constexpr int SI = BI * 128, SJ = BJ * 128;        // bytes of a buffer's operands
   constexpr bool TRI = MODE != DG_FORWARD, TRJ = MODE == DG_WEIGHT;
+  constexpr int G = dg_turn(BJ);
   __shared__ __attribute__((aligned(16))) char smem[2 * (SI + SJ)];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wv % WI, wj = wv / WI;
 
-  // work item: (j tile or expert and row block, i block), dealt to the XCDs in contiguous runs
+  // work item: (j tile or expert and row block, i block)
   int64_t e;
   uint32_t jt, ib;
   int count = 0;
@@ -108,8 +128,13 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
       ntiles = (uint32_t)min(a.n_tiles[0] + (a.routes - valid + BJ - 1) / BJ, a.max_tiles);
       total = ntiles * nib;
     }
-    const uint32_t per = (total + 7) / 8, slot = blockIdx.x >> 3, item = (blockIdx.x & 7) * per + slot;
-    if (slot >= per || item >= total) return;
+    const uint32_t slot = blockIdx.x >> 3, xcd = blockIdx.x & 7;
+    uint32_t item = 0;  // dealt to the XCDs in contiguous runs, or in turns of G row tiles
+    if constexpr (G == 0) {
+      const uint32_t per = (total + 7) / 8;
+      item = xcd * per + slot;
+      if (slot >= per || item >= total) return;
+    }
     if constexpr (MODE == DG_WEIGHT) {
       const uint32_t njb = (uint32_t)((a.nj + BJ - 1) / BJ), ex = item / (njb * nib), r = item - ex * (njb * nib);
       jt = r / nib;
@@ -120,9 +145,18 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_dense_gemm(DenseGemmArgs a) {
     } else {
       // groups of up to 8 row tiles, within a group column block by column block: the 32 items that an XCD's CUs work on
       // share 8 + 4 operand blocks where N is wide
-      const uint32_t group = item / (8 * nib), in = item - group * (8 * nib), rows = min(8u, ntiles - group * 8);
-      ib = in / rows;
-      jt = group * 8 + in - ib * rows;
+      if constexpr (G == 0) {
+        const uint32_t group = item / (8 * nib), in = item - group * (8 * nib), rows = min(8u, ntiles - group * 8);
+        ib = in / rows;
+        jt = group * 8 + in - ib * rows;
+      } else {
+        const uint32_t turn = slot / (G * nib), in = slot - turn * (G * nib), j = (turn * 8 + xcd) * G;
+        if (j >= ntiles) return;
+        const uint32_t rows = min((uint32_t)G, ntiles - j);
+        ib = in / rows;
+        jt = j + in - ib * rows;
+        if (ib >= nib) return;
+      }
       e = a.te[jt];
       count = min(a.tc[jt], BJ);
       off = a.to[jt];
@@ -385,7 +419,8 @@ static void dg_launch(DenseGemmArgs a, hipStream_t s) {
                             : a.x_rows * a.nk >= most || 256 * (MODE == DG_TRANS ? a.ni : a.nk) >= most;
   const int64_t nib = (a.ni + BI - 1) / BI;
   const int64_t items = MODE == DG_WEIGHT ? a.E * ((a.nj + BJ - 1) / BJ) * nib : a.max_tiles * nib;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8));
+  constexpr int64_t G = dg_turn(BJ);
+  const dim3 grid((unsigned)(G ? (a.max_tiles + 8 * G - 1) / (8 * G) * (8 * G) * nib : (items + 7) / 8 * 8));
   hipLaunchKernelGGL((k_dense_gemm<T, BI, BJ, WI, WJ, MODE>), grid, dim3(64 * WI * WJ), 0, s, a);
 }
 
@@ -409,6 +444,8 @@ int dense_gemm_rows(const DenseGemmArgs& a, int dtype, bool transposed, int64_t 
   return launch_status("keep_gather_mm");
 }
 
+// Tiles of 256 x 256 where both sides fill three quarters of one (32 experts of 4096 x 2048, 65536 routes: 1178 us against
+// 1752 with 128 x 128; 64 of 2048 x 768, 32768 routes: 162 against 203).
 int dense_gemm_weight(const DenseGemmArgs& a, int dtype, hipStream_t s) {
   const bool large = a.ni >= 192 && a.nj >= 192;
   if (dtype == KEEP_F16) {
