@@ -110,6 +110,7 @@ __global__ __launch_bounds__(256) void k_combine_grad(const T* y, const float* w
   }
 }
 
+constexpr int64_t COMBINE_VALUES = int64_t(1) << 40;  // more than a GPU holds
 constexpr int64_t COMBINE_BLOCKS = 1 << 23;  // a launch holds 2^32 threads; more work goes round again
 
 template <typename T, typename OT>
@@ -153,6 +154,7 @@ extern "C" int keep_route_combine_rows(const void* y, int y_dtype, const float* 
   KEEP_REQUIRE(k > 0 && H > 0, "k and H must be positive");
   if (T == 0) return KEEP_OK;
   KEEP_REQUIRE(y && out, "null pointer argument");
+  KEEP_REQUIRE(T <= COMBINE_VALUES / k / H, "too many values");
   const bool vec = H % 8 == 0 && aligned(y, 16) && aligned(out, 16);
   by_dtype(y_dtype, [&](auto t) {
     by_dtype(out_dtype, [&](auto o) {
@@ -169,7 +171,7 @@ extern "C" int keep_route_combine_grad(const void* y, int y_dtype, const float* 
   KEEP_REQUIRE(k > 0 && H > 0, "k and H must be positive");
   if (T == 0) return KEEP_OK;
   KEEP_REQUIRE(w && dout && (dy || dw) && (y || !dw), "null pointer argument");
-  KEEP_REQUIRE(T <= 0x7fffffffLL / k, "too many routes");
+  KEEP_REQUIRE(T <= COMBINE_VALUES / k / H, "too many values");
   const bool vec = H % 8 == 0 && aligned(y, 16) && aligned(dout, 16) && aligned(dy, 16);
   by_dtype(y_dtype, [&](auto t) {
     by_dtype(dout_dtype, [&](auto d) {

@@ -278,3 +278,11 @@ def test_capture_check_marks_live_eager_graphs(monkeypatch):
         _grad.check_capture(w.view(1, 3))
     del held
     _grad.check_capture(w.view(1, 3))
+
+
+def test_combine_refuses_more_values_than_a_gpu_holds():
+    lib = _lib.load()
+    assert lib.keep_route_combine_rows(16, 1, 16, 1 << 30, 1 << 10, 8, 16, 1, None) == _lib.KEEP_EINVAL
+    assert "too many" in lib.keep_last_error().decode()
+    assert lib.keep_route_combine_grad(16, 1, 16, 16, 1, 1 << 30, 1 << 10, 8, 16, 16, None) == _lib.KEEP_EINVAL
+    assert "too many" in lib.keep_last_error().decode()
