@@ -99,7 +99,8 @@ __device__ __forceinline__ void dg_dma(const void* base, uint32_t off, uint32_t 
 // Row tiles that an XCD takes in turn (0: a contiguous run of all items). With few routes an expert most tiles read weights
 // of their own, and an XCD whose run has experts of several tiles is done early: 384 experts of 4096 -> 2048, 8192 routes
 // 1213 us in runs, 1110 in turns of 2 (1, 4: the same); 12288 routes of Zipf popularity 1293 against 1226; 64 experts of
-// 2048 -> 768 38.5 against 40. Large tiles share operands with their neighbours instead.
+// 2048 -> 768 38.5 against 40. Large tiles share operands with their neighbours instead (128: 384 experts 1597 against 1440,
+// 256 experts 870 against 944, the same elsewhere).
 constexpr int dg_turn(int bj) { return bj == 64 ? 2 : 0; }
 
 template <typename T, int BI, int BJ, int WI, int WJ, int MODE>
