@@ -445,3 +445,26 @@ def test_capture_is_refused_through_a_cast_too(dev, between):
             keep_amd.gather_mm(x, between(master), idx)
     del held
     assert torch.isfinite(keep_amd.gather_mm(x, between(master), idx)).all()
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+def test_gather_mm_more_tiles_than_a_launch_has_blocks_along_an_axis(dev, transposed):
+    g = torch.Generator(device=dev).manual_seed(2)
+    T, E, N, K = 70_001, 1100, 12, 8  # no plan holds 1100 experts: a tile per route at most
+    x = torch.randint(-4, 5, (T, K), device=dev, generator=g).float()
+    w = torch.randint(-4, 5, (E, N, K), device=dev, generator=g).float()
+    idx = torch.randint(0, E, (T, 1), device=dev, generator=g).int()
+    if transposed:
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    want = (w[idx[:, 0].long()] * x[:, None]).sum(2)  # whole numbers: exact in any order
+    assert torch.equal(keep_amd.gather_mm(x, w, idx)[:, 0], want)
+
+
+def test_route_combine_gradients_of_more_routes_than_a_launch_has_waves(dev):
+    T = (1 << 25) + 5
+    y = torch.arange(T * 4, device=dev).remainder(7).half().view(T, 1, 4).requires_grad_(True)
+    w = torch.arange(T, device=dev).remainder(5).float().view(T, 1).requires_grad_(True)
+    d = torch.arange(T * 4, device=dev).remainder(3).half().view(T, 4)
+    dy, dw = torch.autograd.grad(keep_amd.route_combine(y, w, torch.float16), (y, w), d)
+    assert torch.equal(dy[:, 0], d * w.detach().half())  # whole numbers below 2048
+    assert torch.equal(dw[:, 0], (y.detach()[:, 0].float() * d.float()).sum(1))
