@@ -22,10 +22,12 @@
 // 5; 64 requests of r = 64, 4096 -> 2048: 17 us, the bytes alone 7; 4093 rows in
 // runs of about 100, r = 32, 4096 -> 4096: 48 us (17 + 31), the bytes alone 21.
 //
-// t enters the second product in the rows' 16-bit type (one rounding, half a
-// step of that type relative to the row's largest t), each row times a power of
-// two that brings its largest value to [1, 2): fp16 then holds every row
-// whatever its range. float rows stay float throughout.
+// t enters the second product whole: in 16 bits as a sum of terms of that type,
+// each row times a power of two that brings its largest finite value to [1, 4).
+// Three bf16 terms hold float's 24 bits; two of fp16 hold 22, and are off by at
+// most 2^-25 of the row's largest value. (One term is a rounding to 8 or 11 bits
+// of every t; the others take 1 us of the 52 for 4093 rows, nothing for 64.) float rows
+// stay float throughout.
 #include <algorithm>
 #include <type_traits>
 
@@ -111,6 +113,8 @@ struct LoraWindow {
     return t;
   }
 };
+
+__device__ __forceinline__ bool lora_finite(float v) { return fabsf(v) < __builtin_inff(); }  // (NaN: false)
 
 // Route of row `row` of a tile (-1: past its last).
 __device__ __forceinline__ int64_t lora_route(const LoraArgs& a, const LoraTile& t, int row) {
@@ -219,10 +223,13 @@ __global__ __launch_bounds__(64 * LS_WAVES) void k_lora_shrink(LoraArgs a) {
 // them, so that the lane's results over two products are 8 neighbouring columns of route c, and a row's four lanes make
 // 64 bytes of each load and store. (No loop over columns: loads of a second turn would wait for the first one's stores.)
 // OT: base's and out's type. VEC, WIDE: rows of B, and of base and out, hold whole 16-byte pieces at aligned addresses.
+// Up to rank 32 and 16-bit outputs, 128 registers keep two blocks on a CU (4093 rows of r = 32: 52 us, 65 with one).
 template <typename T, typename OT, bool VEC, bool WIDE, int RT>
-__global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
+__global__ __launch_bounds__(64 * LE_WAVES, sizeof(OT) == 2 && RT <= 2 ? 4 : 1) void k_lora_expand(LoraArgs a) {
   constexpr int V = Dense<T>::V, KS = Dense<T>::KS, RP = 16 * RT, NK = (RP + KS - 1) / KS;
-  __shared__ float ts[LORA_ROWS][NK * KS + 4];
+  constexpr int TERMS = sizeof(T) == 4 ? 1 : __is_same(T, bf16s) ? 3 : 2;
+  __shared__ __attribute__((aligned(16))) T ts[TERMS][LORA_ROWS][NK * KS + V];  // t's terms (the pad: no bank conflicts)
+  __shared__ float tback[LORA_ROWS];                                            // and the rows' powers of two
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int64_t cb = blockIdx.x / a.split, nb = blockIdx.x - cb * a.split;
@@ -244,11 +251,11 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
     }
     auto rows = [&](auto nj_c) {
       constexpr int NJ = decltype(nj_c)::value, OV = 16 / sizeof(OT);
-      int64_t at[NJ];  // of the row in base and out (-1: none)
+      int at[NJ];  // the routes of this lane's rows (-1: none)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int64_t r = lora_route(a, t, 16 * j + c);
-        at[j] = r < 0 ? -1 : r * a.N;
+        at[j] = (int)r;
       }
       // B's rows and base are read before t is there
       uint4 fi[NK][4], base[NJ][2][8 / OV];
@@ -273,7 +280,7 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
           for (int p = 0; p < 2; ++p)
 #pragma unroll
             for (int h = 0; h < 8 / OV; ++h)
-              base[j][p][h] = dense_ld16((const OT*)a.base + max(at[j], (int64_t)0), min(n0 + p * 32 + q * 8, a.N - 8) + h * OV);
+              base[j][p][h] = dense_ld16((const OT*)a.base + (int64_t)max(at[j], 0) * a.N, min(n0 + p * 32 + q * 8, a.N - 8) + h * OV);
       }
       const float sc = a.scales ? a.scales[t.g] : 1.f;
       for (int i = threadIdx.x; i < NJ * 16 * RP / 4; i += 64 * LE_WAVES) {
@@ -298,53 +305,73 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
           f.w = k4 + 3 < a.R ? f.w * sc : 0.f;
           if (a.t_out && nb == 0) *(float4*)(a.t_out + tr * RP + k4) = f;
         }
-        *(float4*)&ts[row][k4] = f;
-        if (NK * KS > RP) *(float4*)&ts[row][RP + k4] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (TERMS == 1) {
+          *(float4*)&ts[0][row][k4] = f;
+        } else {
+          // a row is RP / 4 neighbouring lanes (whole waves are here): 2^e <= its largest value < 2^(e + 1), within the
+          // powers whose inverse is a normal number too
+          float v[4] = {f.x, f.y, f.z, f.w}, mx = 0.f;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mx = fmaxf(mx, lora_finite(v[u]) ? fabsf(v[u]) : 0.f);
+#pragma unroll
+          for (int d = 1; d < RP / 4; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+          const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -126), 126);
+          const float fac = __uint_as_float((uint32_t)(127 - e) << 23);
+          if (k4 == 0) tback[row] = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] *= fac;
+#pragma unroll
+          for (int m = 0; m < TERMS; ++m) {
+            uint32_t w[2] = {0u, 0u};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const T h = from_float<T>(v[u]);
+              const float left = v[u] - to_float(h);  // exact
+              v[u] = lora_finite(left) ? left : 0.f;  // nothing is left of an infinity or NaN
+              w[u >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, h) << (16 * (u & 1));
+            }
+            *(uint2*)&ts[m][row][k4] = make_uint2(w[0], w[1]);
+            if (NK * KS > RP) *(uint2*)&ts[m][row][RP + k4] = make_uint2(0u, 0u);
+          }
+        }
       }
       __syncthreads();
       f4 acc[NJ][4];
       float back[NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        float f[NK][V], mx = 0.f;
+        back[j] = TERMS == 1 ? 1.f : tback[16 * j + c];
+        uint4 fj[TERMS][NK];
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+        for (int m = 0; m < TERMS; ++m)
 #pragma unroll
-          for (int e = 0; e < V; e += 4) {
-            const float4 p = *(const float4*)&ts[16 * j + c][i * KS + q * V + e];
-            f[i][e] = p.x; f[i][e + 1] = p.y; f[i][e + 2] = p.z; f[i][e + 3] = p.w;
-            mx = fmaxf(fmaxf(fmaxf(mx, fabsf(p.x)), fabsf(p.y)), fmaxf(fabsf(p.z), fabsf(p.w)));
-          }
-        uint4 fj[NK];
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-          for (int i = 0; i < NK; ++i)
-            fj[i] = make_uint4(__float_as_uint(f[i][0]), __float_as_uint(f[i][1]), __float_as_uint(f[i][2]),
-                               __float_as_uint(f[i][3]));
-          back[j] = 1.f;
-        } else {
-          mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          // 2^e <= mx: the factor 2^-e (1 for rows of zeros, subnormals, infinities; NaN does not reach mx)
-          const int e = (int)(__float_as_uint(mx) >> 23) - 127;
-          const bool use = e > -127 && e < 127;
-          const float fac = use ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
-          back[j] = use ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
-#pragma unroll
-          for (int i = 0; i < NK; ++i) {
-            uint32_t v[4];
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-              v[p] = (uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(f[i][2 * p] * fac)) |
-                     ((uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(f[i][2 * p + 1] * fac)) << 16);
-            fj[i] = make_uint4(v[0], v[1], v[2], v[3]);
-          }
-        }
+          for (int i = 0; i < NK; ++i) fj[m][i] = *(const uint4*)&ts[m][16 * j + c][i * KS + q * V];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           acc[j][u] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < NK; ++i) acc[j][u] = dense_mfma<T>(fi[i][u], fj[i], acc[j][u]);
+          for (int m = TERMS - 1; m >= 0; --m)
+#pragma unroll
+            for (int i = 0; i < NK; ++i) acc[j][u] = dense_mfma<T>(fi[i][u], fj[m][i], acc[j][u]);
+        }
+        if constexpr (TERMS > 1) {
+          // an infinity in B is one in the output, whatever the signs of t's other terms: there the first term's sums count
+          float z = 0.f;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) z = fmaf(acc[j][u][v], 0.f, z);
+          if (__any(!(z == 0.f))) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              f4 first{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int i = 0; i < NK; ++i) first = dense_mfma<T>(fi[i][u], fj[0][i], first);
+#pragma unroll
+              for (int v = 0; v < 4; ++v)
+                if (!lora_finite(first[v])) acc[j][u][v] = first[v];
+            }
+          }
         }
       }
 #pragma unroll
@@ -359,10 +386,10 @@ __global__ __launch_bounds__(64 * LE_WAVES) void k_lora_expand(LoraArgs a) {
             f[u] = acc[j][2 * p + (u >> 2)][u & 3] * back[j];
             if (a.base) {
               if constexpr (WIDE) f[u] += dense_at<OT>(base[j][p][u / OV], u % OV);
-              else f[u] += n + u < a.N ? to_float(((const OT*)a.base)[at[j] + n + u]) : 0.f;
+              else f[u] += n + u < a.N ? to_float(((const OT*)a.base)[at[j] * a.N + n + u]) : 0.f;
             }
           }
-          dense_st<OT, 8>((OT*)a.out + at[j] + n, a.N - n, f, WIDE);
+          dense_st<OT, 8>((OT*)a.out + at[j] * a.N + n, a.N - n, f, WIDE);
         }
       __syncthreads();  // ts is written again
     };
