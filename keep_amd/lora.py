@@ -62,10 +62,13 @@ class _GatherLora(torch.autograd.Function):
         nx, na, nb, nbase = ctx.needs_input_grad[:4]
         (n, rank, K), N, R, device = a.shape, b.shape[1], idx.numel(), x.device
         make = torch.empty_like if R else torch.zeros_like
+        # a float32 output over 16-bit rows: its gradient keeps its bits and range, so the products are float32's
+        dtype, wide = x.dtype, dy.dtype != x.dtype and bool(R and (nx or na or nb))
+        if wide:
+            x, a, b = x.float(), a.float(), b.float()
         dx, da, db = (make(t_) if need else None for t_, need in ((x, nx), (a, na), (b, nb)))
         if R and (nx or na or nb):
-            # a float32 output over 16-bit rows: its gradient enters the products in their type
-            g, dt = dy.to(x.dtype).contiguous(), ops._DT[x.dtype]
+            g, dt = dy.contiguous(), ops._DT[x.dtype]
             planned = int(na or nb or (ctx.x_div > 1 and R >= PLANNED_ROUTES and n <= ops.PLAN_EXPERTS))
             with ops._on(device):
                 need = _lib.load().keep_lora_backward_workspace_bytes(dt, R, ctx.x_div, n, rank, K, N, int(nx), planned)
@@ -73,6 +76,8 @@ class _GatherLora(torch.autograd.Function):
                 _lib.call("keep_lora_backward", x.data_ptr(), dt, x.shape[0], a.data_ptr(), b.data_ptr(),
                           ops._ptr(scales), idx.data_ptr(), R, ctx.x_div, n, rank, K, N, t.data_ptr(), g.data_ptr(),
                           ops._ptr(dx), ops._ptr(da), ops._ptr(db), planned, ws.data_ptr(), need, ops._stream(device))
+        if wide:
+            dx, da, db = (None if g is None else g.to(dtype) for g in (dx, da, db))
         return dx, da, db, dy.reshape(ctx.base_shape) if nbase else None, None, None, None, None
 
 
@@ -84,7 +89,7 @@ def gather_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, ind
     ``indices [T]`` -> ``[T, N]``; ``indices [T, k]`` (an adapter per route of a token) -> ``[T, k, N]``. ``base`` (of
     the output's shape) is added, in float32 with one rounding; the output has its dtype, without it ``x``'s. ``scales``
     (``[n]``, kept in float32) multiplies each adapter and takes no gradient. Gradients of the factors need
-    ``n <= 1024``. The low-rank row is float32, and enters the second product with 22 (fp16) or 24 bits.
+    ``n <= 1024``; over a float32 ``base`` they are formed in float32 and rounded once. The low-rank row is float32, and enters the second product with 22 (fp16) or 24 bits.
     """
 
     device = ops._dense_device(x, lora_a, lora_b, base)
