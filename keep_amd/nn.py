@@ -348,7 +348,9 @@ class SwitchLinear:
             raise ValueError(f"x {tuple(x.shape)} and indices {tuple(indices.shape)} match neither the token nor "
                              "the per-route layout")
         if self.bias is not None:
-            y = y + self.bias[indices.long().clamp(0, self.num_experts - 1)].to(y.dtype)  # (routes out of range: NaN)
+            e = indices.long()
+            valid = (e >= 0) & (e < self.num_experts)  # the other routes' rows are NaN, and have no share in a bias
+            y = y + torch.where(valid[..., None], self.bias[torch.where(valid, e, 0)], 0).to(y.dtype)
         return y if adapter_indices is None else _add_adapters(self, y, rows.view(x.shape), indices, adapter_indices)
 
 
