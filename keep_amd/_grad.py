@@ -58,3 +58,22 @@ def mark(out: torch.Tensor) -> torch.Tensor:
             if node is not None:
                 node.metadata[_EAGER] = True
     return out
+
+
+class _Partial(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, out, x):
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise RuntimeError("a product with codes has no gradient, and this layer's input requires one: detach the input "
+                           "to train what does not pass the codes")
+
+
+def partial(out: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+    """``out`` of a layer on codes, with a graph from its other paths. Where ``x`` requires a gradient too, the backward
+    pass would give it the share of those paths alone, and raises instead."""
+
+    return _Partial.apply(out, x) if wanted(x) else out

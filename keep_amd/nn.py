@@ -24,7 +24,7 @@ from typing import Callable
 import numpy as np
 import torch
 
-from keep_amd import _lib, ops
+from keep_amd import _grad, _lib, ops
 from keep_amd.dense import gather_mm
 from keep_amd.lora import LoraAdapters
 from keep_amd.router import RouterOutput, _slot_args, router_dual_topk
@@ -1006,6 +1006,10 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, gate, up, down, *, k: int, 
     return out, r
 
 
+def _holds_codes(glu) -> bool:
+    return glu is not None and not all(isinstance(p, SwitchLinear) for p in (glu.gate_proj, glu.up_proj, glu.down_proj))
+
+
 class RoutedVQMoE:
     """Router + routed E8P SwiGLU experts + weighted combine (one MoE layer).
 
@@ -1032,8 +1036,10 @@ class RoutedVQMoE:
     that gave up (NaN output).
 
     ``glu`` may hold dense projections (``SwitchLinear``): the layer is then differentiable in ``x``, the experts'
-    weights, the shared expert's and ``residual`` (the router's outputs take no gradient). ``adapter_indices`` (one
-    per token, -1: none) adds the adapters of the projections that have some.
+    weights, the shared expert's and ``residual`` (the router's outputs take no gradient). Codes have no gradient:
+    beside them ``residual`` and a dense shared expert's weights get theirs while ``x`` requires none; where it does,
+    the backward pass raises. ``adapter_indices`` (one per token, -1: none) adds the adapters of the projections that
+    have some.
     """
 
     def __init__(self, glu: QuantizedVQSwitchGLU, *, top_k: int, score_func: str = "softmax",
@@ -1086,7 +1092,8 @@ class RoutedVQMoE:
             return moe_decode(x, idx, weight, (g.codes, g.scales), (u.codes, u.scales), (d.codes, d.scales),
                               limit=self.limit, codebook=g.codebook, out_dtype=od)
         y = self.glu(x, idx)  # [T, k, H]
-        return ops.route_combine(y, weight, od)
+        out = ops.route_combine(y, weight, od)
+        return _grad.partial(out, x) if out.requires_grad and _holds_codes(self.glu) else out
 
     def _layer_path(self, x: torch.Tensor) -> bool:
         g, d = self.glu.gate_proj, self.glu.down_proj
@@ -1140,4 +1147,7 @@ class RoutedVQMoE:
             return out, r
         from keep_amd.block import combine_add
         sh = self.shared(x) if self.shared_experts is not None else None
-        return combine_add(out, sh, residual, self.out_dtype), r
+        out = combine_add(out, sh, residual, self.out_dtype)
+        if out.requires_grad and (_holds_codes(self.glu) or _holds_codes(self.shared_experts)):
+            out = _grad.partial(out, x)
+        return out, r
