@@ -3,17 +3,23 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 _EAGER = "keep_amd: eager graph"
 _STEPS = 6  # views, casts and the like between a leaf and a call's argument
 
 
 def wanted(*tensors) -> bool:
-    """Whether autograd records a call on these tensors."""
+    """Whether autograd records a call on these tensors. A forward-mode tangent counts too: the operators' functions
+    have no rule for one, and refuse it."""
 
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:  # inside a dual_level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 return True
     return False
 

@@ -118,7 +118,7 @@ def gather_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, ind
         raise ValueError(f"base must have shape {shape} in {x.dtype} or float32, found {tuple(base.shape)} "
                          f"in {base.dtype}")
     if scales is not None:
-        if torch.is_grad_enabled() and scales.requires_grad:
+        if _grad.wanted(scales):
             raise ValueError("scales take no gradient")
         if tuple(scales.shape) != (n,):
             raise ValueError(f"scales must have shape ({n},), found {tuple(scales.shape)}")
