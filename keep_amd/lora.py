@@ -174,6 +174,8 @@ class LoraAdapters:
             raise ValueError(f"adapter_indices must hold one adapter per row ({x.shape[0]}), found {tuple(idx.shape)}")
         if experts is None:
             return gather_lora(x, self.a, self.b, idx, base=base, scales=self._scales)
+        if self.scales is not None and _grad.wanted(self.scales):  # the copy has no graph
+            raise ValueError("scales take no gradient")
         E = self.num_experts
         e = ops._index_tensor(experts, x.device)
         # a route without an expert has a NaN base row already
