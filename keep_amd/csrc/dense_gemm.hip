@@ -87,13 +87,12 @@ __device__ __forceinline__ int64_t dg_row(const DenseGemmArgs& a, int r) {
 // 16 bytes per lane to lds_wave_base + 16 lane, from an address per lane, or from one offset per lane off a common
 // base. Written out, since the compiler waits for every copy in flight before any LDS read that follows the builtin: here
 // the reads are of the other buffer, and the loop's own wait and barrier stand between a copy and its readers. (No
-// register is written, so none can be reused early.)
+// register is written, so none can be reused early; M0 is an operand, which the compiler sets and knows.)
 __device__ __forceinline__ void dg_dma(const void* g, uint32_t lds_wave_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_wave_base), "v"(g) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(lds_wave_base), "v"(g) : "memory");
 }
 __device__ __forceinline__ void dg_dma(const void* base, uint32_t off, uint32_t lds_wave_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_wave_base), "v"(off), "s"(base)
-               : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds_wave_base), "v"(off), "s"(base) : "memory");
 }
 
 // Row tiles that an XCD takes in turn (0: a contiguous run of all items). With few routes an expert most tiles read weights
