@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 _EAGER = "keep_amd: eager graph"
-_STEPS = 6  # views, casts and the like between a leaf and a call's argument
+_NODES = 12  # steps looked at between a call's argument and its leaves: views, casts, a merge of weights
 
 
 def wanted(*tensors) -> bool:
@@ -24,17 +24,16 @@ def wanted(*tensors) -> bool:
     return False
 
 
-def _leaf_node(node):
-    """The gradient node of the leaf that ``node``'s graph reads alone (a parameter, its view or cast), or None."""
+def _leaf_nodes(node) -> list:
+    """The gradient nodes of the leaves near ``node`` (parameters, their views, casts and sums)."""
 
-    for _ in range(_STEPS):
-        if node is None or hasattr(node, "variable"):
-            return node
-        following = [f for f, _ in node.next_functions if f is not None]
-        if len(following) != 1:
-            return None
-        node = following[0]
-    return None
+    leaves, todo = [], [node]
+    for node in todo:
+        if hasattr(node, "variable"):
+            leaves.append(node)
+        elif len(todo) < _NODES:
+            todo.extend(f for f, _ in node.next_functions if f is not None)
+    return leaves
 
 
 def check_capture(*tensors) -> None:
@@ -42,27 +41,29 @@ def check_capture(*tensors) -> None:
 
     A leaf has one gradient node at a time, bound to the stream that made it. While an eager graph is alive, a
     backward pass under capture would make that other stream wait on the capturing one, which ends the process. Eager
-    calls leave a mark on the node (``mark``), which lives as long as some graph holds it. Leaves are found through
-    views, casts and other steps of one input."""
+    calls leave a mark on the node (``mark``), which lives as long as something holds it: a graph, or what keeps the
+    node itself (a data-parallel wrapper, a stored gradient edge), where the node stays bound to its stream too."""
 
     if not torch.cuda.is_current_stream_capturing():
         return
     for t in tensors:
         if t is not None and t.requires_grad:
-            node = _leaf_node(torch.autograd.graph.get_gradient_edge(t).node)
-            if node is not None and _EAGER in node.metadata:
-                raise RuntimeError("graph capture of a differentiable call on a leaf that an eager graph still holds: "
-                                   "drop that graph's outputs first, or capture on leaves of its own")
+            for node in _leaf_nodes(torch.autograd.graph.get_gradient_edge(t).node):
+                if _EAGER in node.metadata:
+                    raise RuntimeError("graph capture of a differentiable call on a leaf whose gradient node an eager "
+                                       "graph made and something still holds: drop that graph's outputs (and what else "
+                                       "holds the node) first, or capture on leaves of its own, as t.detach()"
+                                       ".requires_grad_()")
 
 
 def mark(out: torch.Tensor) -> torch.Tensor:
     """``out`` of an eager call, its leaves' gradient nodes marked."""
 
     if not torch.cuda.is_current_stream_capturing():
-        for node, _ in out.grad_fn.next_functions:
-            node = _leaf_node(node)
-            if node is not None:
-                node.metadata[_EAGER] = True
+        for first, _ in out.grad_fn.next_functions:
+            if first is not None:
+                for node in _leaf_nodes(first):
+                    node.metadata[_EAGER] = True
     return out
 
 
