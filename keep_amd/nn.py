@@ -640,8 +640,7 @@ class QuantizedVQSwitchGLU:
 
         if self.hot_tier is not None:
             raise ValueError("adapters and the hot tier do not combine")
-        if adapter_indices is not None and all(p.adapters is None
-                                               for p in (self.gate_proj, self.up_proj, self.down_proj)):
+        if adapter_indices is not None and not _has_adapters(self):
             raise ValueError("adapter_indices need a projection with adapters")
 
         def project(p, rows, ad):
@@ -1010,6 +1009,10 @@ def _holds_codes(glu) -> bool:
     return glu is not None and not all(isinstance(p, SwitchLinear) for p in (glu.gate_proj, glu.up_proj, glu.down_proj))
 
 
+def _has_adapters(glu) -> bool:
+    return any(p.adapters is not None for p in (glu.gate_proj, glu.up_proj, glu.down_proj))
+
+
 class RoutedVQMoE:
     """Router + routed E8P SwiGLU experts + weighted combine (one MoE layer).
 
@@ -1039,7 +1042,7 @@ class RoutedVQMoE:
     weights, the shared expert's and ``residual`` (the router's outputs take no gradient). Codes have no gradient:
     beside them ``residual`` and a dense shared expert's weights get theirs while ``x`` requires none; where it does,
     the backward pass raises. ``adapter_indices`` (one per token, -1: none) adds the adapters of the projections that
-    have some.
+    have some, the shared expert's too.
     """
 
     def __init__(self, glu: QuantizedVQSwitchGLU, *, top_k: int, score_func: str = "softmax",
@@ -1066,13 +1069,16 @@ class RoutedVQMoE:
         self.shared_experts = shared_experts
         self.slot_map = slot_map
 
-    def shared(self, x: torch.Tensor) -> torch.Tensor:
-        """The shared expert's output for every row of ``x``, float32 ``[T, H]``."""
+    def shared(self, x: torch.Tensor, adapter_indices=None) -> torch.Tensor:
+        """The shared expert's output for every row of ``x``, float32 ``[T, H]``; ``adapter_indices``: with its
+        adapters."""
 
         se = self.shared_experts
         T = x.shape[0]
         idx = torch.zeros((T, 1), dtype=torch.int32, device=x.device)
         w = torch.ones((T, 1), dtype=torch.float32, device=x.device)
+        if adapter_indices is not None:
+            return se(x, idx, adapter_indices).reshape(T, -1).float()
         g, u, d = se.gate_proj, se.up_proj, se.down_proj
         if (T <= self.decode_max_tokens and se._all_e8p() and se.hot_tier is None
                 and x.dtype in (torch.float16, torch.bfloat16)):
@@ -1122,6 +1128,11 @@ class RoutedVQMoE:
                  adapter_indices=None):
         extra = self.shared_experts is not None or residual is not None
         od = torch.float32 if extra else self.out_dtype
+        shared_adapters = None
+        if adapter_indices is not None and self.shared_experts is not None and _has_adapters(self.shared_experts):
+            shared_adapters = adapter_indices
+            if not _has_adapters(self.glu):
+                adapter_indices = None
         entry = self._tiles_layer_path(x, logits) if adapter_indices is None else None
         if entry is not None:
             g, u, d = self.glu.gate_proj, self.glu.up_proj, self.glu.down_proj
@@ -1146,7 +1157,7 @@ class RoutedVQMoE:
         if not extra:
             return out, r
         from keep_amd.block import combine_add
-        sh = self.shared(x) if self.shared_experts is not None else None
+        sh = self.shared(x, shared_adapters) if self.shared_experts is not None else None
         out = combine_add(out, sh, residual, self.out_dtype)
         if out.requires_grad and (_holds_codes(self.glu) or _holds_codes(self.shared_experts)):
             out = _grad.partial(out, x)
