@@ -10,7 +10,7 @@
 // writes its row of dy once and takes dout, which the k routes of a token
 // share, from the caches. Measured: 2048 x 6 rows of 4096, bf16 to float32
 // (134 MB) 23.8 us, 5.6 TB/s; backward of 1021 x 8 rows of 4096, bf16 (151 MB) 28 to 31 us, where a copy of as many
-// bytes takes 29.
+// bytes takes 29. Rows of no whole number of eight values go value by value: 2048 x 6 rows of 4092 66 us.
 #include <algorithm>
 
 #include "common.h"

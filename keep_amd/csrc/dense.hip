@@ -141,7 +141,9 @@ __global__ __launch_bounds__(64 * GF_WAVES) void k_gather_few(GatherArgs a) {
 }
 
 // W [E][K][N]: a lane loads V neighbouring columns of V rows of W (rows V q + s of the step) and V values of its route's
-// x; product (s, u) takes value u of row s and value s of x.
+// x; product (s, u) takes value u of row s and value s of x. Bound by the wait for each step's loads: a wave walks all of K
+// for its 128 columns, so a token fills few CUs. One token of 6 experts, fp16 4096 -> 2048, 258 us (k_gather_few on the other
+// layout 17.6); eight tokens of 6, bf16, 298 (127).
 constexpr int GT_WAVES = 4;
 
 template <typename T, bool VEC>
@@ -193,7 +195,8 @@ __global__ __launch_bounds__(64 * GT_WAVES) void k_gather_trans(GatherArgs a) {
 // Lane (c, q) of a step holds four neighbouring values of row 4 s + q of the wide side and one value per 16 of the narrow
 // side; product (u, b) takes value u. Eight waves take every eighth run of 32 routes, whose ids a lane each loads once, so
 // that a run's rows are all in flight together; the waves are added in order through LDS. NB: 16-wide pieces of the narrow
-// side, one where a second would be empty. Bound by the wait for a run's rows: 2048 routes of 8 adapters, r = 16, 8.3 to
+// side, one where a second would be empty. As dW of an odd width it reads rows value by value: a training step of 1024 tokens
+// of 64 experts, 2048 -> 767, takes 2153 us (dx's share with k_gather_trans) where 768 takes 271. Bound by the wait for a run's rows: 2048 routes of 8 adapters, r = 16, 8.3 to
 // 11.7 us a factor (4096 or 2048 wide, bf16), 37 with one wave a block and a route id per step.
 constexpr int RO_WAVES = 8, RO_V = 4, RO_RUN = 32, RO_UN = RO_RUN / 4;
 

@@ -18,14 +18,15 @@
 // loads (four rows of 16 columns a time), its 32-byte pairs permuted likewise.
 // Past an operand's end, lanes copy a zero instead.
 //
-// Bound by the matrix cores and LDS alike: a step of a 256 x 256 tile is 512
-// products of 16 clocks on four SIMDs, 2048 clocks, and its 64 KiB of copies and
-// 192 KiB of fragments (each read by two or four waves, half a step ahead of its
-// products, without bank conflicts) are as many at 128 bytes a clock. Measured,
-// bf16: 8192 x 8192 x 8192 forward 854 to 880 us (1250 to 1290 TFLOP/s), dx 1219
-// to 1275 TFLOP/s, dW about 1100; 65536 routes of 32 experts, 4096 -> 2048, 1045
-// us (1052). Of a tile of 4096 summed values about 11 us are its first copies and
-// its stores; the last round of tiles fills part of the CUs.
+// A step of a 256 x 256 tile is 512 products of 16 clocks on four SIMDs, 2048
+// clocks (0.85 us at 2.4 GHz), and its 64 KiB of copies and 192 KiB of fragments
+// (each read by two or four waves, half a step ahead of its products, without
+// bank conflicts) are as many clocks of LDS at 128 bytes each. Measured, a step
+// takes 1.6 us: waves wait 32 to 44 % of their cycles. First copies and stores
+// add 10 to 14 us a tile: 115 us for 4096 summed values. bf16: 8192 x 8192 x 8192
+// forward 848 us (1297 TFLOP/s), dx 865 to 907, dW 1013; 65536 routes of 32
+// experts, 4096 -> 2048, 1039 to 1058 us (1058 to 1039 TFLOP/s). The last round
+// of tiles fills part of the CUs.
 // Eight waves of 64 x 128 results each and four of 128 x 128 hold the same tile:
 // the eight hide each other's waits. Tiles in turn on a resident workgroup, the
 // next one's copies under the stores, took 66 to 86 registers more than there are.

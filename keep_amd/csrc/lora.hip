@@ -17,10 +17,12 @@
 // One launch that repeats t in every block of columns took 1.1 to 1.6 times as
 // long at every size (one CU reads A, where the slices read it on many).
 //
-// Bound: the dependent loads at a block's start (window, partial sums, rows).
-// One row, r = 16, 4096 -> 4096: 9.3 us of which two empty launches take about
-// 5; 64 requests of r = 64, 4096 -> 2048: 17 us, the bytes alone 7; 4093 rows in
-// runs of about 100, r = 32, 4096 -> 4096: 48 us (17 + 31), the bytes alone 21.
+// Bound: the dependent loads at a block's start (window, partial sums, rows):
+// waves wait 48 % (shrink) and 57 % (expand) of their cycles at 4093 rows.
+// In a graph, both launches: one row, r = 16, 4096 -> 4096, 8.5 us, of which two
+// empty launches take about 5; 64 requests of r = 64, 4096 -> 2048, 17 us, the
+// bytes alone 7; 4093 rows in runs of about 100, r = 32, 4096 -> 4096, 49 us (17
+// + 32), the bytes alone 21.
 //
 // t enters the second product whole: in 16 bits as a sum of terms of that type,
 // each row times a power of two that brings its largest finite value to [1, 4).
@@ -228,7 +230,7 @@ template <typename T, typename OT, bool VEC, bool WIDE, int RT>
 __global__ __launch_bounds__(64 * LE_WAVES, sizeof(OT) == 2 && RT <= 2 ? 4 : 1) void k_lora_expand(LoraArgs a) {
   constexpr int V = Dense<T>::V, KS = Dense<T>::KS, RP = 16 * RT, NK = (RP + KS - 1) / KS;
   constexpr int TERMS = sizeof(T) == 4 ? 1 : __is_same(T, bf16s) ? 3 : 2;
-  __shared__ __attribute__((aligned(16))) T ts[TERMS][LORA_ROWS][NK * KS + V];  // t's terms (the pad: no bank conflicts)
+  __shared__ __attribute__((aligned(16))) T ts[TERMS][LORA_ROWS][NK * KS + V];  // t's terms (the pad spreads rows over the banks)
   __shared__ float tback[LORA_ROWS];                                            // and the rows' powers of two
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -431,7 +433,7 @@ __global__ __launch_bounds__(256) void k_lora_transpose(TransposeArgs a) {
 static int lora_rt(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }
 
 // Blocks per window: one per position while every row may be a request of its own and the windows are few, down to about
-// as many as a window of long runs has tiles (4093 rows in runs of about 100: 6 blocks 48 us, 8 53).
+// as many as a window of long runs has tiles (4093 rows in runs of about 100: 6 blocks 49 us, 8 54).
 static int64_t lora_heads(int64_t routes) {
   const int64_t windows = (routes + 127) / 128;
   return std::min<int64_t>(std::min<int64_t>(routes, 128), windows <= 2 ? 128 : std::max<int64_t>(6, 192 / windows));
@@ -439,8 +441,10 @@ static int64_t lora_heads(int64_t routes) {
 static int64_t lora_blocks(int64_t routes) { return (routes + 127) / 128 * lora_heads(routes); }
 
 // Slices of K, a power of two (a wave's steps then come in whole batches): about 40 KiB of A each (one row, r = 16 of 4096:
-// 4 slices 9.3 us, 1 12.0; r = 128 of 8192: 16 slices 20, 4 28), while the tiles leave CUs free (64 requests of r = 64: 4
-// slices 16.4 us, 8 19.4; 4093 rows of r = 32: 4 slices 48, 16 68). Each wave takes at least a step of 64 bytes of a row.
+// 4 slices 8.5 us, 1 11.1; r = 128 of 8192: 16 slices 19, 4 26), while the tiles leave CUs free (64 requests of r = 64: 4
+// slices 17.3 us, 8 18.8; 4093 rows of r = 32: 4 slices 49, 16 97). Each wave takes at least a step of 64 bytes of a row.
+// Up to 256 rows count as requests of their own, which they need not be: of r = 64, 256 rows of one adapter take 35 us in
+// their one slice and 21 in four (257 rows: 20), 256 rows of 96 adapters in turn 44 and 51; 512 such rows 107, in one 94.
 static int64_t lora_slices(int64_t routes, int64_t R, int64_t K, int size) {
   const int64_t steps = (K * size + 63) / 64, want = R * K * size / (40 << 10) + 1;
   const int64_t room = routes <= 256 ? 256 / routes : 20000 / routes;

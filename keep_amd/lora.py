@@ -20,9 +20,9 @@ from keep_amd import _grad, _lib, ops
 
 MAX_RANK = 128
 # Routes (2D indices) from which a plan brings the routes of one adapter together first: rows of a request lie together
-# as they are, its routes' experts do not. Microseconds without and with one, routes of random adapters, bf16: 32 adapters of
-# r = 16, 2048 -> 1024: 128 routes 10 / 15, 256 12 / 19, 512 25 / 19, 4096 126 / 28; 64 of r = 32, 4096 -> 2048: 128 routes
-# 15 / 18, 256 27 / 25, 512 53 / 27, 4096 303 / 50.
+# as they are, its routes' experts do not. Microseconds without and with one, routes of random adapters, bf16, in a graph: 32
+# adapters of r = 16, 2048 -> 1024: 128 routes 10 / 16, 256 12 / 22, 512 26 / 20, 4096 135 / 30; 64 of r = 32, 4096 -> 2048:
+# 128 routes 16 / 19, 256 26 / 26, 512 57 / 26, 4096 327 / 52.
 PLANNED_ROUTES = 256
 
 
