@@ -89,7 +89,8 @@ def gather_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, ind
     ``indices [T]`` -> ``[T, N]``; ``indices [T, k]`` (an adapter per route of a token) -> ``[T, k, N]``. ``base`` (of
     the output's shape) is added, in float32 with one rounding; the output has its dtype, without it ``x``'s. ``scales``
     (``[n]``, kept in float32) multiplies each adapter and takes no gradient. Gradients of the factors need
-    ``n <= 1024``; over a float32 ``base`` they are formed in float32 and rounded once. The low-rank row is float32, and enters the second product with 22 (fp16) or 24 bits.
+    ``n <= 1024``; over a float32 ``base`` they are formed in float32 and rounded once. The low-rank row is float32,
+    and enters the second product with 22 bits (fp16) or 24.
     """
 
     device = ops._dense_device(x, lora_a, lora_b, base)

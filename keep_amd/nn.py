@@ -1042,7 +1042,7 @@ class RoutedVQMoE:
     weights, the shared expert's and ``residual`` (the router's outputs take no gradient). Codes have no gradient:
     beside them ``residual`` and a dense shared expert's weights get theirs while ``x`` requires none; where it does,
     the backward pass raises. ``adapter_indices`` (one per token, -1: none) adds the adapters of the projections that
-    have some, the shared expert's too.
+    have some, the shared expert's too; with ``slot_map`` a routed expert's are its pool row's, as its weights.
     """
 
     def __init__(self, glu: QuantizedVQSwitchGLU, *, top_k: int, score_func: str = "softmax",
