@@ -23,6 +23,8 @@ extern "C" {
 #endif
 
 enum { KEEP_F32 = 0, KEEP_F16 = 1, KEEP_BF16 = 2 };
+enum { KEEP_E4M3 = 3 }; /* 8-bit operands of keep_linear_q8, for its workspace; no other entry point takes it */
+enum { KEEP_ACT_NONE = 0, KEEP_ACT_RELU = 1, KEEP_ACT_SILU = 2, KEEP_ACT_GELU = 3, KEEP_ACT_GELU_TANH = 4 };
 enum { KEEP_OK = 0, KEEP_EINVAL = -1, KEEP_ELAUNCH = -2, KEEP_EUNSUPPORTED = -3 };
 enum { KEEP_SCORE_SOFTMAX = 0, KEEP_SCORE_SIGMOID = 1, KEEP_SCORE_SQRTSOFTPLUS = 2 };
 
@@ -624,6 +626,74 @@ int keep_lora_backward(const void* x, int dtype, int64_t x_rows, const void* a, 
                        void* workspace, int64_t workspace_bytes, void* stream);
 int64_t keep_lora_backward_workspace_bytes(int dtype, int64_t routes, int64_t x_div, int64_t adapters, int64_t rank,
                                            int64_t K, int64_t N, int dx, int planned);
+
+/* Root-mean-square norm of T rows of n values (1..16384) with the residual's addition: h = round(residual + x), formed in
+ * fp32 and rounded to the residual's dtype (x's or float32), r = 1 / sqrt(mean(h^2) + eps), y = round(h r weight) in x's
+ * dtype. residual and h both NULL: h = x. weight [n] of any float dtype or NULL (ones); rstd fp32 [T] receives r, or NULL.
+ * The sum of the block's residual stream and its next input, and the norm that follows (ffn_norm,
+ * src/ramp/models/deepseek_v4_flash_adapter.py:1794,1806). */
+int keep_rmsnorm(const void* x, int x_dtype, const void* residual, int residual_dtype, int64_t T, int64_t n,
+                 const void* weight, int weight_dtype, float eps, void* h, void* y, float* rstd, void* stream);
+
+/* The same with y in 8 bits: q [T, n] e4m3 of h r weight / s, rounded once and clamped to +-448, s = max(max |h r weight|,
+ * 1e-4) / 448 over quant_block neighbouring values (a power of two in 16..512; the row's last block may be shorter; with
+ * pow2_scales the next power of two), scales fp32 [T, ceil(n / quant_block)]: the values that act_quant
+ * (scripts/runpod/v41_reap/torch_kernel.py:40-53) writes back, kept as codes. */
+int keep_rmsnorm_quant(const void* x, int x_dtype, const void* residual, int residual_dtype, int64_t T, int64_t n,
+                       const void* weight, int weight_dtype, float eps, int64_t quant_block, int pow2_scales, void* h,
+                       void* q, float* scales, void* stream);
+
+/* keep_rmsnorm's gradients, from its h (x without a residual) and rstd: with g = dy weight,
+ * d = r (g - h r^2 mean(g h)) + dh; dx (dy's dtype) and dresidual (h's dtype) receive d, dweight (weight's dtype) the sum over
+ * the rows of dy h r, in a fixed order. dh (h's dtype) or NULL: the gradient of the h output. Outputs may be NULL; the
+ * workspace (keep_rmsnorm_grad_workspace_bytes) is needed with dweight. */
+int keep_rmsnorm_grad(const void* h, int h_dtype, const void* dy, int dy_dtype, const void* dh, const float* rstd,
+                      int64_t T, int64_t n, const void* weight, int weight_dtype, void* dx, void* dresidual,
+                      void* dweight, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t keep_rmsnorm_grad_workspace_bytes(int64_t T, int64_t n);
+
+/* The choice of experts among groups (MoEGate with groups; _expert_select,
+ * src/ramp/models/deepseek_v4_flash_adapter.py:923-940, is the case of one group). logits [T, E] of any float dtype, scores as
+ * keep_router_dual_topk's (a softmax row of -inf alone: 0); key = score + bias (fp32 [E] or NULL). groups (1..64, dividing E)
+ * of E / groups neighbouring experts: the topk_groups groups with the largest sum of their two largest keys are kept, and the
+ * k largest keys in them chosen; the lower index first among equals, NaN as -inf. idx int32 and w fp32 [T, k] in descending
+ * order of the keys: w = score route_scale, renormalised to sum to route_scale (+ 1e-20) with renormalize. load int32 [E] or
+ * NULL: the chosen experts are counted into it (added to what it holds). E <= 1024, k <= 32, T <= 2^25. */
+int keep_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int64_t k, const float* bias, int64_t groups,
+                       int64_t topk_groups, int score_func, int renormalize, float route_scale, int32_t* idx, float* w,
+                       int32_t* load, void* stream);
+
+/* The gradient of its logits [T, E] (their dtype) from dw [T, k], for the experts idx that it chose. */
+int keep_route_experts_grad(const void* logits, int dtype, int64_t T, int64_t E, int64_t k, const int32_t* idx,
+                            const float* dw, int score_func, int renormalize, float route_scale, void* dlogits,
+                            void* stream);
+
+/* Dense projection with its epilogue: u = x weight^T + bias, out = round(residual + act(u)). x [M, K] and weight [N, K] of one
+ * dtype, their rows x_ld and w_ld values apart (whole 16-byte pieces; x and weight 16-byte aligned). Where K is no whole
+ * number of pieces, what lies between a row's K values and the next piece enters the sums: zeros. bias [N], residual [M, N]
+ * and out [M, N] of any float dtype, dense; bias and residual may be NULL. u [M, N] (x's dtype) receives the values before the
+ * activation, or NULL. fp32 sums in a fixed order. N, K <= 2^20. The workspace holds keep_linear_workspace_bytes (may be 0),
+ * 16-byte aligned. */
+int keep_linear(const void* x, int64_t x_ld, int dtype, int64_t M, const void* weight, int64_t w_ld, int64_t N, int64_t K,
+                const void* bias, int bias_dtype, int act, const void* residual, int residual_dtype, void* u, void* out,
+                int out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+/* dtype KEEP_E4M3: of keep_linear_q8. */
+int64_t keep_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+
+/* The same on 8-bit operands (e4m3): x [M, K] with scales [M, ceil(K / 128)], weight [N, K] with scales
+ * [ceil(N / 128), ceil(K / 128)], both fp32. */
+int keep_linear_q8(const void* x, int64_t x_ld, const float* x_scales, int64_t M, const void* weight, int64_t w_ld,
+                   const float* w_scales, int64_t N, int64_t K, const void* bias, int bias_dtype, int act,
+                   const void* residual, int residual_dtype, void* out, int out_dtype, void* workspace,
+                   int64_t workspace_bytes, void* stream);
+
+/* keep_linear's gradients from dy [M, N] of x's dtype: du = dy act'(u) rounded to it, dx = du weight [M, K], dweight = du^T x
+ * [N, K], dbias = the sum of the unrounded du [N], each or NULL; u as keep_linear gave it (NULL without an activation). x and
+ * weight as there. The residual's gradient is dy. The workspace holds keep_linear_grad_workspace_bytes, 256-byte aligned. */
+int keep_linear_grad(const void* dy, const void* u, int act, const void* x, int64_t x_ld, const void* weight,
+                     int64_t w_ld, int dtype, int64_t M, int64_t N, int64_t K, void* dx, void* dweight, void* dbias,
+                     int bias_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t keep_linear_grad_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 
 /* Random-sign Walsh-Hadamard transform of T rows of n activations (16 <= n <= 8192,
  * a power of two): forward y = FWHT(x * signs) / sqrt(n), inverse (inverse != 0)

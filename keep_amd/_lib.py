@@ -68,6 +68,21 @@ _SIGS = {
     "keep_lora_backward": [_P, c_int, c_int64, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P,
                            _P, _P, _P, _P, c_int, _P, c_int64, _P],
     "keep_lora_backward_workspace_bytes": [c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int],
+    "keep_rmsnorm": [_P, c_int, _P, c_int, c_int64, c_int64, _P, c_int, c_float, _P, _P, _P, _P],
+    "keep_rmsnorm_quant": [_P, c_int, _P, c_int, c_int64, c_int64, _P, c_int, c_float, c_int64, c_int, _P, _P, _P, _P],
+    "keep_rmsnorm_grad": [_P, c_int, _P, c_int, _P, _P, c_int64, c_int64, _P, c_int, _P, _P, _P, _P, c_int64, _P],
+    "keep_rmsnorm_grad_workspace_bytes": [c_int64, c_int64],
+    "keep_route_experts": [_P, c_int, c_int64, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int, c_float, _P, _P, _P,
+                           _P],
+    "keep_route_experts_grad": [_P, c_int, c_int64, c_int64, c_int64, _P, _P, c_int, c_int, c_float, _P, _P],
+    "keep_linear": [_P, c_int64, c_int, c_int64, _P, c_int64, c_int64, c_int64, _P, c_int, c_int, _P, c_int, _P, _P, c_int,
+                    _P, c_int64, _P],
+    "keep_linear_workspace_bytes": [c_int, c_int64, c_int64, c_int64],
+    "keep_linear_q8": [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int64, _P, c_int, c_int, _P, c_int, _P, c_int,
+                       _P, c_int64, _P],
+    "keep_linear_grad": [_P, _P, c_int, _P, c_int64, _P, c_int64, c_int, c_int64, c_int64, c_int64, _P, _P, _P, c_int, _P,
+                         c_int64, _P],
+    "keep_linear_grad_workspace_bytes": [c_int, c_int64, c_int64, c_int64],
     "keep_rht": [_P, c_int, _P, c_int, c_int64, c_int64, _P, c_int, _P],
     "keep_rmsnorm_quant_rht": [_P, c_int, c_int64, c_int64, _P, c_int, c_float, c_int64, c_int, _P, _P, _P, c_int, _P],
     "keep_moe_combine_add": [_P, _P, c_int, _P, c_int, c_int64, _P, c_int, _P],
@@ -127,6 +142,8 @@ _RESTYPE = {"keep_last_error": c_char_p, "keep_moe_tiles_workspace_bytes": c_int
             "keep_vq_grouped_gemm_q8_workspace_bytes": c_int64,
             "keep_lora_workspace_bytes": c_int64, "keep_lora_rank_stride": c_int64,
             "keep_lora_backward_workspace_bytes": c_int64,
+            "keep_rmsnorm_grad_workspace_bytes": c_int64, "keep_linear_workspace_bytes": c_int64,
+            "keep_linear_grad_workspace_bytes": c_int64,
             "keep_route_plan_blocks_workspace_bytes": c_int64}
 EXPORTED = tuple(_SIGS)
 

@@ -25,7 +25,9 @@ OBJ = PKG / "_build"
 ARCH = os.environ.get("KEEP_AMD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 SOURCES = ["abi.cpp", "matvec.hip", "moe.hip", "moe_i8.hip", "moe_tiles.hip", "router.hip", "plan.hip", "gemm_q8.hip", "rows.hip", "rht.hip", "layer.hip", "block.hip", "encode.hip",
-           "combine.hip", "dense.hip", "dense_gemm.hip", "lora.hip", "plan_blocks.hip"]
+           "combine.hip", "dense.hip", "dense_gemm.hip", "lora.hip", "plan_blocks.hip", "norm.hip", "norm_grad.hip",
+           "route_experts.hip", "linear.hip", "linear_gemm_bf16.hip", "linear_gemm_f16.hip", "linear_gemm_f32.hip",
+           "linear_gemm_e4m3.hip"]
 FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wno-unused-command-line-argument"]

@@ -1,0 +1,416 @@
+// Dense projections with their epilogue and their gradients:
+//
+//   u = x W^T + b          out = round(residual + act(u))
+//   du = round(dy act'(u)) dx = du W        dW = du^T x        db = sum of du's rows (before its rounding)
+//
+// 8-bit operands (e4m3): x W^T with a float32 scale per 128 values of a row of x and per 128 x 128 values of W, no gradients.
+// Sums are held in fp32 on the matrix cores. Up to 16 rows stream W straight to the matrix cores (k_linear_few: a byte of W
+// serves few products, so that HBM bounds it); more run through LDS (linear_gemm_dev.h), in slices of the summed index
+// (k_linear_join) where there are fewer tiles than CUs. u is kept for the gradient in x's dtype and du rounded to it: the
+// matrix cores take 16-bit operands, and both roundings are half a step of the dtype that dy has.
+#include <algorithm>
+
+#include "linear_dev.h"
+#include "parts_dev.h"
+
+namespace keep {
+
+void linear_gemm_bf16(const LinearGemmArgs& a, int mode, int tile, hipStream_t s);
+void linear_gemm_f16(const LinearGemmArgs& a, int mode, int tile, hipStream_t s);
+void linear_gemm_f32(const LinearGemmArgs& a, int mode, int tile, hipStream_t s);
+void linear_gemm_e4m3(const LinearGemmArgs& a, int mode, int tile, hipStream_t s);
+
+static void linear_gemm(const LinearGemmArgs& a, int dtype, int mode, int tile, hipStream_t s) {
+  if (dtype == KEEP_BF16) linear_gemm_bf16(a, mode, tile, s);
+  else if (dtype == KEEP_F16) linear_gemm_f16(a, mode, tile, s);
+  else if (dtype == KEEP_F32) linear_gemm_f32(a, mode, tile, s);
+  else linear_gemm_e4m3(a, mode, tile, s);
+}
+
+static int64_t linear_size(int dtype) { return dtype == KEEP_E4M3 ? 1 : dtype_size(dtype); }
+
+// ------------------------------------------------------------------ few rows
+
+constexpr int LINEAR_FEW = 16;  // rows
+
+// WAVES waves share 16 rows of W (and of x): wave s takes the s-th share of the summed index and the shares are added in order
+// through LDS. Lane (c, q) holds W row n0 + c, so that its results are outputs n0 + 4 q + v of row c.
+template <typename T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinearGemmArgs a) {
+  constexpr int SZ = sizeof(T), LB = SZ == 1 ? 32 : 16;  // bytes of a lane's piece
+  constexpr int VL = LB / SZ, KS = 4 * VL, UN = SZ == 1 ? 4 : 8;
+  __shared__ float4 red[WAVES][64];
+  const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * 16, j0 = (int64_t)blockIdx.y * 16;
+  const char* xrow = (const char*)a.pj + min(j0 + c, a.nj - 1) * a.ldj * SZ + q * LB;
+  const char* wrow = (const char*)a.pi + min(n0 + c, a.ni - 1) * a.ldi * SZ + q * LB;
+  const int64_t kb = (a.nk + KS - 1) / KS;  // (8-bit: a scale's span each)
+  const float* xs = SZ == 1 ? a.sj + min(j0 + c, a.nj - 1) * kb : nullptr;
+  const float* ws = SZ == 1 ? a.si + n0 / 128 * kb : nullptr;
+  const int steps = (int)kb, per = (steps + WAVES - 1) / WAVES;
+  const int s0 = min(steps, wv * per), s1 = min(steps, s0 + per), whole = min(s1, (int)(a.nk / KS));
+  f4 acc{0.f, 0.f, 0.f, 0.f};
+  const auto product = [&](const uint4* i, const uint4* j, float scale) {
+    if constexpr (SZ == 1) {
+      linear_h8 fi[4], fj[4];
+      linear_e4m3(i[0], i[1], fi);
+      linear_e4m3(j[0], j[1], fj);
+      f4 p{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < 4; ++t) p = __builtin_amdgcn_mfma_f32_16x16x32_f16(fi[t], fj[t], p, 0, 0, 0);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[v] = fmaf(p[v], scale, acc[v]);
+    } else {
+      acc = dense_mfma<T>(i[0], j[0], acc);
+    }
+  };
+  constexpr int P = LB / 16;
+  int s = s0;
+  for (; s + UN <= whole; s += UN) {
+    uint4 fi[UN][P], fj[UN][P];
+    float sc[UN];
+#pragma unroll
+    for (int d = 0; d < UN; ++d) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        fi[d][p] = dense_ld16((const uint8_t*)wrow, (s + d) * (KS * SZ) + p * 16);
+        fj[d][p] = dense_ld16((const uint8_t*)xrow, (s + d) * (KS * SZ) + p * 16);
+      }
+      sc[d] = SZ == 1 ? xs[s + d] * ws[s + d] : 1.f;
+    }
+#pragma unroll
+    for (int d = 0; d < UN; ++d) product(fi[d], fj[d], sc[d]);
+  }
+  for (; s < s1; ++s) {
+    uint4 fi[P], fj[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const bool in = (int64_t)s * KS + (q * LB + p * 16) / SZ < a.nk;  // (pieces are whole or past the end)
+      const int64_t at = (int64_t)s * (KS * SZ) + p * 16;
+      fi[p] = in ? dense_ld16((const uint8_t*)wrow, at) : make_uint4(0u, 0u, 0u, 0u);
+      fj[p] = in ? dense_ld16((const uint8_t*)xrow, at) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    product(fi, fj, SZ == 1 ? xs[s] * ws[s] : 1.f);
+  }
+  red[wv][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (wv > 0) return;
+  float f[4] = {0.f, 0.f, 0.f, 0.f}, b[4];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    const float4 p = red[w][lane];
+    f[0] += p.x; f[1] += p.y; f[2] += p.z; f[3] += p.w;
+  }
+  const int64_t n = n0 + q * 4;
+  if (j0 + c >= a.nj || n >= a.ni) return;
+  a.e.load_bias<4>(n, a.ni - n, b);
+  a.e.store<4>(j0 + c, a.ni, n, a.ni - n, f, b);
+}
+
+template <typename T>
+static void linear_few_launch(const LinearGemmArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.ni + 15) / 16), (unsigned)((a.nj + 15) / 16));
+  if (grid.x * grid.y <= 256) hipLaunchKernelGGL((k_linear_few<T, 16>), grid, dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL((k_linear_few<T, 8>), grid, dim3(512), 0, s, a);
+}
+
+static void linear_few(const LinearGemmArgs& a, int dtype, hipStream_t s) {
+  if (dtype == KEEP_BF16) linear_few_launch<bf16s>(a, s);
+  else if (dtype == KEEP_F16) linear_few_launch<_Float16>(a, s);
+  else if (dtype == KEEP_F32) linear_few_launch<float>(a, s);
+  else linear_few_launch<e4m3s>(a, s);
+}
+
+// ------------------------------------------------------------------ slices added
+
+__global__ __launch_bounds__(256) void k_linear_join(LinearGemmArgs a) {
+  const int64_t groups = (a.ni + 7) / 8, n = a.nj * groups;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / groups, col = (i - row * groups) * 8;
+    float f[8], b[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) f[u] = 0.f;
+    for (int s = 0; s < a.slices; ++s) {
+      float p[8];
+      linear_ld<float, 8>(a.part + (s * a.nj + row) * a.ni + col, a.ni - col, p, a.ni % 4 == 0);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f[u] += p[u];
+    }
+    a.e.load_bias<8>(col, a.ni - col, b);
+    a.e.store<8>(row, a.ni, col, a.ni - col, f, b);
+  }
+}
+
+struct LinearPlan {
+  int tile, slices;
+};
+
+// The tile (rows of J, of I 128; 256: 256 x 256, 8-bit 128 x 256) and the slices of a product. 0: the kernel for few rows.
+static LinearPlan linear_plan(int dtype, int mode, int64_t ni, int64_t nj, int64_t nk) {
+  if (mode == LINEAR_FORWARD && nj <= LINEAR_FEW) return {0, 1};
+  const auto tiles = [&](int64_t bi, int64_t bj) { return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj); };
+  const int64_t large = dtype == KEEP_F32 ? 0 : dtype == KEEP_E4M3 ? tiles(256, 128) : tiles(256, 256);
+  int tile = 64;
+  if (large >= 192) tile = 256;
+  else if (nj > 64 && tiles(128, 128) >= 128) tile = 128;
+  const int64_t n = tile == 256 ? large : tile == 128 ? tiles(128, 128) : tiles(128, 64);
+  const int64_t steps = (nk * linear_size(dtype) + 127) / 128;
+  // slices of at least eight steps while the tiles leave CUs without work
+  const int64_t slices = tile == 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>({512 / n, steps / 8, 32}));
+  return {tile, (int)slices};
+}
+
+static int64_t linear_part_bytes(const LinearPlan& p, int64_t ni, int64_t nj) {
+  return p.slices > 1 ? p.slices * ni * nj * 4 : 0;
+}
+
+static bool linear_gemm_fits(const LinearPlan& p, int64_t ni, int64_t nj) {
+  const int64_t bi = p.tile == 0 ? 16 : p.tile == 256 ? 256 : 128, bj = p.tile == 0 ? 16 : std::min(p.tile, 128);
+  return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj) <= (int64_t(1) << 22) / p.slices;
+}
+
+static void linear_product(LinearGemmArgs a, int dtype, int mode, const LinearPlan& p, void* part, hipStream_t s) {
+  a.slices = p.slices;
+  a.part = (float*)part;
+  if (p.tile == 0) {
+    linear_few(a, dtype, s);
+    return;
+  }
+  linear_gemm(a, dtype, mode, p.tile, s);
+  if (p.slices > 1) {
+    const int64_t n = a.nj * ((a.ni + 7) / 8);
+    hipLaunchKernelGGL(k_linear_join, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)), dim3(256), 0, s, a);
+  }
+}
+
+// ------------------------------------------------------------------ the gradient before the products
+
+struct LinearDuArgs {
+  const void *dy, *u;
+  int act;
+  int64_t M, N, ld;  // ld: of du, whole 16-byte pieces, zeros behind the columns
+  void* du;          // or null
+  float* part;       // [gridDim.y][N] sums of du, or null
+  int64_t rows;      // of a block
+};
+
+// Threads of 8 neighbouring columns, 8 rows at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void k_linear_du(LinearDuArgs a) {
+  __shared__ float red[8][32][8 + 1];
+  const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5;
+  const int64_t col = ((int64_t)blockIdx.x * 32 + cg) * 8;
+  const int64_t r0 = (int64_t)blockIdx.y * a.rows, r1 = min(a.M, r0 + a.rows);
+  const bool vec = a.N % 8 == 0 && ((uintptr_t)a.dy & 15) == 0 && (!a.u || ((uintptr_t)a.u & 15) == 0);
+  float sum[8] = {};
+  if (col < a.ld) {
+    for (int64_t r = r0 + rg; r < r1; r += 8) {
+      float d[8], u[8];
+      const int64_t left = max(a.N - col, (int64_t)0);
+      linear_ld<T, 8>((const T*)a.dy + r * a.N + col, left, d, vec);
+      if (a.act) {
+        linear_ld<T, 8>((const T*)a.u + r * a.N + col, left, u, vec);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] *= linear_slope(u[i], a.act);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += d[i];
+      if (a.du) {
+        if (left < 8)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] = i < left ? d[i] : 0.f;
+        dense_st<T, 8>((T*)a.du + r * a.ld + col, a.ld - col, d, true);
+      }
+    }
+  }
+  if (!a.part) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[rg][cg][i] = sum[i];
+  __syncthreads();
+  // a thread a column: the block's 256
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= a.N) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v += red[k][threadIdx.x >> 3][threadIdx.x & 7];
+  a.part[blockIdx.y * a.N + n] = v;
+}
+
+constexpr int64_t LINEAR_MAX = int64_t(1) << 20;  // N and K: a tile's rows then lie within 32-bit offsets
+
+// Row blocks of k_linear_du: enough for the CUs, a few thousand rows at most each.
+static int64_t linear_du_blocks(int64_t M, int64_t N) {
+  const int64_t strips = (N + 255) / 256;
+  return std::max<int64_t>(1, std::min<int64_t>({(M + 31) / 32, (1024 + strips - 1) / strips, 512}));
+}
+
+static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+static int64_t linear_pitch(int64_t n, int64_t size) { return (n * size + 15) / 16 * 16 / size; }
+
+struct LinearGradPlan {
+  LinearPlan rows, weight;
+  int64_t du, part, db, bytes;  // offsets
+};
+
+static LinearGradPlan linear_grad_plan(int dtype, int64_t M, int64_t N, int64_t K) {
+  LinearGradPlan p{};
+  const int64_t size = linear_size(dtype);
+  p.rows = linear_plan(dtype, LINEAR_ROWS, K, M, N);
+  p.weight = linear_plan(dtype, LINEAR_WEIGHT, K, N, M);
+  p.part = up256(M * linear_pitch(N, size) * size);
+  p.db = p.part + up256(std::max(linear_part_bytes(p.rows, K, M), linear_part_bytes(p.weight, K, N)));
+  p.bytes = p.db + up256(linear_du_blocks(M, N) * N * 4);
+  return p;
+}
+
+static bool linear_vec(std::initializer_list<const void*> ps, int64_t n) {
+  if (n % 8) return false;
+  for (const void* p : ps)
+    if (!aligned(p, 16)) return false;
+  return true;
+}
+
+// What forward calls ask beside their operands.
+static int linear_epilogue(LinearEpilogue& e, int64_t M, int64_t N, const void* bias, int bdt, int act, const void* res,
+                           int rdt, void* u, int udt, void* out, int odt) {
+  KEEP_REQUIRE((!bias || dtype_ok(bdt)) && (!res || dtype_ok(rdt)) && dtype_ok(odt), "bad dtype enum");
+  KEEP_REQUIRE(act >= LINEAR_NONE && act <= LINEAR_GELU_TANH, "bad activation %d", act);
+  KEEP_REQUIRE(aligned(out, dtype_size(odt)) && (!bias || aligned(bias, dtype_size(bdt))) &&
+                   (!res || aligned(res, dtype_size(rdt))) && (!u || aligned(u, dtype_size(udt))),
+               "misaligned pointer");
+  e.bias = bias; e.bdt = bdt; e.act = act; e.res = res; e.rdt = rdt; e.u = u; e.udt = udt; e.out = out; e.odt = odt;
+  e.vec = linear_vec({bias, res, u, out}, N);
+  return KEEP_OK;
+}
+
+static int linear_sizes(int64_t M, int64_t N, int64_t K) {
+  KEEP_REQUIRE_DIMS(M, N, K);
+  KEEP_REQUIRE(N >= 1 && K >= 1 && N <= LINEAR_MAX && K <= LINEAR_MAX, "N and K must be in 1..2^20");
+  KEEP_REQUIRE(M <= (int64_t(1) << 40) / std::max(N, K) / 4, "too many values");  // more than a GPU holds
+  return KEEP_OK;
+}
+
+// Rows of n values at a pitch of ld: the kernels read whole 16-byte pieces.
+#define KEEP_REQUIRE_PITCH(p, ld, n, size, what)                                                         \
+  KEEP_REQUIRE(aligned(p, 16) && (ld) >= (n) && (ld) < KEEP_DIM_LIMIT && (ld) <= 4 * LINEAR_MAX &&       \
+                   ((ld) * (size)) % 16 == 0,                                                            \
+               what " must be 16-byte aligned, its pitch at least a row and a multiple of 16 bytes")
+
+}  // namespace keep
+
+using namespace keep;
+
+extern "C" int64_t keep_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (!(dtype_ok(dtype) || dtype == KEEP_E4M3) || linear_sizes(M, N, K) != KEEP_OK || M == 0) return 0;
+  return linear_part_bytes(linear_plan(dtype, LINEAR_FORWARD, N, M, K), N, M);
+}
+
+static int linear_forward(LinearGemmArgs& a, int dtype, void* ws, int64_t ws_bytes, hipStream_t s) {
+  const LinearPlan p = linear_plan(dtype, LINEAR_FORWARD, a.ni, a.nj, a.nk);
+  const int64_t need = linear_part_bytes(p, a.ni, a.nj);
+  KEEP_REQUIRE(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need),
+               "the workspace must hold %lld bytes, 16-byte aligned", (long long)need);
+  KEEP_REQUIRE(linear_gemm_fits(p, a.ni, a.nj), "too many outputs");
+  linear_product(a, dtype, LINEAR_FORWARD, p, ws, s);
+  return KEEP_OK;
+}
+
+extern "C" int keep_linear(const void* x, int64_t x_ld, int dtype, int64_t M, const void* weight, int64_t w_ld, int64_t N,
+                           int64_t K, const void* bias, int bias_dtype, int act, const void* residual,
+                           int residual_dtype, void* u, void* out, int out_dtype, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+  if (const int rc = linear_sizes(M, N, K)) return rc;
+  KEEP_REQUIRE(dtype_ok(dtype), "bad dtype enum");
+  if (M == 0) return KEEP_OK;
+  KEEP_REQUIRE(x && weight && out, "null pointer argument");
+  KEEP_REQUIRE_PITCH(x, x_ld, K, linear_size(dtype), "x");
+  KEEP_REQUIRE_PITCH(weight, w_ld, K, linear_size(dtype), "weight");
+  LinearGemmArgs a{};
+  a.pi = weight; a.pj = x; a.ldi = w_ld; a.ldj = x_ld; a.ni = N; a.nj = M; a.nk = K;
+  if (const int rc = linear_epilogue(a.e, M, N, bias, bias_dtype, act, residual, residual_dtype, u, dtype, out, out_dtype))
+    return rc;
+  if (const int rc = linear_forward(a, dtype, workspace, workspace_bytes, (hipStream_t)stream)) return rc;
+  return launch_status("keep_linear");
+}
+
+extern "C" int keep_linear_q8(const void* x, int64_t x_ld, const float* x_scales, int64_t M, const void* weight,
+                              int64_t w_ld, const float* w_scales, int64_t N, int64_t K, const void* bias,
+                              int bias_dtype, int act, const void* residual, int residual_dtype, void* out,
+                              int out_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = linear_sizes(M, N, K)) return rc;
+  if (M == 0) return KEEP_OK;
+  KEEP_REQUIRE(x && weight && x_scales && w_scales && out, "null pointer argument");
+  KEEP_REQUIRE(aligned(x_scales, 4) && aligned(w_scales, 4), "misaligned pointer");
+  KEEP_REQUIRE_PITCH(x, x_ld, K, 1, "x");
+  KEEP_REQUIRE_PITCH(weight, w_ld, K, 1, "weight");
+  LinearGemmArgs a{};
+  a.pi = weight; a.pj = x; a.ldi = w_ld; a.ldj = x_ld; a.ni = N; a.nj = M; a.nk = K;
+  a.si = w_scales; a.sj = x_scales;
+  if (const int rc = linear_epilogue(a.e, M, N, bias, bias_dtype, act, residual, residual_dtype, nullptr, 0, out, out_dtype))
+    return rc;
+  if (const int rc = linear_forward(a, KEEP_E4M3, workspace, workspace_bytes, (hipStream_t)stream)) return rc;
+  return launch_status("keep_linear_q8");
+}
+
+extern "C" int64_t keep_linear_grad_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+  if (!dtype_ok(dtype) || linear_sizes(M, N, K) != KEEP_OK || M == 0) return 0;
+  return linear_grad_plan(dtype, M, N, K).bytes;
+}
+
+extern "C" int keep_linear_grad(const void* dy, const void* u, int act, const void* x, int64_t x_ld, const void* weight,
+                                int64_t w_ld, int dtype, int64_t M, int64_t N, int64_t K, void* dx, void* dweight,
+                                void* dbias, int bias_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (const int rc = linear_sizes(M, N, K)) return rc;
+  KEEP_REQUIRE(dtype_ok(dtype) && (!dbias || dtype_ok(bias_dtype)), "bad dtype enum");
+  KEEP_REQUIRE(act >= LINEAR_NONE && act <= LINEAR_GELU_TANH, "bad activation %d", act);
+  if (M == 0) return KEEP_OK;
+  const int64_t size = linear_size(dtype);
+  KEEP_REQUIRE(dy && (dx || dweight || dbias) && (u || !act) && (x || !dweight) && (weight || !dx),
+               "null pointer argument");
+  KEEP_REQUIRE(aligned(dy, size) && aligned(u, size) && aligned(dx, size) && aligned(dweight, size) &&
+                   (!dbias || aligned(dbias, dtype_size(bias_dtype))),
+               "misaligned pointer");
+  if (dweight) KEEP_REQUIRE_PITCH(x, x_ld, K, size, "x");
+  if (dx) KEEP_REQUIRE_PITCH(weight, w_ld, K, size, "weight");
+  const LinearGradPlan p = linear_grad_plan(dtype, M, N, K);
+  KEEP_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= p.bytes,
+               "the workspace must hold %lld bytes, 256-byte aligned", (long long)p.bytes);
+  KEEP_REQUIRE(linear_gemm_fits(p.rows, K, M) && linear_gemm_fits(p.weight, K, N), "too many outputs");
+  hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  // du: dy itself where no activation changes it and its rows are whole pieces
+  const bool same = !act && (N * size) % 16 == 0 && aligned(dy, 16);
+  const bool products = dx || dweight;
+  const void* du = same ? dy : ws + p.du;
+  if (dbias || (products && !same)) {
+    LinearDuArgs d{};
+    d.dy = dy; d.u = u; d.act = act; d.M = M; d.N = N; d.ld = linear_pitch(N, size);
+    d.du = products && !same ? ws + p.du : nullptr;
+    d.part = dbias ? (float*)(ws + p.db) : nullptr;
+    const int64_t blocks = linear_du_blocks(M, N);
+    d.rows = (M + blocks - 1) / blocks;
+    const dim3 grid((unsigned)((N + 255) / 256), (unsigned)blocks);
+    if (dtype == KEEP_F32) hipLaunchKernelGGL(k_linear_du<float>, grid, dim3(256), 0, s, d);
+    else if (dtype == KEEP_F16) hipLaunchKernelGGL(k_linear_du<_Float16>, grid, dim3(256), 0, s, d);
+    else hipLaunchKernelGGL(k_linear_du<bf16s>, grid, dim3(256), 0, s, d);
+    if (dbias) parts_sum(d.part, blocks, N, dbias, bias_dtype, s);
+  }
+  LinearGemmArgs a{};
+  a.e.odt = dtype;
+  if (dx) {
+    a.pi = weight; a.ldi = w_ld; a.pj = du; a.ldj = linear_pitch(N, size);
+    a.ni = K; a.nj = M; a.nk = N;
+    a.e.out = dx;
+    a.e.vec = linear_vec({dx}, K);
+    linear_product(a, dtype, LINEAR_ROWS, p.rows, ws + p.part, s);
+  }
+  if (dweight) {
+    a.pi = x; a.ldi = x_ld; a.pj = du; a.ldj = linear_pitch(N, size);
+    a.ni = K; a.nj = N; a.nk = M;
+    a.e.out = dweight;
+    a.e.vec = linear_vec({dweight}, K);
+    linear_product(a, dtype, LINEAR_WEIGHT, p.weight, ws + p.part, s);
+  }
+  return launch_status("keep_linear_grad");
+}

@@ -1,0 +1,148 @@
+// Gradients of the root-mean-square norm with the residual's addition (norm.hip): with g = dy w, c = sum(g h) over the row
+// and dh the gradient of h,
+//   d = r (g - h r^2 c / n) + dh,  dx = round(d),  dresidual = round(d),  dw = sum over the rows of dy h r
+// Bound by HBM: h, dy and dh are read once, dx (and dresidual, where its dtype is another) written once. dw is summed in a
+// fixed order: per block in registers, then over the blocks.
+#include "norm_dev.h"
+#include "parts_dev.h"
+
+namespace keep {
+
+struct NormGradArgs {
+  const void *h, *w, *dy, *dh;  // dh: or null
+  int wdt;
+  const float* rstd;
+  int64_t T;
+  int n;
+  void *dx, *dres;  // either null
+  float* part;      // [blocks][n] sums of the weight's gradient, or null
+};
+
+// H: type of h, dh and dresidual; X: of dy and dx. A block takes every gridDim-th group of rows and adds its share of dw in
+// registers, so that the shares that are left for k_parts_sum are as many as blocks.
+template <typename X, typename H, int TPR, int NV, bool EVEN>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm_grad(NormGradArgs a) {
+  constexpr int BT = TPR < 256 ? 256 : TPR, RPB = BT / TPR;
+  __shared__ float red[BT / 64];
+  __shared__ float other[RPB > 1 ? TPR * NV * 8 : 1];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, n = a.n;
+  float dw[NV][8];
+#pragma unroll
+  for (int v = 0; v < NV; ++v)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) dw[v][u] = 0.f;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.T; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t row = r0 + sub;
+    const bool live = row < a.T;
+    const int64_t at = (live ? row : 0) * n;
+    float h[NV][8], g[NV][8];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) norm_ld<EVEN>((const H*)a.h + at, (v * TPR + t) * 8, n, h[v]);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) norm_ld<EVEN>((const X*)a.dy + at, (v * TPR + t) * 8, n, g[v]);
+    const float r = live ? a.rstd[row] : 0.f;
+    float c = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float w[8];
+      norm_weight<EVEN>(a.w, a.wdt, (v * TPR + t) * 8, n, w);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (live) dw[v][u] = fmaf(g[v][u], h[v][u] * r, dw[v][u]);
+        g[v][u] *= w[u];
+        c = fmaf(g[v][u], h[v][u], c);
+      }
+    }
+    c = norm_sum<TPR, BT>(c, red);
+    if (!live || !(a.dx || a.dres)) continue;
+    const float k = r * r * (c / (float)n);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = (v * TPR + t) * 8;
+      float d[8];
+      if (a.dh) norm_ld<EVEN>((const H*)a.dh + at, i, n, d);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float e = r * fmaf(-h[v][u], k, g[v][u]);
+        d[u] = a.dh ? e + d[u] : e;
+      }
+      if (a.dx) norm_st<EVEN>((X*)a.dx + at, i, n, d);
+      if (a.dres) norm_st<EVEN>((H*)a.dres + at, i, n, d);
+    }
+  }
+  if (!a.part) return;
+  if constexpr (RPB > 1) {
+    for (int s = 1; s < RPB; ++s) {
+      __syncthreads();
+      if (sub == s)
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) other[(v * 8 + u) * TPR + t] = dw[v][u];
+      __syncthreads();
+      if (sub == 0)
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) dw[v][u] += other[(v * 8 + u) * TPR + t];
+    }
+    if (sub > 0) return;
+  }
+#pragma unroll
+  for (int v = 0; v < NV; ++v) norm_st<EVEN>(a.part + (int64_t)blockIdx.x * n, (v * TPR + t) * 8, n, dw[v]);
+}
+
+// Rows of a block of k_rmsnorm_grad, and its blocks: two per CU.
+static int norm_rows_per_block(int64_t n) { return n <= 2048 ? 4 : 1; }
+static int64_t norm_parts(int64_t T, int64_t n) {
+  const int64_t rpb = norm_rows_per_block(n);
+  return std::min<int64_t>((T + rpb - 1) / rpb, 512);
+}
+
+template <typename X, typename H>
+static void norm_grad_launch(const NormGradArgs& a, int64_t blocks, hipStream_t s) {
+  norm_by_width(a.n, [&](auto tpr, auto nv, auto even) {
+    constexpr int TPR = decltype(tpr)::value, BT = TPR < 256 ? 256 : TPR;
+    hipLaunchKernelGGL((k_rmsnorm_grad<X, H, TPR, decltype(nv)::value, decltype(even)::value>), dim3((unsigned)blocks), dim3(BT), 0, s, a);
+  });
+}
+
+}  // namespace keep
+
+using namespace keep;
+
+extern "C" int64_t keep_rmsnorm_grad_workspace_bytes(int64_t T, int64_t n) {
+  if (!dims_ok({T, n}) || n > NORM_MAX) return 0;
+  return norm_parts(T, n) * n * 4;
+}
+
+extern "C" int keep_rmsnorm_grad(const void* h, int h_dtype, const void* dy, int dy_dtype, const void* dh,
+                                 const float* rstd, int64_t T, int64_t n, const void* weight, int weight_dtype,
+                                 void* dx, void* dresidual, void* dweight, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+  KEEP_REQUIRE_NORM(T, n, 0.f);
+  KEEP_REQUIRE(dtype_ok(h_dtype) && dtype_ok(dy_dtype) && (!weight || dtype_ok(weight_dtype)), "bad dtype enum");
+  KEEP_REQUIRE(h_dtype == dy_dtype || h_dtype == KEEP_F32, "h must have dy's dtype or float32");
+  if (T == 0) return KEEP_OK;
+  KEEP_REQUIRE(h && dy && rstd && (dx || dresidual || dweight) && (weight || !dweight), "null pointer argument");
+  KEEP_REQUIRE(aligned(h, dtype_size(h_dtype)) && aligned(dy, dtype_size(dy_dtype)) &&
+                   aligned(dh, dtype_size(h_dtype)) && aligned(rstd, 4) && aligned(dx, dtype_size(dy_dtype)) &&
+                   aligned(dresidual, dtype_size(h_dtype)) &&
+                   (!weight || (aligned(weight, dtype_size(weight_dtype)) &&
+                                aligned(dweight, dtype_size(weight_dtype)))),
+               "misaligned pointer");
+  const int64_t blocks = norm_parts(T, n);
+  KEEP_REQUIRE(!dweight || (workspace && aligned(workspace, 4) && workspace_bytes >= blocks * n * 4),
+               "the workspace must hold %lld bytes", (long long)(blocks * n * 4));
+  NormGradArgs a{};
+  a.h = h; a.w = weight; a.dy = dy; a.dh = dh; a.wdt = weight_dtype; a.rstd = rstd; a.T = T; a.n = (int)n;
+  a.dx = dx; a.dres = dresidual; a.part = dweight ? (float*)workspace : nullptr;
+  hipStream_t s = (hipStream_t)stream;
+  if (dy_dtype == KEEP_F32) norm_grad_launch<float, float>(a, blocks, s);
+  else if (dy_dtype == KEEP_F16 && h_dtype == KEEP_F32) norm_grad_launch<_Float16, float>(a, blocks, s);
+  else if (dy_dtype == KEEP_F16) norm_grad_launch<_Float16, _Float16>(a, blocks, s);
+  else if (h_dtype == KEEP_F32) norm_grad_launch<bf16s, float>(a, blocks, s);
+  else norm_grad_launch<bf16s, bf16s>(a, blocks, s);
+  if (dweight) parts_sum(a.part, blocks, n, dweight, weight_dtype, s);
+  return launch_status("keep_rmsnorm_grad");
+}

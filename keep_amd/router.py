@@ -14,9 +14,10 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from keep_amd import _lib
-from keep_amd.ops import _device_of, _ptr, _stream, _to_dev
+from keep_amd import _grad, _lib
+from keep_amd.ops import _DT, _dense_device, _device_of, _on, _ptr, _stream, _to_dev
 
 OFF = -1.0e30  # bias of an absent expert (reference omlx_routed.py:40)
 
@@ -107,3 +108,89 @@ def resident_bias(resident_mask, correction_bias=None) -> torch.Tensor:
     base = torch.zeros(m.shape, dtype=torch.float32, device=m.device) if correction_bias is None else \
         correction_bias.to(torch.float32).to(m.device)
     return torch.where(m, base, torch.full_like(base, OFF))
+
+
+class ExpertRoutes(NamedTuple):
+    idx: torch.Tensor  # [T, k] int32 chosen experts, the largest key first
+    weight: torch.Tensor  # [T, k] float32 routing weights
+    load: torch.Tensor | None  # [E] int32 tokens per expert (count_load)
+
+
+def _route(z, k: int, bias, groups: int, topk_groups: int, func: int, renormalize: bool, scale: float, count: bool):
+    T, E = z.shape
+    idx = torch.empty((T, k), dtype=torch.int32, device=z.device)
+    weight = torch.empty((T, k), dtype=torch.float32, device=z.device)
+    load = torch.zeros(E, dtype=torch.int32, device=z.device) if count else None
+    if T:
+        _lib.call("keep_route_experts", z.data_ptr(), _DT[z.dtype], T, E, k, _ptr(bias), groups, topk_groups, func,
+                  int(renormalize), scale, idx.data_ptr(), weight.data_ptr(), _ptr(load), _stream(z.device))
+    return idx, weight, load
+
+
+class _RouteExperts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, k, bias, groups, topk_groups, func, renormalize, scale, count):
+        z = z.contiguous()
+        idx, weight, load = _route(z, k, bias, groups, topk_groups, func, renormalize, scale, count)
+        ctx.save_for_backward(z, idx)
+        ctx.args = (func, int(renormalize), scale)
+        ctx.mark_non_differentiable(*(t for t in (idx, load) if t is not None))
+        return idx, weight, load
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _, dweight, __):
+        z, idx = ctx.saved_tensors
+        dz, dw = torch.empty_like(z), dweight.float().contiguous()
+        if z.shape[0]:
+            with _on(z.device):
+                _lib.call("keep_route_experts_grad", z.data_ptr(), _DT[z.dtype], *z.shape, idx.shape[1], idx.data_ptr(),
+                          dw.data_ptr(), *ctx.args, dz.data_ptr(), _stream(z.device))
+        return (dz,) + (None,) * 8
+
+
+def route_experts(logits: torch.Tensor, k: int, *, bias: torch.Tensor | None = None, score_func: str = "softmax",
+                  groups: int = 1, topk_groups: int | None = None, renormalize: bool = True, route_scale: float = 1.0,
+                  count_load: bool = False) -> ExpertRoutes:
+    """Each token's experts from the router's ``logits [T, E]`` (any float dtype), with gradients of the logits.
+
+    Keys are ``score + bias`` (``bias [E]`` float32 balances the choice and takes no gradient). With ``groups`` of
+    ``E / groups`` neighbouring experts, the ``topk_groups`` groups of the largest sum of their two largest keys are
+    kept, and the ``k`` largest keys in them chosen; the lower index first among equals, NaN as -inf. Weights are the
+    chosen experts' scores, renormalised to sum to 1 (``+1e-20``) with ``renormalize``, times ``route_scale``. The choice
+    does not depend on float32's rounding: without a bias it is the order of the logits, with one that of keys formed in
+    64 bits. ``count_load`` counts the tokens of every expert (what a balancing bias is adjusted by).
+
+    ``router_dual_topk`` is the residency cache's form: a served and a demanded choice, no groups, no gradients.
+    """
+
+    device = _dense_device(logits, bias)
+    if logits.ndim != 2 or logits.dtype not in _DT:
+        raise ValueError("logits must be 2D [tokens, experts] in float32, float16 or bfloat16, found "
+                         f"{tuple(logits.shape)} in {logits.dtype}")
+    if score_func not in _lib.SCORE_FUNCS:
+        raise ValueError(f"score_func must be one of {sorted(_lib.SCORE_FUNCS)}")
+    E = logits.shape[1]
+    if not 1 <= E <= 1024:
+        raise ValueError(f"route_experts serves 1..1024 experts, found {E}")
+    if not 1 <= groups <= 64 or E % groups:
+        raise ValueError(f"groups must be in 1..64 and divide {E}, found {groups}")
+    tg = groups if topk_groups is None else topk_groups
+    if not 1 <= tg <= groups:
+        raise ValueError(f"topk_groups must be in 1..{groups}, found {tg}")
+    if not 1 <= k <= min(32, tg * (E // groups)):
+        raise ValueError(f"k must be in 1..min(32, {tg * (E // groups)}), found {k}")
+    if bias is not None:
+        if tuple(bias.shape) != (E,):
+            raise ValueError(f"bias must have shape ({E},), found {tuple(bias.shape)}")
+        if _grad.wanted(bias):
+            raise ValueError("the bias takes no gradient: it enters the choice alone")
+        bias = _to_dev(bias.detach(), device, torch.float32)
+    args = (int(k), bias, int(groups), int(tg), _lib.SCORE_FUNCS[score_func], bool(renormalize), float(route_scale),
+            bool(count_load))
+    with _on(device):
+        if not _grad.wanted(logits):
+            return ExpertRoutes(*_route(logits.contiguous(), *args))
+        _grad.check_capture(logits)
+        idx, weight, load = _RouteExperts.apply(logits, *args)
+        return ExpertRoutes(idx, _grad.mark(weight), load)
