@@ -58,7 +58,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm(NormArgs a) {
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) h[v][u] = to_float(from_float<R>(p[v][u] + h[v][u]));
+        for (int u = 0; u < 8; u += 2) {
+          h[v][u] += p[v][u];
+          h[v][u + 1] += p[v][u + 1];
+          if constexpr (sizeof(R) == 2) {  // the stream as it is kept
+            const uint32_t w = norm_pair<R>(h[v][u], h[v][u + 1]);
+            h[v][u] = pair_lo<PairOf<R>::value>(w);
+            h[v][u + 1] = pair_hi<PairOf<R>::value>(w);
+          }
+        }
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v)
@@ -82,27 +90,21 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm(NormArgs a) {
       if constexpr (!QUANT) {
         if (live) norm_st<EVEN>((X*)a.y + at, i, n, h[v]);
       } else {
-        float top = 0.f;
-        bool nan = false;
+        // a maximum of the bits, which a NaN outranks
+        uint32_t bits = 0u;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          top = fmaxf(top, fabsf(h[v][u]));
-          nan = nan || h[v][u] != h[v][u];
-        }
-        if (nan) top = __builtin_nanf("");
-        for (int o = 1; o < a.qblock / 8; o <<= 1) {
-          const float other = __shfl_xor(top, o, 64);
-          top = other != other || top != top ? __builtin_nanf("") : fmaxf(top, other);
-        }
+        for (int u = 0; u < 8; ++u) bits = max(bits, __float_as_uint(h[v][u]) & 0x7fffffffu);
+        for (int o = 1; o < a.qblock / 8; o <<= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, o, 64));
+        const float top = __uint_as_float(bits);
         float s = (top < 1e-4f ? 1e-4f : top) / 448.f;
-        if (a.pow2 && s == s && s < __builtin_inff()) s = norm_pow2_ceil(s);
-        uint32_t word[2] = {0u, 0u};
+        if (a.pow2 && s < __builtin_inff()) s = norm_pow2_ceil(s);
+        // times 1 / s: a value is at most 448 and two roundings, which the conversion rounds to 448
+        const float inv = 1.f / s;
+        uint32_t word[2];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          float q = h[v][u] / s;
-          q = q > 448.f ? 448.f : q < -448.f ? -448.f : q;
-          const int b = __builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
-          word[u >> 2] |= ((uint32_t)b & 0xffu) << (8 * (u & 3));
+        for (int u = 0; u < 2; ++u) {
+          int b = __builtin_amdgcn_cvt_pk_fp8_f32(h[v][4 * u] * inv, h[v][4 * u + 1] * inv, 0, false);
+          word[u] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(h[v][4 * u + 2] * inv, h[v][4 * u + 3] * inv, b, true);
         }
         if (live) {
           uint8_t* to = a.q + at + i;

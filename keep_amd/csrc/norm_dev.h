@@ -12,25 +12,50 @@ namespace keep {
 constexpr int NORM_MAX = 16384;  // values of a row: 512 threads of four vectors
 constexpr int64_t NORM_BLOCKS = 1 << 22;  // a launch holds 2^32 threads; more rows go round again
 
+// Two values as a 16-bit pair, rounded to nearest even, NaN kept (bf16: one instruction of this GPU, from_float's bits).
+template <typename T>
+__device__ __forceinline__ uint32_t norm_pair(float lo, float hi) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  if constexpr (__is_same(T, bf16s)) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{lo, hi}, b2_t));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{lo, hi}, h2_t));
+}
+
+// Eight values as they lie in memory, read before they are needed.
+template <typename T>
+struct NormRaw {
+  uint32_t w[2 * sizeof(T)];
+  template <bool EVEN>
+  __device__ __forceinline__ void load(const T* row, int i, int n) {
+    if (EVEN ? i < n : i + 8 <= n) {
+      __builtin_memcpy(w, row + i, 8 * sizeof(T));
+    } else {
+#pragma unroll
+      for (int u = 0; u < (int)(2 * sizeof(T)); ++u) w[u] = 0u;
+      if constexpr (!EVEN) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (i + u < n) {
+            if constexpr (sizeof(T) == 4) w[u] = __builtin_bit_cast(uint32_t, row[i + u]);
+            else w[u / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[i + u]) << (16 * (u & 1));
+          }
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if constexpr (sizeof(T) == 4) f[u] = __uint_as_float(w[u]);
+      else f[u] = (u & 1) ? pair_hi<PairOf<T>::value>(w[u / 2]) : pair_lo<PairOf<T>::value>(w[u / 2]);
+    }
+  }
+};
+
 // Values i .. i + 8 of a row of n, zeros past its end. EVEN: n is a multiple of eight.
 template <bool EVEN, typename T>
 __device__ __forceinline__ void norm_ld(const T* row, int i, int n, float (&f)[8]) {
-  if (EVEN ? i < n : i + 8 <= n) {
-    if constexpr (sizeof(T) == 2) {
-      uint32_t w[4];
-      __builtin_memcpy(w, row + i, 16);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        f[2 * u] = pair_lo<PairOf<T>::value>(w[u]);
-        f[2 * u + 1] = pair_hi<PairOf<T>::value>(w[u]);
-      }
-    } else {
-      __builtin_memcpy(f, row + i, 32);
-    }
-  } else {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) f[u] = !EVEN && i + u < n ? to_float(row[i + u]) : 0.f;
-  }
+  NormRaw<T> r;
+  r.template load<EVEN>(row, i, n);
+  r.get(f);
 }
 
 template <bool EVEN, typename T>
@@ -39,9 +64,7 @@ __device__ __forceinline__ void norm_st(T* row, int i, int n, const float (&f)[8
     if constexpr (sizeof(T) == 2) {
       uint32_t w[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        w[u] = (uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(f[2 * u])) |
-               ((uint32_t)__builtin_bit_cast(uint16_t, from_float<T>(f[2 * u + 1])) << 16);
+      for (int u = 0; u < 4; ++u) w[u] = norm_pair<T>(f[2 * u], f[2 * u + 1]);
       __builtin_memcpy(row + i, w, 16);
     } else {
       __builtin_memcpy(row + i, f, 32);

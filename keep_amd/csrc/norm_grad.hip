@@ -18,11 +18,15 @@ struct NormGradArgs {
   float* part;      // [blocks][n] sums of the weight's gradient, or null
 };
 
-// H: type of h, dh and dresidual; X: of dy and dx. A block takes every gridDim-th group of rows and adds its share of dw in
-// registers, so that the shares that are left for k_parts_sum are as many as blocks.
+// Threads of a block: two rows and more where a row has fewer than 256.
+constexpr int norm_grad_block(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// H: type of h, dh and dresidual; X: of dy and dx. A block takes every gridDim-th group of rows, reads a group's values while
+// it works on the one before, and adds its share of dw in registers, so that the shares that are left for k_parts_sum are as
+// many as blocks.
 template <typename X, typename H, int TPR, int NV, bool EVEN>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm_grad(NormGradArgs a) {
-  constexpr int BT = TPR < 256 ? 256 : TPR, RPB = BT / TPR;
+__global__ __launch_bounds__(norm_grad_block(TPR)) void k_rmsnorm_grad(NormGradArgs a) {
+  constexpr int BT = norm_grad_block(TPR), RPB = BT / TPR;
   __shared__ float red[BT / 64];
   __shared__ float other[RPB > 1 ? TPR * NV * 8 : 1];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, n = a.n;
@@ -31,39 +35,58 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm_grad(NormGrad
   for (int v = 0; v < NV; ++v)
 #pragma unroll
     for (int u = 0; u < 8; ++u) dw[v][u] = 0.f;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.T; r0 += (int64_t)gridDim.x * RPB) {
+  float w[NV][8];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) norm_weight<EVEN>(a.w, a.wdt, (v * TPR + t) * 8, n, w[v]);
+  struct Row {
+    NormRaw<H> h[NV], dh[NV];
+    NormRaw<X> dy[NV];
+    float r;
+  };
+  const auto load = [&](Row& o, int64_t row) {
+    const int64_t at = row < a.T ? row : a.T - 1;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = (v * TPR + t) * 8;
+      o.h[v].template load<EVEN>((const H*)a.h + at * n, i, n);
+      o.dy[v].template load<EVEN>((const X*)a.dy + at * n, i, n);
+      if (a.dh) o.dh[v].template load<EVEN>((const H*)a.dh + at * n, i, n);
+    }
+    o.r = a.rstd[at];
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  Row next;
+  load(next, (int64_t)blockIdx.x * RPB + sub);
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.T; r0 += step) {
     const int64_t row = r0 + sub;
     const bool live = row < a.T;
-    const int64_t at = (live ? row : 0) * n;
+    const int64_t at = row * n;
+    const Row now = next;
+    if (r0 + step < a.T) load(next, row + step);
     float h[NV][8], g[NV][8];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) norm_ld<EVEN>((const H*)a.h + at, (v * TPR + t) * 8, n, h[v]);
-#pragma unroll
-    for (int v = 0; v < NV; ++v) norm_ld<EVEN>((const X*)a.dy + at, (v * TPR + t) * 8, n, g[v]);
-    const float r = live ? a.rstd[row] : 0.f;
     float c = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      float w[8];
-      norm_weight<EVEN>(a.w, a.wdt, (v * TPR + t) * 8, n, w);
+      now.h[v].get(h[v]);
+      now.dy[v].get(g[v]);
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        if (live) dw[v][u] = fmaf(g[v][u], h[v][u] * r, dw[v][u]);
-        g[v][u] *= w[u];
+        if (live) dw[v][u] = fmaf(g[v][u], h[v][u] * now.r, dw[v][u]);
+        g[v][u] *= w[v][u];
         c = fmaf(g[v][u], h[v][u], c);
       }
     }
     c = norm_sum<TPR, BT>(c, red);
     if (!live || !(a.dx || a.dres)) continue;
-    const float k = r * r * (c / (float)n);
+    const float k = now.r * now.r * (c / (float)n);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = (v * TPR + t) * 8;
       float d[8];
-      if (a.dh) norm_ld<EVEN>((const H*)a.dh + at, i, n, d);
+      now.dh[v].get(d);
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const float e = r * fmaf(-h[v][u], k, g[v][u]);
+        const float e = now.r * fmaf(-h[v][u], k, g[v][u]);
         d[u] = a.dh ? e + d[u] : e;
       }
       if (a.dx) norm_st<EVEN>((X*)a.dx + at, i, n, d);
@@ -92,17 +115,39 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm_grad(NormGrad
   for (int v = 0; v < NV; ++v) norm_st<EVEN>(a.part + (int64_t)blockIdx.x * n, (v * TPR + t) * 8, n, dw[v]);
 }
 
-// Rows of a block of k_rmsnorm_grad, and its blocks: two per CU.
-static int norm_rows_per_block(int64_t n) { return n <= 2048 ? 4 : 1; }
+// f(TPR, NV, EVEN) for rows of n values: two vectors a thread, whose row and the one to come are in registers.
+template <typename F>
+static void norm_grad_by_width(int64_t n, F f) {
+  using std::integral_constant;
+  constexpr integral_constant<int, 1> one;
+  constexpr integral_constant<int, 2> two;
+  if (n % 8) {
+    if (n <= 1024) f(integral_constant<int, 64>{}, two, std::false_type{});
+    else if (n <= 4096) f(integral_constant<int, 256>{}, two, std::false_type{});
+    else f(integral_constant<int, 1024>{}, two, std::false_type{});
+  } else if (n <= 512) f(integral_constant<int, 64>{}, one, std::true_type{});
+  else if (n <= 1024) f(integral_constant<int, 64>{}, two, std::true_type{});
+  else if (n <= 2048) f(integral_constant<int, 128>{}, two, std::true_type{});
+  else if (n <= 4096) f(integral_constant<int, 256>{}, two, std::true_type{});
+  else if (n <= 8192) f(integral_constant<int, 512>{}, two, std::true_type{});
+  else f(integral_constant<int, 1024>{}, two, std::true_type{});
+}
+
+// Rows of a block of k_rmsnorm_grad, and its blocks: three per CU, as many as their registers let in.
+static int norm_rows_per_block(int64_t n) {
+  int rows = 1;
+  norm_grad_by_width(n, [&](auto tpr, auto, auto) { rows = norm_grad_block(decltype(tpr)::value) / decltype(tpr)::value; });
+  return rows;
+}
 static int64_t norm_parts(int64_t T, int64_t n) {
   const int64_t rpb = norm_rows_per_block(n);
-  return std::min<int64_t>((T + rpb - 1) / rpb, 512);
+  return std::min<int64_t>((T + rpb - 1) / rpb, 768);
 }
 
 template <typename X, typename H>
 static void norm_grad_launch(const NormGradArgs& a, int64_t blocks, hipStream_t s) {
-  norm_by_width(a.n, [&](auto tpr, auto nv, auto even) {
-    constexpr int TPR = decltype(tpr)::value, BT = TPR < 256 ? 256 : TPR;
+  norm_grad_by_width(a.n, [&](auto tpr, auto nv, auto even) {
+    constexpr int TPR = decltype(tpr)::value, BT = norm_grad_block(TPR);
     hipLaunchKernelGGL((k_rmsnorm_grad<X, H, TPR, decltype(nv)::value, decltype(even)::value>), dim3((unsigned)blocks), dim3(BT), 0, s, a);
   });
 }

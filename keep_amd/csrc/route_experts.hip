@@ -24,21 +24,13 @@ namespace keep {
 
 struct ChooseArgs {
   const void* z;
-  int zdt;
   const float* bias;
   int T, E, k, groups, topk_groups;
   int func, renorm;
   float scale;
   int32_t* idx;
   float* w;
-  int32_t* load;  // or null
 };
-
-__device__ __forceinline__ float ch_load(const void* z, int dt, int64_t i) {
-  if (dt == KEEP_F32) return ((const float*)z)[i];
-  if (dt == KEEP_BF16) return to_float(((const bf16s*)z)[i]);
-  return to_float(((const _Float16*)z)[i]);
-}
 
 // Which experts a lane holds: i-th is first + i step for i < n.
 struct ChooseLane {
@@ -54,48 +46,107 @@ struct ChooseLane {
   }
 };
 
-__device__ __forceinline__ int ch_reduce_min(int v) { return (int)rt_wave_u32<false>((uint32_t)v); }
+// op over groups of `n` lanes (a power of two), in every one of them.
+template <typename Op>
+__device__ __forceinline__ void ch_lanes(int n, Op op) {
+  // quad_perm [1,0,3,2] and [2,3,0,1], row_half_mirror, row_mirror: after each step the lanes so far hold the same value
+  if (n > 1) op([](float v) { return rt_dpp_f<0xB1>(v); });
+  if (n > 2) op([](float v) { return rt_dpp_f<0x4E>(v); });
+  if (n > 4) op([](float v) { return rt_dpp_f<0x141>(v); });
+  if (n > 8) op([](float v) { return rt_dpp_f<0x140>(v); });
+  if (n > 16) op([](float v) { return __shfl_xor(v, 16, 64); });
+  if (n > 32) op([](float v) { return __shfl_xor(v, 32, 64); });
+}
 
-// Softmax scores of a row whose logits are all -inf are 0.
+__device__ __forceinline__ int ch_min(int v) { return (int)rt_wave_u32<false>((uint32_t)v); }
+__device__ __forceinline__ float ch_lane(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+// The largest of the lanes' values, as a scalar.
+__device__ __forceinline__ uint32_t ch_max(uint32_t v) {
+  v = rt_dpp_u32<true, 0xB1>(v);
+  v = rt_dpp_u32<true, 0x4E>(v);
+  v = rt_dpp_u32<true, 0x141>(v);
+  v = rt_dpp_u32<true, 0x140>(v);
+  const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+  return max(max(a, b), max(c, d));
+}
+
+// What turns a logit into a score: for the softmax its largest logit and the sum's reciprocal.
+struct ChooseScore {
+  float m, r;
+  __device__ __forceinline__ float of(float z, int func) const {
+    if (func == KEEP_SCORE_SOFTMAX) return expf(z - m) * r;
+    if (func == KEEP_SCORE_SIGMOID) return __builtin_amdgcn_rcpf(1.f + expf(-z));
+    return sqrtf(fmaxf(z, 0.f) + log1pf(expf(-fabsf(z))));
+  }
+};
+
+// The scores of a lane's n logits (those behind them 0). Those of a softmax row whose logits are all -inf are 0.
 template <int PER>
-__device__ __forceinline__ void ch_scores(const float (&z)[PER], int n, int func, float (&s)[PER]) {
+__device__ __forceinline__ ChooseScore ch_scores(const float (&z)[PER], int n, int func, float (&s)[PER]) {
+  ChooseScore c{0.f, 0.f};
   if (func == KEEP_SCORE_SOFTMAX) {
     float m = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < PER; ++i) m = fmaxf(m, z[i]);
-    m = wave_max(m);
+    m = rt_wave_reduce(m, true);
+    c.m = m == -__builtin_inff() ? 0.f : m;
     float part = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      s[i] = i < n && (m > -__builtin_inff() || z[i] != z[i]) ? expf(z[i] - m) : 0.f;
+      s[i] = i < n ? expf(z[i] - c.m) : 0.f;
       part += s[i];
     }
-    const float sum = wave_sum(part);
-    const float r = sum == 0.f ? 0.f : 1.f / sum;
+    const float sum = rt_wave_reduce(part, false);
+    c.r = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] *= r;
+    for (int i = 0; i < PER; ++i) s[i] *= c.r;
+  } else if (func == KEEP_SCORE_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] = i < n ? c.of(z[i], KEEP_SCORE_SIGMOID) : 0.f;
   } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) s[i] = i < n ? rt_score_of(z[i], func) : 0.f;
+    for (int i = 0; i < PER; ++i) s[i] = i < n ? c.of(z[i], KEEP_SCORE_SQRTSOFTPLUS) : 0.f;
   }
+  return c;
 }
 
+// The lanes' doubles combined, without the LDS pipe: a token that is chosen in 64 bits shall not hold up the launch (by way of
+// LDS, 5 us behind 8192 tokens; 1 to 2).
+__device__ __forceinline__ double ch_lane_d(double v, int lane) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+  return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+}
+template <typename Op>
+__device__ __forceinline__ void ch_rows_d(int n, Op op) {  // inside 16 lanes, as ch_lanes
+  if (n > 1) op([](double v) { return rt_dpp_d<0xB1, 0xF>(v); });
+  if (n > 2) op([](double v) { return rt_dpp_d<0x4E, 0xF>(v); });
+  if (n > 4) op([](double v) { return rt_dpp_d<0x141, 0xF>(v); });
+  if (n > 8) op([](double v) { return rt_dpp_d<0x140, 0xF>(v); });
+}
 __device__ __forceinline__ double ch_wave_max_d(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = fmax(v, __shfl_xor(v, m, 64));
-  return v;
+  ch_rows_d(16, [&](auto from) { v = fmax(v, from(v)); });
+  return fmax(fmax(ch_lane_d(v, 0), ch_lane_d(v, 16)), fmax(ch_lane_d(v, 32), ch_lane_d(v, 48)));
+}
+__device__ __forceinline__ double ch_wave_sum_d(double v) {
+  ch_rows_d(16, [&](auto from) { v += from(v); });
+  return (ch_lane_d(v, 0) + ch_lane_d(v, 16)) + (ch_lane_d(v, 32) + ch_lane_d(v, 48));
 }
 
 // The choice in 64 bits: lane j < k gets winner j. The logits are read again: the few tokens that come here shall not cost
 // the others registers.
-template <int PER>
+template <typename Z, int PER>
 __device__ __forceinline__ int ch_exact(const ChooseArgs& a, const ChooseLane& l, int64_t t, int lane) {
   const int n = l.n, first = l.first, lg = l.lg, group = l.group;
   float z[PER];
   double key[PER];
   const double none = -__builtin_inf();
 #pragma unroll
-  for (int i = 0; i < PER; ++i) z[i] = i < n ? ch_load(a.z, a.zdt, t * a.E + first + i * lg) : -__builtin_inff();
+  for (int i = 0; i < PER; ++i) z[i] = i < n ? to_float(((const Z*)a.z)[t * a.E + first + i * lg]) : -__builtin_inff();
   if (a.func == KEEP_SCORE_SOFTMAX) {
     double m = none;
 #pragma unroll
@@ -107,8 +158,7 @@ __device__ __forceinline__ int ch_exact(const ChooseArgs& a, const ChooseLane& l
       key[i] = i < n && (m > none || z[i] != z[i]) ? exp((double)z[i] - m) : 0.;
       sum += key[i];
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    sum = ch_wave_sum_d(sum);
 #pragma unroll
     for (int i = 0; i < PER; ++i) key[i] = sum == 0. ? 0. : key[i] / sum;
   } else if (a.func == KEEP_SCORE_SIGMOID) {
@@ -132,16 +182,18 @@ __device__ __forceinline__ int ch_exact(const ChooseArgs& a, const ChooseLane& l
       t2 = fmax(t2, fmin(t1, key[i]));
       t1 = fmax(t1, key[i]);
     }
-    for (int o = 1; o < lg; o <<= 1) {
-      const double o1 = __shfl_xor(t1, o, 64), o2 = __shfl_xor(t2, o, 64);
+    const auto join = [&](auto from) {
+      const double o1 = from(t1), o2 = from(t2);
       t2 = fmax(fmin(t1, o1), fmax(t2, o2));
       t1 = fmax(t1, o1);
-    }
+    };
+    ch_rows_d(lg, join);
+    for (int o = 16; o < lg; o <<= 1) join([&](double v) { return __shfl_xor(v, o, 64); });
     double v = a.E > a.groups ? t1 + t2 : t1;
     if (v != v) v = none;
     int rank = 0;
     for (int h = 0; h < a.groups; ++h) {
-      const double o = __shfl(v, h * lg, 64);
+      const double o = ch_lane_d(v, h * lg);
       rank += o > v || (o == v && h < group) ? 1 : 0;
     }
     in = in && rank < a.topk_groups;
@@ -164,7 +216,7 @@ __device__ __forceinline__ int ch_exact(const ChooseArgs& a, const ChooseLane& l
         at = first + i * lg;
       }
     const double top = ch_wave_max_d(best);
-    const int e = ch_reduce_min(best == top ? at : 0x7fffffff);
+    const int e = ch_min(best == top ? at : 0x7fffffff);
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (e == first + i * lg && i < n) open &= ~(1u << i);
@@ -173,26 +225,32 @@ __device__ __forceinline__ int ch_exact(const ChooseArgs& a, const ChooseLane& l
   return mine;
 }
 
-// How far a score formed in fp32 may be from the real one: expf and the divisions 2^-21 of it; the softmax's exponent loses
-// |z - m| 2^-24 too, up to 104 before the score is 0.
-__device__ __forceinline__ float ch_unsure(int func) { return func == KEEP_SCORE_SOFTMAX ? 0x1p-17f : 0x1p-20f; }
+// How far a score formed in fp32 may be from the real one, of the row's largest score. Sigmoid and sqrt(softplus): expf and
+// log1pf by a step or two, the sum, the reciprocal or root: under 4 x 2^-23. Softmax: the exponent rounds by |z - m| 2^-24, which
+// times e^(z - m) is under 0.4 x 2^-24 of the largest; expf by a step; the sum of up to 32 values a lane and 64 lanes by 40 2^-24.
+__device__ __forceinline__ float ch_unsure(int func) { return func == KEEP_SCORE_SOFTMAX ? 0x1p-18f : 0x1p-21f; }
 
-template <int PER>
+// Rounds of the selection: a lane's keys are sorted once with their experts, a round is the wave's largest head, whose lane
+// pops it. Lane j keeps winner j; scores and biases of the winners are read and formed again by their lanes together, and
+// neighbours compared there.
+template <typename Z, int PER>
 __global__ __launch_bounds__(256) void k_route_experts(ChooseArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const ChooseLane l(a.E, a.groups, lane);
+  const Z* row = (const Z*)a.z + t * a.E;
+  const bool biased = a.bias != nullptr, grouped = a.topk_groups < a.groups;
+  Z raw[PER];
   float z[PER], b[PER], s[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = l.first + i * l.lg;
-    z[i] = i < l.n ? ch_load(a.z, a.zdt, t * a.E + e) : -__builtin_inff();
-    b[i] = a.bias && i < l.n ? a.bias[e] : 0.f;
-  }
-  ch_scores<PER>(z, l.n, a.func, s);
+  for (int i = 0; i < PER; ++i) raw[i] = i < l.n ? row[l.first + i * l.lg] : Z{};
+#pragma unroll
+  for (int i = 0; i < PER; ++i) b[i] = biased && i < l.n ? a.bias[l.first + i * l.lg] : 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) z[i] = i < l.n ? to_float(raw[i]) : -__builtin_inff();
+  const ChooseScore score = ch_scores<PER>(z, l.n, a.func, s);
   bool sure = true, in = l.n > 0;
-  const bool biased = a.bias != nullptr, grouped = a.topk_groups < a.groups;
   // how far any two keys' scores may be off together
   float unsure = 0.f;
   if (biased || grouped) {
@@ -200,21 +258,23 @@ __global__ __launch_bounds__(256) void k_route_experts(ChooseArgs a) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) m = fmaxf(m, s[i]);
     unsure = 2.f * ch_unsure(a.func) * rt_wave_reduce(m, true);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s[i] += b[i];  // the keys
   }
   if (grouped) {
     const float none = -__builtin_inff();
     float t1 = none, t2 = none;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const float v = i < l.n ? s[i] + b[i] : none;
+      const float v = i < l.n ? s[i] : none;
       t2 = fmaxf(t2, fminf(t1, v));
       t1 = fmaxf(t1, v);
     }
-    for (int o = 1; o < l.lg; o <<= 1) {
-      const float o1 = __shfl_xor(t1, o, 64), o2 = __shfl_xor(t2, o, 64);
+    ch_lanes(l.lg, [&](auto from) {
+      const float o1 = from(t1), o2 = from(t2);
       t2 = fmaxf(fminf(t1, o1), fmaxf(t2, o2));
       t1 = fmaxf(t1, o1);
-    }
+    });
     const bool pair = a.E > a.groups;
     float v = pair ? t1 + t2 : t1;
     if (v != v) v = none;
@@ -222,101 +282,106 @@ __global__ __launch_bounds__(256) void k_route_experts(ChooseArgs a) {
     const float err = 2.f * unsure + 0x1p-21f * rt_wave_reduce(l.n > 0 ? fabsf(t1) + (pair ? fabsf(t2) : 0.f) : 0.f, true);
     int rank = 0;
     for (int h = 0; h < a.groups; ++h) {
-      const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), h * l.lg));
+      const float o = ch_lane(v, h * l.lg);
       rank += o > v || (o == v && h < l.group) ? 1 : 0;
     }
     in = in && rank < a.topk_groups;
     // the last group that is in and the first that is not
     const uint64_t ma = __ballot(l.group < a.groups && rank == a.topk_groups - 1);
     const uint64_t mb = __ballot(l.group < a.groups && rank == a.topk_groups);
-    if (ma == 0 || mb == 0) {
-      sure = false;
-    } else {
-      const int la = __builtin_ctzll(ma), lb = __builtin_ctzll(mb);
-      sure = __shfl(v, la, 64) - __shfl(v, lb, 64) > err;
-    }
+    sure = ma != 0 && mb != 0 && ch_lane(v, __builtin_ctzll(ma ? ma : 1)) - ch_lane(v, __builtin_ctzll(mb ? mb : 1)) > err;
   }
   // without a bias the logits are the keys
   uint32_t key[PER];
+  int at[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) key[i] = in && i < l.n ? rt_sortable(biased ? s[i] + b[i] : z[i]) : 0u;
+  for (int i = 0; i < PER; ++i) {
+    key[i] = in && i < l.n ? rt_sortable(biased ? s[i] : z[i]) : 0u;
+    at[i] = l.first + i * l.lg;
+  }
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {  // odd-even transposition sort, descending; equal keys keep their order
+#pragma unroll
+    for (int i = p & 1; i + 1 < PER; i += 2) {
+      const bool swap = key[i + 1] > key[i];
+      const uint32_t k0 = key[i], k1 = key[i + 1];
+      const int e0 = at[i], e1 = at[i + 1];
+      key[i] = swap ? k1 : k0;
+      key[i + 1] = swap ? k0 : k1;
+      at[i] = swap ? e1 : e0;
+      at[i + 1] = swap ? e0 : e1;
+    }
+  }
   int mine = 0;
-  float ws = 0.f, total = 0.f, pk = 0.f, pz = 0.f, pb = 0.f;
-  const int rounds = biased ? a.k + 1 : a.k;
+  uint32_t mykey = 0u;
+  const int rounds = min(biased ? a.k + 1 : a.k, a.topk_groups * (a.E / a.groups));
   for (int j = 0; j < rounds; ++j) {
-    uint32_t top = 0u;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) top = max(top, key[i]);
-    const uint32_t best = rt_wave_u32<true>(top);
-    if (best == 0u) break;  // fewer than k + 1 experts
-    int at = 0x7fffffff;
-    float zs = 0.f, bs = 0.f, ss = 0.f;
-#pragma unroll
-    for (int i = PER - 1; i >= 0; --i)
-      if (key[i] == best) {
-        at = l.first + i * l.lg;
-        zs = z[i];
-        bs = b[i];
-        ss = s[i];
-      }
-    const uint64_t who = __ballot(top == best);
-    int owner = __builtin_ctzll(who), e;
+    const uint32_t best = ch_max(key[0]);
+    const uint64_t who = __ballot(key[0] == best);
+    int owner = __builtin_ctzll(who);
     if (who & (who - 1)) {  // several lanes: the lowest expert
-      e = ch_reduce_min(at);
-      owner = __builtin_ctzll(__ballot(at == e));
+      const int e = ch_min(key[0] == best ? at[0] : 0x7fffffff);
+      owner = __builtin_ctzll(__ballot(key[0] == best && at[0] == e));
     }
-    e = __builtin_amdgcn_readlane(at, owner);
-    const auto of = [&](float v) {
-      return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), owner));
-    };
-    const float se = of(ss);
-    if (biased) {
-      const float ke = rt_unsortable(best), ze = of(zs), be = of(bs);
-      if (j > 0) {
-        const float err = unsure + 0x1p-23f * (fabsf(ke) + fabsf(pk));  // (a key further down may be off as far)
-        sure = sure && (pk - ke > err || (ze == pz && be == pb));
-      }
-      pk = ke; pz = ze; pb = be;
-    }
-    if (j == a.k) break;
+    const int e = __builtin_amdgcn_readlane(at[0], owner);
+    mine = lane == j ? e : mine;
+    mykey = lane == j ? best : mykey;
+    const uint32_t pop = lane == owner ? 0xffffffffu : 0u;  // (bitfield selects)
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (at == e && key[i] == best && l.first + i * l.lg == e) key[i] = 0u;
-    if (lane == j) {
-      mine = e;
-      ws = se;
+    for (int i = 0; i + 1 < PER; ++i) {
+      key[i] = (key[i + 1] & pop) | (key[i] & ~pop);
+      at[i] = (int)(((uint32_t)at[i + 1] & pop) | ((uint32_t)at[i] & ~pop));
     }
-    total += se;
+    key[PER - 1] &= ~pop;
   }
-  if (!sure) {
-    mine = ch_exact<PER>(a, l, t, lane);
-    total = 0.f;
-    for (int j = 0; j < a.k; ++j) {  // the scores of the choice, in its order
-      const int e = __builtin_amdgcn_readlane(mine, j);
-      float v = 0.f;
-      bool here = false;
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i < l.n && l.first + i * l.lg == e) {
-          v = s[i];
-          here = true;
-        }
-      const int owner = __builtin_ctzll(__ballot(here));
-      const float se = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), owner));
-      if (lane == j) ws = se;
-      total += se;
+  const bool chosen = lane < a.k;
+  if (biased) {
+    // each winner against the next one (lane k: the first that is not chosen); a key further down may be off as far
+    const float kw = mykey ? rt_unsortable(mykey) : -__builtin_inff(), kn = __shfl_down(kw, 1, 64);
+    const uint64_t close = __ballot(chosen && !(kw - kn > unsure + 0x1p-23f * (fabsf(kw) + fabsf(kn))));
+    if (close) {  // equal logits under equal biases are no cause, nor is the end of the experts
+      const bool have = mykey != 0u;
+      const float zw = have ? to_float(row[mine]) : 0.f, bw = have ? a.bias[mine] : 0.f;
+      const float zn = __shfl_down(zw, 1, 64), bn = __shfl_down(bw, 1, 64);
+      const bool next = __shfl_down((int)have, 1, 64) != 0;
+      sure = sure && __all(!(close >> lane & 1) || !next || (zw == zn && bw == bn));
     }
   }
-  if (lane < a.k) {
+  if (!sure) mine = ch_exact<Z, PER>(a, l, t, lane);
+  const float zw = !chosen ? 0.f : biased || !sure ? to_float(row[mine]) : rt_unsortable(mykey);
+  const float sw = chosen ? score.of(zw, a.func) : 0.f;
+  float w = sw;
+  if (a.renorm) {
+    float total = 0.f;
+    for (int j = 0; j < a.k; ++j) total += ch_lane(sw, j);
+    w = sw / (total + 1e-20f);
+  }
+  if (chosen) {
     a.idx[t * a.k + lane] = mine;
-    a.w[t * a.k + lane] = (a.renorm ? ws / (total + 1e-20f) : ws) * a.scale;
-    if (a.load) atomicAdd(a.load + mine, 1);
+    a.w[t * a.k + lane] = w * a.scale;
   }
+}
+
+// The tokens of every expert: a block counts a run of routes in LDS and adds its counts. Counted by the tokens' own waves,
+// one global addition a route, 24576 routes took 15 us beside the choice's 9; here 4.
+constexpr int LOAD_ROUTES = 8192;
+__global__ __launch_bounds__(1024) void k_route_load(const int32_t* idx, int64_t routes, int E, int32_t* load) {
+  __shared__ int count[64 * RT_MAX_PER_LANE];
+  for (int e = threadIdx.x; e < E; e += 1024) count[e] = 0;
+  __syncthreads();
+  const int64_t r0 = (int64_t)blockIdx.x * LOAD_ROUTES;
+#pragma unroll
+  for (int i = 0; i < LOAD_ROUTES / 1024; ++i) {
+    const int64_t r = r0 + i * 1024 + threadIdx.x;
+    if (r < routes) atomicAdd(&count[idx[r]], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += 1024)
+    if (count[e]) atomicAdd(load + e, count[e]);
 }
 
 struct ChooseGradArgs {
   const void* z;
-  int zdt;
   const int32_t* idx;
   const float* dw;
   int T, E, k;
@@ -325,49 +390,39 @@ struct ChooseGradArgs {
   void* dz;
 };
 
-__device__ __forceinline__ void ch_store(void* p, int dt, int64_t i, float v) {
-  if (dt == KEEP_F32) ((float*)p)[i] = v;
-  else if (dt == KEEP_BF16) ((bf16s*)p)[i] = from_float<bf16s>(v);
-  else ((_Float16*)p)[i] = from_float<_Float16>(v);
-}
-
-template <int PER>
+template <typename Z, int PER>
 __global__ __launch_bounds__(256) void k_route_experts_grad(ChooseGradArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const int n = lane < a.E ? (a.E - lane + 63) / 64 : 0;
+  const Z* row = (const Z*)a.z + t * a.E;
+  Z raw[PER];
   float z[PER], s[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) z[i] = i < n ? ch_load(a.z, a.zdt, t * a.E + lane + 64 * i) : -__builtin_inff();
-  ch_scores<PER>(z, n, a.func, s);
+  for (int i = 0; i < PER; ++i) raw[i] = i < n ? row[lane + 64 * i] : Z{};
   // lane j < k: the j-th choice
-  const bool chosen = lane < a.k;
-  const int e = chosen ? a.idx[t * a.k + lane] : 0;
+  int e = lane < a.k ? a.idx[t * a.k + lane] : -1;
+  const bool chosen = e >= 0 && e < a.E;
   const float g = chosen ? a.dw[t * a.k + lane] : 0.f;
-  float se = 0.f, ze = 0.f;
+  const float ze = chosen ? to_float(row[e]) : 0.f;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const float sv = __shfl(s[i], e & 63, 64), zv = __shfl(z[i], e & 63, 64);
-    if ((e >> 6) == i) {
-      se = sv;
-      ze = zv;
-    }
-  }
-  if (!chosen) se = 0.f;
+  for (int i = 0; i < PER; ++i) z[i] = i < n ? to_float(raw[i]) : -__builtin_inff();
+  const ChooseScore score = ch_scores<PER>(z, n, a.func, s);
+  const float se = chosen ? score.of(ze, a.func) : 0.f;
   float p = a.scale * g;
   if (a.renorm) {
-    const float total = wave_sum(se) + 1e-20f;
-    p = a.scale / total * (g - wave_sum(g * se) / total);
+    const float total = rt_wave_reduce(se, false) + 1e-20f;
+    p = a.scale / total * (g - rt_wave_reduce(g * se, false) / total);
   }
   float dot = 0.f;
   if (a.func == KEEP_SCORE_SOFTMAX) {
-    dot = wave_sum(chosen ? p * se : 0.f);
+    dot = rt_wave_reduce(chosen ? p * se : 0.f, false);
   } else if (a.func == KEEP_SCORE_SIGMOID) {
     p *= 1.f - se;  // (times the score below)
   } else {
     // sigmoid(z) / (2 s) over s; where both vanish, s^2 -> e^z and the slope is s / 2
-    p *= se > 0.f ? 0.5f * rt_score_of(ze, KEEP_SCORE_SIGMOID) / se / se : 0.f;
+    p *= se > 0.f ? 0.5f * score.of(ze, KEEP_SCORE_SIGMOID) / se / se : 0.f;
   }
   float d[PER];
 #pragma unroll
@@ -381,7 +436,29 @@ __global__ __launch_bounds__(256) void k_route_experts_grad(ChooseGradArgs a) {
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i)
-    if (i < n) ch_store(a.dz, a.zdt, t * a.E + lane + 64 * i, s[i] * d[i]);
+    if (i < n) ((Z*)a.dz)[t * a.E + lane + 64 * i] = from_float<Z>(s[i] * d[i]);
+}
+
+template <typename Z>
+static void choose_launch(const ChooseArgs& a, int64_t per, hipStream_t s) {
+  const dim3 grid((unsigned)((a.T + 3) / 4)), block(256);
+  if (per <= 1) hipLaunchKernelGGL((k_route_experts<Z, 1>), grid, block, 0, s, a);
+  else if (per <= 2) hipLaunchKernelGGL((k_route_experts<Z, 2>), grid, block, 0, s, a);
+  else if (per <= 4) hipLaunchKernelGGL((k_route_experts<Z, 4>), grid, block, 0, s, a);
+  else if (per <= 6) hipLaunchKernelGGL((k_route_experts<Z, 6>), grid, block, 0, s, a);
+  else if (per <= 8) hipLaunchKernelGGL((k_route_experts<Z, 8>), grid, block, 0, s, a);
+  else if (per <= 16) hipLaunchKernelGGL((k_route_experts<Z, 16>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((k_route_experts<Z, 32>), grid, block, 0, s, a);  // groups a little more than a power of two
+}
+
+template <typename Z>
+static void choose_grad_launch(const ChooseGradArgs& a, int64_t per, hipStream_t s) {
+  const dim3 grid((unsigned)((a.T + 3) / 4)), block(256);
+  if (per <= 2) hipLaunchKernelGGL((k_route_experts_grad<Z, 2>), grid, block, 0, s, a);
+  else if (per <= 4) hipLaunchKernelGGL((k_route_experts_grad<Z, 4>), grid, block, 0, s, a);
+  else if (per <= 6) hipLaunchKernelGGL((k_route_experts_grad<Z, 6>), grid, block, 0, s, a);
+  else if (per <= 8) hipLaunchKernelGGL((k_route_experts_grad<Z, 8>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((k_route_experts_grad<Z, 16>), grid, block, 0, s, a);
 }
 
 }  // namespace keep
@@ -412,20 +489,18 @@ extern "C" int keep_route_experts(const void* logits, int dtype, int64_t T, int6
   KEEP_REQUIRE(aligned(logits, dtype_size(dtype)) && aligned(bias, 4) && aligned(idx, 4) && aligned(w, 4) &&
                    aligned(load, 4),
                "misaligned pointer");
-  ChooseArgs a{logits, dtype, bias, (int)T, (int)E, (int)k, (int)groups, (int)topk_groups, score_func, renormalize,
-               route_scale, idx, w, load};
+  ChooseArgs a{logits, bias, (int)T, (int)E, (int)k, (int)groups, (int)topk_groups, score_func, renormalize,
+               route_scale, idx, w};
   int lg = 1;
   while (lg * 2 * groups <= 64) lg *= 2;
   const int64_t per = (E / groups + lg - 1) / lg;
-  const dim3 grid((unsigned)((T + 3) / 4)), block(256);
   hipStream_t s = (hipStream_t)stream;
-  if (per <= 1) hipLaunchKernelGGL(k_route_experts<1>, grid, block, 0, s, a);
-  else if (per <= 2) hipLaunchKernelGGL(k_route_experts<2>, grid, block, 0, s, a);
-  else if (per <= 4) hipLaunchKernelGGL(k_route_experts<4>, grid, block, 0, s, a);
-  else if (per <= 6) hipLaunchKernelGGL(k_route_experts<6>, grid, block, 0, s, a);
-  else if (per <= 8) hipLaunchKernelGGL(k_route_experts<8>, grid, block, 0, s, a);
-  else if (per <= 16) hipLaunchKernelGGL(k_route_experts<16>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(k_route_experts<32>, grid, block, 0, s, a);  // groups one more than a power of two
+  if (dtype == KEEP_F32) choose_launch<float>(a, per, s);
+  else if (dtype == KEEP_F16) choose_launch<_Float16>(a, per, s);
+  else choose_launch<bf16s>(a, per, s);
+  if (load)
+    hipLaunchKernelGGL(k_route_load, dim3((unsigned)((T * k + LOAD_ROUTES - 1) / LOAD_ROUTES)), dim3(1024), 0, s, idx, T * k,
+                       (int)E, load);
   return launch_status("keep_route_experts");
 }
 
@@ -439,14 +514,11 @@ extern "C" int keep_route_experts_grad(const void* logits, int dtype, int64_t T,
   KEEP_REQUIRE(aligned(logits, dtype_size(dtype)) && aligned(idx, 4) && aligned(dw, 4) &&
                    aligned(dlogits, dtype_size(dtype)),
                "misaligned pointer");
-  ChooseGradArgs a{logits, dtype, idx, dw, (int)T, (int)E, (int)k, score_func, renormalize, route_scale, dlogits};
+  ChooseGradArgs a{logits, idx, dw, (int)T, (int)E, (int)k, score_func, renormalize, route_scale, dlogits};
   const int64_t per = (E + 63) / 64;
-  const dim3 grid((unsigned)((T + 3) / 4)), block(256);
   hipStream_t s = (hipStream_t)stream;
-  if (per <= 2) hipLaunchKernelGGL(k_route_experts_grad<2>, grid, block, 0, s, a);
-  else if (per <= 4) hipLaunchKernelGGL(k_route_experts_grad<4>, grid, block, 0, s, a);
-  else if (per <= 6) hipLaunchKernelGGL(k_route_experts_grad<6>, grid, block, 0, s, a);
-  else if (per <= 8) hipLaunchKernelGGL(k_route_experts_grad<8>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(k_route_experts_grad<16>, grid, block, 0, s, a);
+  if (dtype == KEEP_F32) choose_grad_launch<float>(a, per, s);
+  else if (dtype == KEEP_F16) choose_grad_launch<_Float16>(a, per, s);
+  else choose_grad_launch<bf16s>(a, per, s);
   return launch_status("keep_route_experts_grad");
 }
