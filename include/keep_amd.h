@@ -658,7 +658,7 @@ int64_t keep_rmsnorm_grad_workspace_bytes(int64_t T, int64_t n);
  * of E / groups neighbouring experts: the topk_groups groups with the largest sum of their two largest keys are kept, and the
  * k largest keys in them chosen; the lower index first among equals, NaN as -inf. idx int32 and w fp32 [T, k] in descending
  * order of the keys: w = score route_scale, renormalised to sum to route_scale (+ 1e-20) with renormalize. load int32 [E] or
- * NULL: the chosen experts are counted into it (added to what it holds). E <= 1024, k <= 32, T <= 2^25. */
+ * NULL: receives the tokens of every expert (T = 0: nothing is written). E <= 1024, k <= 32, T <= 2^25. */
 int keep_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int64_t k, const float* bias, int64_t groups,
                        int64_t topk_groups, int score_func, int renormalize, float route_scale, int32_t* idx, float* w,
                        int32_t* load, void* stream);

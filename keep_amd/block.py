@@ -20,7 +20,8 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from keep_amd import _lib
+from keep_amd import _grad, _lib
+from keep_amd.ops import _DT, _dense_device, _on, _ptr, _stream
 
 NORM_WIDTH = 16384  # values of a row that the norms serve
 
@@ -31,7 +32,6 @@ def rmsnorm_quant_rht(x: torch.Tensor, gamma: torch.Tensor | None = None, eps: f
     ``quant_block`` values (0: none), ``out = RHT(q, rht_signs)`` (no signs: q).
     Returns ``out`` or ``(out, y)`` with ``return_normed``."""
 
-    from keep_amd.ops import _DT, _stream
     from keep_amd.rht import check_signs
 
     if not x.is_cuda:
@@ -72,8 +72,6 @@ def rmsnorm_quant_rht(x: torch.Tensor, gamma: torch.Tensor | None = None, eps: f
 
 
 def _norm_args(x, weight, eps: float, residual) -> torch.device:
-    from keep_amd.ops import _DT, _dense_device
-
     device = _dense_device(x, weight, residual)
     if x.dtype not in _DT:
         raise ValueError(f"x must be float32, float16 or bfloat16, found {x.dtype}")
@@ -92,8 +90,6 @@ def _norm_args(x, weight, eps: float, residual) -> torch.device:
 
 def _rmsnorm(x, weight, eps: float, residual, keep_rstd: bool):
     """``(y, h, rstd)`` of contiguous rows; h is x without a residual."""
-
-    from keep_amd.ops import _DT, _ptr, _stream
 
     n = x.shape[-1]
     rows = x.numel() // n
@@ -119,8 +115,6 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        from keep_amd.ops import _DT, _on, _ptr, _stream
-
         h, weight, rstd = ctx.saved_tensors
         nx, nr, nw = ctx.needs_input_grad[:3]
         if dy is None:  # h alone was used
@@ -151,9 +145,6 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e
     rounded stream. ``weight [n]`` of any float dtype. Differentiable in ``x``, ``residual`` and ``weight``; the gradients
     of ``x`` and a ``residual`` of its dtype are the same values, in one tensor."""
 
-    from keep_amd import _grad
-    from keep_amd.ops import _on
-
     device = _norm_args(x, weight, eps, residual)
     with _on(device):
         xc = x.contiguous()
@@ -176,9 +167,6 @@ def rmsnorm_quant(x: torch.Tensor, weight: torch.Tensor | None = None, eps: floa
     normed values, rounded once. ``quant_block`` (a power of two in 16..512) neighbouring values share a scale,
     ``max(max |y|, 1e-4) / 448``, with ``pow2_scales`` the next power of two: ``act_quant``'s
     (``torch_kernel.py:40-53``). ``linear_q8`` reads blocks of 128. No gradients."""
-
-    from keep_amd import _grad
-    from keep_amd.ops import _DT, _on, _ptr, _stream
 
     device = _norm_args(x, weight, eps, residual)
     if not 16 <= quant_block <= 512 or quant_block & (quant_block - 1):
@@ -206,9 +194,6 @@ def combine_add(routed: torch.Tensor, shared: torch.Tensor | None = None, residu
     """``round_out(residual + (routed + shared))`` with fp32 sums; ``routed`` is float32. Differentiable: every
     term's gradient is the output's, in its dtype."""
 
-    from keep_amd import _grad
-    from keep_amd.ops import _DT, _on
-
     if routed.dtype != torch.float32 or not routed.is_cuda:
         raise ValueError("routed must be a float32 device tensor")
     for name, t in (("shared", shared), ("residual", residual)):
@@ -223,8 +208,6 @@ def combine_add(routed: torch.Tensor, shared: torch.Tensor | None = None, residu
 
 
 def _combine_add(routed, shared, residual, od: torch.dtype) -> torch.Tensor:
-    from keep_amd.ops import _DT, _stream
-
     r = routed.contiguous()
     sh = None if shared is None else shared.contiguous()
     rs = None if residual is None else residual.contiguous()

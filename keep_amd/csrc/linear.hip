@@ -146,18 +146,19 @@ struct LinearPlan {
   int tile, slices;
 };
 
-// The tile (rows of J, of I 128; 256: 256 x 256, 8-bit 128 x 256) and the slices of a product. 0: the kernel for few rows.
+// The tile (64, 128: rows of J, of I 128; 192: 128 of J x 256 of I; 256: 256 x 256) and the slices of a product. 0: the kernel
+// for few rows.
 static LinearPlan linear_plan(int dtype, int mode, int64_t ni, int64_t nj, int64_t nk) {
   if (mode == LINEAR_FORWARD && nj <= LINEAR_FEW) return {0, 1};
   const auto tiles = [&](int64_t bi, int64_t bj) { return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj); };
-  const int64_t large = dtype == KEEP_F32 ? 0 : dtype == KEEP_E4M3 ? tiles(256, 128) : tiles(256, 256);
   int tile = 64;
-  if (large >= 192) tile = 256;
-  else if (nj > 64 && tiles(128, 128) >= 128) tile = 128;
-  const int64_t n = tile == 256 ? large : tile == 128 ? tiles(128, 128) : tiles(128, 64);
+  if (dtype == KEEP_BF16 || dtype == KEEP_F16) tile = tiles(256, 256) >= 224 ? 256 : tile;
+  if (tile == 64 && dtype != KEEP_F32 && tiles(256, 128) >= 192) tile = 192;
+  if (tile == 64 && nj > 64 && tiles(128, 128) >= 128) tile = 128;
+  const int64_t n = tile == 256 ? tiles(256, 256) : tile == 192 ? tiles(256, 128) : tiles(128, tile);
   const int64_t steps = (nk * linear_size(dtype) + 127) / 128;
   // slices of at least eight steps while the tiles leave CUs without work
-  const int64_t slices = tile == 256 ? 1 : std::max<int64_t>(1, std::min<int64_t>({512 / n, steps / 8, 32}));
+  const int64_t slices = tile > 128 ? 1 : std::max<int64_t>(1, std::min<int64_t>({512 / n, steps / 8, 32}));
   return {tile, (int)slices};
 }
 
@@ -166,7 +167,7 @@ static int64_t linear_part_bytes(const LinearPlan& p, int64_t ni, int64_t nj) {
 }
 
 static bool linear_gemm_fits(const LinearPlan& p, int64_t ni, int64_t nj) {
-  const int64_t bi = p.tile == 0 ? 16 : p.tile == 256 ? 256 : 128, bj = p.tile == 0 ? 16 : std::min(p.tile, 128);
+  const int64_t bi = p.tile == 0 ? 16 : p.tile > 128 ? 256 : 128, bj = p.tile == 0 ? 16 : std::min(p.tile, 128);
   return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj) <= (int64_t(1) << 22) / p.slices;
 }
 

@@ -40,7 +40,8 @@ struct LinearStep {
   static constexpr int K = 128 / sizeof(T);  // summed values of a step
 };
 
-template <typename T, int BI, int BJ, int WI, int WJ, int MODE>
+// TAIL: the summed index may end inside the last step. (The choice costs every copy of the loop a branch, 8 % of a step.)
+template <typename T, int BI, int BJ, int WI, int WJ, int MODE, bool TAIL>
 __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) {
   constexpr int NT = 64 * WI * WJ, TI = BI / WI, TJ = BJ / WJ, FI = TI / 16, FJ = TJ / 16;
   constexpr int LI = BI * 8 / NT, LJ = BJ * 8 / NT;  // 16-byte copies per thread and step
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
     if (jside && part && !TRJ && (wv * 64 + (i - LI) * NT) / 8 >= count) return;  // rows past the last: not stored
     const char* base = jside ? jbase + step * jstep : ibase + step * istep;
     const uint32_t o = jside ? oj[jside ? i - LI : 0] : oi[jside ? 0 : i];
-    if ((int64_t)(step + 1) * KS <= a.nk) {
+    if (!TAIL || (int64_t)(step + 1) * KS <= a.nk) {
       dg_dma(base, o, to);
     } else {
       int L = tid + (jside ? i - LI : i) * NT;
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
       struct Half {
         uint4 f[NR];
       };
-      constexpr int CC = (NC * 2 + FJ - 1) / FJ;  // copies per group of products: all in the first half of the groups
+      constexpr int CC = (NC + FJ - 1) / FJ;  // copies per group of products
       const auto half = [&](const Half& use, Half& next, int nstep, int nks, bool copies, int cstep) {
 #pragma unroll
         for (int j = 0; j < FJ; ++j) {
@@ -289,8 +290,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
 template <typename T, int BI, int BJ, int WI, int WJ, int MODE>
 void linear_gemm_launch(const LinearGemmArgs& a, hipStream_t s) {
   const int64_t items = ((a.ni + BI - 1) / BI) * ((a.nj + BJ - 1) / BJ) * a.slices;
-  hipLaunchKernelGGL((k_linear_gemm<T, BI, BJ, WI, WJ, MODE>), dim3((unsigned)((items + 7) / 8 * 8)),
-                     dim3(64 * WI * WJ), 0, s, a);
+  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * WI * WJ);
+  if (a.nk % LinearStep<T>::K == 0)
+    hipLaunchKernelGGL((k_linear_gemm<T, BI, BJ, WI, WJ, MODE, false>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((k_linear_gemm<T, BI, BJ, WI, WJ, MODE, true>), grid, block, 0, s, a);
 }
 
 template <typename T, int MODE>
@@ -298,8 +301,8 @@ void linear_gemm_tile(const LinearGemmArgs& a, int tile, hipStream_t s) {
   if (tile == 64) linear_gemm_launch<T, 128, 64, 2, 2, MODE>(a, s);
   else if constexpr (sizeof(T) == 4) linear_gemm_launch<T, 128, 128, 2, 2, MODE>(a, s);
   else if (tile == 128) linear_gemm_launch<T, 128, 128, 2, 2, MODE>(a, s);
-  else if constexpr (sizeof(T) == 1) linear_gemm_launch<T, 256, 128, 4, 2, MODE>(a, s);
-  else linear_gemm_launch<T, 256, 256, 4, 2, MODE>(a, s);
+  else if (tile == 192 || sizeof(T) == 1) linear_gemm_launch<T, 256, 128, 4, 2, MODE>(a, s);
+  else if constexpr (sizeof(T) == 2) linear_gemm_launch<T, 256, 256, 4, 2, MODE>(a, s);
 }
 
 template <typename T>

@@ -30,6 +30,7 @@ struct ChooseArgs {
   float scale;
   int32_t* idx;
   float* w;
+  int32_t* load;  // or null: cleared for k_route_load
 };
 
 // Which experts a lane holds: i-th is first + i step for i < n.
@@ -237,6 +238,8 @@ template <typename Z, int PER>
 __global__ __launch_bounds__(256) void k_route_experts(ChooseArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (a.load && blockIdx.x == 0)
+    for (int e = threadIdx.x; e < a.E; e += 256) a.load[e] = 0;
   if (t >= a.T) return;
   const ChooseLane l(a.E, a.groups, lane);
   const Z* row = (const Z*)a.z + t * a.E;
@@ -490,7 +493,7 @@ extern "C" int keep_route_experts(const void* logits, int dtype, int64_t T, int6
                    aligned(load, 4),
                "misaligned pointer");
   ChooseArgs a{logits, bias, (int)T, (int)E, (int)k, (int)groups, (int)topk_groups, score_func, renormalize,
-               route_scale, idx, w};
+               route_scale, idx, w, load};
   int lg = 1;
   while (lg * 2 * groups <= 64) lg *= 2;
   const int64_t per = (E / groups + lg - 1) / lg;

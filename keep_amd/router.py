@@ -120,7 +120,7 @@ def _route(z, k: int, bias, groups: int, topk_groups: int, func: int, renormaliz
     T, E = z.shape
     idx = torch.empty((T, k), dtype=torch.int32, device=z.device)
     weight = torch.empty((T, k), dtype=torch.float32, device=z.device)
-    load = torch.zeros(E, dtype=torch.int32, device=z.device) if count else None
+    load = (torch.empty if T else torch.zeros)(E, dtype=torch.int32, device=z.device) if count else None
     if T:
         _lib.call("keep_route_experts", z.data_ptr(), _DT[z.dtype], T, E, k, _ptr(bias), groups, topk_groups, func,
                   int(renormalize), scale, idx.data_ptr(), weight.data_ptr(), _ptr(load), _stream(z.device))
@@ -129,24 +129,26 @@ def _route(z, k: int, bias, groups: int, topk_groups: int, func: int, renormaliz
 
 class _RouteExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, k, bias, groups, topk_groups, func, renormalize, scale, count):
+    def forward(ctx, z, choice, *args):
+        """``choice`` receives the outputs that take no gradient."""
+
         z = z.contiguous()
-        idx, weight, load = _route(z, k, bias, groups, topk_groups, func, renormalize, scale, count)
+        idx, weight, load = _route(z, *args)
+        choice += (idx, load)
         ctx.save_for_backward(z, idx)
-        ctx.args = (func, int(renormalize), scale)
-        ctx.mark_non_differentiable(*(t for t in (idx, load) if t is not None))
-        return idx, weight, load
+        ctx.args = (args[4], int(args[5]), args[6])  # score function, renormalize, scale
+        return weight
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, _, dweight, __):
+    def backward(ctx, dweight):
         z, idx = ctx.saved_tensors
-        dz, dw = torch.empty_like(z), dweight.float().contiguous()
+        dz, dw = torch.empty_like(z), dweight.contiguous()
         if z.shape[0]:
             with _on(z.device):
                 _lib.call("keep_route_experts_grad", z.data_ptr(), _DT[z.dtype], *z.shape, idx.shape[1], idx.data_ptr(),
                           dw.data_ptr(), *ctx.args, dz.data_ptr(), _stream(z.device))
-        return (dz,) + (None,) * 8
+        return (dz,) + (None,) * 9
 
 
 def route_experts(logits: torch.Tensor, k: int, *, bias: torch.Tensor | None = None, score_func: str = "softmax",
@@ -192,5 +194,6 @@ def route_experts(logits: torch.Tensor, k: int, *, bias: torch.Tensor | None = N
         if not _grad.wanted(logits):
             return ExpertRoutes(*_route(logits.contiguous(), *args))
         _grad.check_capture(logits)
-        idx, weight, load = _RouteExperts.apply(logits, *args)
-        return ExpertRoutes(idx, _grad.mark(weight), load)
+        choice = []
+        weight = _grad.mark(_RouteExperts.apply(logits, choice, *args))
+        return ExpertRoutes(choice[0], weight, choice[1])
