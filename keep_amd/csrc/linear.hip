@@ -31,7 +31,7 @@ static int64_t linear_size(int dtype) { return dtype == KEEP_E4M3 ? 1 : dtype_si
 
 // ------------------------------------------------------------------ few rows
 
-constexpr int LINEAR_FEW = 16;  // rows
+constexpr int LINEAR_FEW = 16;  // rows of the kernel below
 
 // WAVES waves share 16 rows of W (and of x): wave s takes the s-th share of the summed index and the shares are added in order
 // through LDS. Lane (c, q) holds W row n0 + c, so that its results are outputs n0 + 4 q + v of row c.
@@ -144,37 +144,39 @@ __global__ __launch_bounds__(256) void k_linear_join(LinearGemmArgs a) {
 
 struct LinearPlan {
   int tile, slices;
+  int64_t tiles;
 };
 
-// The tile (64, 128: rows of J, of I 128; 192: 128 of J x 256 of I; 256: 256 x 256) and the slices of a product. 0: the kernel
-// for few rows.
+// The tile and the slices of a product: the largest tile that still gives the CUs about one each. Microseconds of bf16, one
+// launch, tiles of 256 x 256 / 256 x 128 / 128 x 128: 8192 x 4096 -> 8192 454 / 520 / 590; 4096 x 4096 -> 2048 (128, 256
+// and 512 tiles) 106 / 73 / 87. Of fp16, 128 x 128 by one group of waves / by two / 64 x 64 by two: 600 x 4096 -> 2048 (80
+// and 320 tiles) 43 / 32 / 24, 333 x 2880 -> 1440 (36, 138) 31 / 24 / 11.
+// Slices take a second launch, 5 us: they pay where a group of waves would walk more than 24 steps and CUs have no work (64 x 64
+// tiles, one slice against four: 200 x 7168 -> 2048 35 / 14, 64 x 4096 -> 4096 22 / 9, 333 x 2880 -> 1440 11.2 / 11.4).
 static LinearPlan linear_plan(int dtype, int mode, int64_t ni, int64_t nj, int64_t nk) {
-  if (mode == LINEAR_FORWARD && nj <= LINEAR_FEW) return {0, 1};
   const auto tiles = [&](int64_t bi, int64_t bj) { return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj); };
-  int tile = 64;
-  if (dtype == KEEP_BF16 || dtype == KEEP_F16) tile = tiles(256, 256) >= 224 ? 256 : tile;
-  if (tile == 64 && dtype != KEEP_F32 && tiles(256, 128) >= 192) tile = 192;
-  if (tile == 64 && nj > 64 && tiles(128, 128) >= 128) tile = 128;
-  const int64_t n = tile == 256 ? tiles(256, 256) : tile == 192 ? tiles(256, 128) : tiles(128, tile);
-  const int64_t steps = (nk * linear_size(dtype) + 127) / 128;
-  // slices of at least eight steps while the tiles leave CUs without work
-  const int64_t slices = tile > 128 ? 1 : std::max<int64_t>(1, std::min<int64_t>({512 / n, steps / 8, 32}));
-  return {tile, (int)slices};
+  if (mode == LINEAR_FORWARD && nj <= LINEAR_FEW) return {LINEAR_TILE_FEW, 1, tiles(16, 16)};
+  const bool small = dtype == KEEP_F32;
+  if (!small && dtype != KEEP_E4M3 && tiles(256, 256) >= 224) return {LINEAR_TILE_256, 1, tiles(256, 256)};
+  if (!small && tiles(256, 128) >= 192) return {LINEAR_TILE_256_128, 1, tiles(256, 128)};
+  const int64_t n = tiles(128, 128);
+  if (nj > 64 && ni > 64 && n >= 128) return {n <= 256 ? LINEAR_TILE_128_2 : LINEAR_TILE_128, 1, n};
+  const int64_t m = tiles(64, 64), steps = (nk * linear_size(dtype) + 127) / 128;
+  const int64_t slices = steps <= 48 ? 1 : std::max<int64_t>(1, std::min<int64_t>({512 / m, steps / 8, 32}));
+  return {LINEAR_TILE_64, (int)slices, m};
 }
 
 static int64_t linear_part_bytes(const LinearPlan& p, int64_t ni, int64_t nj) {
   return p.slices > 1 ? p.slices * ni * nj * 4 : 0;
 }
 
-static bool linear_gemm_fits(const LinearPlan& p, int64_t ni, int64_t nj) {
-  const int64_t bi = p.tile == 0 ? 16 : p.tile > 128 ? 256 : 128, bj = p.tile == 0 ? 16 : std::min(p.tile, 128);
-  return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj) <= (int64_t(1) << 22) / p.slices;
-}
+// Blocks of a launch: it holds 2^32 threads.
+static bool linear_gemm_fits(const LinearPlan& p) { return p.tiles <= (int64_t(1) << 22) / p.slices; }
 
 static void linear_product(LinearGemmArgs a, int dtype, int mode, const LinearPlan& p, void* part, hipStream_t s) {
   a.slices = p.slices;
   a.part = (float*)part;
-  if (p.tile == 0) {
+  if (p.tile == LINEAR_TILE_FEW) {
     linear_few(a, dtype, s);
     return;
   }
@@ -312,7 +314,7 @@ static int linear_forward(LinearGemmArgs& a, int dtype, void* ws, int64_t ws_byt
   const int64_t need = linear_part_bytes(p, a.ni, a.nj);
   KEEP_REQUIRE(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need),
                "the workspace must hold %lld bytes, 16-byte aligned", (long long)need);
-  KEEP_REQUIRE(linear_gemm_fits(p, a.ni, a.nj), "too many outputs");
+  KEEP_REQUIRE(linear_gemm_fits(p), "too many outputs");
   linear_product(a, dtype, LINEAR_FORWARD, p, ws, s);
   return KEEP_OK;
 }
@@ -377,7 +379,7 @@ extern "C" int keep_linear_grad(const void* dy, const void* u, int act, const vo
   const LinearGradPlan p = linear_grad_plan(dtype, M, N, K);
   KEEP_REQUIRE(workspace && aligned(workspace, 256) && workspace_bytes >= p.bytes,
                "the workspace must hold %lld bytes, 256-byte aligned", (long long)p.bytes);
-  KEEP_REQUIRE(linear_gemm_fits(p.rows, K, M) && linear_gemm_fits(p.weight, K, N), "too many outputs");
+  KEEP_REQUIRE(linear_gemm_fits(p.rows) && linear_gemm_fits(p.weight), "too many outputs");
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   // du: dy itself where no activation changes it and its rows are whole pieces

@@ -156,6 +156,8 @@ struct LinearGemmArgs {
   LinearEpilogue e;
 };
 
+// Columns x rows of a tile, and the groups of waves that share its sum (2: two).
+enum { LINEAR_TILE_FEW = 0, LINEAR_TILE_64, LINEAR_TILE_128_2, LINEAR_TILE_128, LINEAR_TILE_256_128, LINEAR_TILE_256 };
 enum { LINEAR_FORWARD = 0, LINEAR_ROWS = 1, LINEAR_WEIGHT = 2 };  // out, dx, dW
 
 }  // namespace keep

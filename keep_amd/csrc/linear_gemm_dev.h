@@ -7,8 +7,9 @@
 //
 // The side whose index is contiguous in the output is "I", the first MFMA operand (dense_dev.h), the other "J". A step sums
 // 128 bytes of a row: 64 16-bit values, 32 floats, 128 8-bit ones. Its operands are copied to LDS by the DMA path into one of
-// two buffers while the matrix cores work on the other; one barrier a step. Where there are fewer tiles than CUs the summed
-// index is cut into slices, whose float32 sums k_linear_join adds in order.
+// two buffers while the matrix cores work on the other; one barrier a step. Where there are few tiles G groups of waves of a
+// block take a part of the summed index each, in buffers of their own, and their sums are added in LDS; where there are fewer
+// still it is cut into slices too, whose float32 sums k_linear_join adds. Both in order.
 //
 // 8-bit values (e4m3) come with a scale per 128 of a row of x and per 128 x 128 of W: a step is one scale's span, so its
 // products start from zero and enter the sums times both scales, one multiply-add a value.
@@ -41,8 +42,8 @@ struct LinearStep {
 };
 
 // TAIL: the summed index may end inside the last step. (The choice costs every copy of the loop a branch, 8 % of a step.)
-template <typename T, int BI, int BJ, int WI, int WJ, int MODE, bool TAIL>
-__global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) {
+template <typename T, int BI, int BJ, int WI, int WJ, int G, int MODE, bool TAIL>
+__global__ __launch_bounds__(64 * WI * WJ * G) void k_linear_gemm(LinearGemmArgs a) {
   constexpr int NT = 64 * WI * WJ, TI = BI / WI, TJ = BJ / WJ, FI = TI / 16, FJ = TJ / 16;
   constexpr int LI = BI * 8 / NT, LJ = BJ * 8 / NT;  // 16-byte copies per thread and step
   constexpr int SI = BI * 128, SJ = BJ * 128;        // bytes of a buffer's operands
@@ -50,8 +51,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
   constexpr bool TRI = MODE != LINEAR_FORWARD, TRJ = MODE == LINEAR_WEIGHT;
   constexpr bool Q8 = sizeof(T) == 1;
   static_assert(!Q8 || MODE == LINEAR_FORWARD, "8-bit values have no gradient");
-  __shared__ __attribute__((aligned(16))) char smem[2 * (SI + SJ)];
-  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, q = lane >> 4;
+  __shared__ __attribute__((aligned(16))) char smem_all[G * 2 * (SI + SJ)];
+  const int gr = G > 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT) : 0;  // group
+  char* smem = smem_all + gr * (2 * (SI + SJ));
+  const int tid = threadIdx.x - gr * NT, lane = tid & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wv % WI, wj = wv / WI;
 
   // ---- work item (slice, j tile, i tile): items go to the XCDs in contiguous runs; inside a slice, groups of up to 8 j
@@ -66,7 +69,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
   const int64_t i0 = (int64_t)ib * BI, j0 = (int64_t)jb * BJ;
   const int count = (int)min((int64_t)BJ, a.nj - j0);
   const int all = (int)((a.nk + KS - 1) / KS), each = (all + a.slices - 1) / a.slices;
-  const int s0 = min(all, (int)slice * each), s1 = min(all, s0 + each);
+  const int b0 = min(all, (int)slice * each), b1 = min(all, b0 + each);
+  const int turns = (b1 - b0 + G - 1) / G;  // steps of a group; the last ones may have fewer
+  const int s0 = min(b1, b0 + gr * turns), s1 = min(b1, s0 + turns);
 
   // ---- copies of a step. Common case: 32-bit offsets off a base that moves on with the steps. In the last step of a summed
   // index that ends inside it, an address per lane, past the end that of a zero. Rows and columns past the last repeat it:
@@ -83,7 +88,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
     const int L = tid + i * NT;
     if constexpr (!TRI) {
       const int row = L >> 3;
-      oi[i] = (uint32_t)((min(i0 + row, a.ni - 1) - i0) * a.ldi * SZ) + ((L & 7) ^ dg_swz_i(row)) * 16;
+      oi[i] = (uint32_t)((min(i0 + row, a.ni - 1) - i0) * a.ldi * SZ) + ((L & 7) ^ dg_swz_j(row)) * 16;
     } else {
       const int64_t last = (a.ni + V - 1) / V * V - V;
       oi[i] = (uint32_t)(((L / RI) * a.ldi + min(i0 + col_t(L, RI, BI / 16, false), last)) * SZ);
@@ -118,7 +123,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
       asm volatile("" : "+v"(L));  // made here, not kept over the loop
       const bool tr = jside ? TRJ : TRI;
       const int64_t k = (int64_t)step * KS + (tr ? L / (jside ? RJ : RI)
-                                                 : ((L & 7) ^ (jside ? dg_swz_j(L >> 3) : dg_swz_i(L >> 3))) * V);
+                                                 : ((L & 7) ^ dg_swz_j(L >> 3)) * V);
       dg_dma(k < a.nk ? (const void*)(base + o) : (const void*)&g_linear_zero, to);
     }
   };
@@ -128,12 +133,11 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
   for (int j = 0; j < FJ; ++j)
 #pragma unroll
     for (int i = 0; i < FI; ++i) acc[j][i] = f4{0.f, 0.f, 0.f, 0.f};
-  // results of plain I fragments 4 g + u are columns 64 g + 16 q + 4 u + v
   const auto read = [&](int n, int step, int ks) -> uint4 {  // fragment n, the I side's first
     const char* bi = smem + (step & 1) * (SI + SJ);
     const char* bj = bi + SI;
     if (n < FI) {
-      if constexpr (!TRI) return dg_frag<1>(bi, wi * TI + (n >> 2) * 64 + (c >> 2) * 16 + (n & 3) * 4 + (c & 3), ks, q);
+      if constexpr (!TRI) return dg_frag<0>(bi, wi * TI + n * 16 + c, ks, q);
       else if constexpr (SZ == 4) return lg_frag_tf<BI>(bi, wi * FI + n, ks, lane);
       else return dg_frag_t<BI>(bi, wi * FI + n, ks, lane);
     } else {
@@ -161,13 +165,20 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
       const float* sj[FJ];
 #pragma unroll
       for (int j = 0; j < FJ; ++j) sj[j] = a.sj + (j0 + min(wj * TJ + j * 16 + c, count - 1)) * kb;
+      if (s0 < s1) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) copy(i, s0, PART);
-      float xs[FJ], ws = si[s0];
+        for (int i = 0; i < NC; ++i) copy(i, s0, PART);
+      }
+      float xs[FJ], ws = s0 < s1 ? si[s0] : 0.f;
 #pragma unroll
-      for (int j = 0; j < FJ; ++j) xs[j] = sj[j][s0];
+      for (int j = 0; j < FJ; ++j) xs[j] = s0 < s1 ? sj[j][s0] : 0.f;
       landed();
-      for (int s = s0; s < s1; ++s) {
+      for (int turn = 0; turn < turns; ++turn) {
+        const int s = s0 + turn;
+        if (G > 1 && s >= s1) {
+          landed();
+          continue;
+        }
         float nxs[FJ], nws = ws;
         if (s + 1 < s1) {  // into the other buffer, which everybody has read
           nws = si[s + 1];
@@ -228,8 +239,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
         }
       };
       Half h0, h1;
+      if (G == 1 || s0 < s1) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) copy(i, s0, PART);
+        for (int i = 0; i < NC; ++i) copy(i, s0, PART);
+      }
       landed();
       if (s0 + 1 < s1) {
 #pragma unroll
@@ -237,24 +250,25 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
       }
 #pragma unroll
       for (int n = 0; n < NR; ++n) h0.f[n] = read(n, s0, 0);
-      for (int s = s0; s < s1; ++s) {
-        half(h0, h1, s, 1, false, 0);
+      for (int turn = 0; turn < turns; ++turn) {
+        const int s = s0 + turn;
+        if (G == 1 || s < s1) half(h0, h1, s, 1, false, 0);
         landed();  // step s is read by everybody, step s + 1 is there
         // (after the last step h0 takes the buffer's old bytes, not used)
-        half(h1, h0, s + 1, 0, s + 2 < s1, s + 2);
+        if (G == 1 || s < s1) half(h1, h0, s + 1, 0, s + 2 < s1, s + 2);
       }
     }
   };
-  if (s0 < s1) {
+  if (turns > 0) {
     if (TRJ || count == BJ) sum(std::false_type{});
     else if constexpr (!TRJ) sum(std::true_type{});
   }
 
   // ---- results, through LDS: a lane's columns of a row are few and its rows many, a thread of the epilogue takes eight
   // neighbouring columns, so that a row's pieces lie together in memory. FP fragments of every wave at a time.
-  constexpr int FP = 2, ROWS = WJ * FP * 16, PITCH = BI + 4, CG = BI / 8;
+  constexpr int FP = FJ > 1 ? 2 : 1, ROWS = WJ * FP * 16, PITCH = BI + 4, CG = BI / 8;
   static_assert(FJ % FP == 0 && ROWS * PITCH * 4 <= 2 * (SI + SJ) && NT % CG == 0, "LDS");
-  float* tile = (float*)smem;
+  float* tile = (float*)smem_all + gr * (ROWS * PITCH);
   const int64_t col = i0 + (tid % CG) * 8;
   float b[8];
   a.e.load_bias<8>(col, a.ni - col, b);
@@ -267,18 +281,24 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
         const f4 r = acc[p * FP + jj][i];
-        *(float4*)(row + (TRI ? i * 16 + q * 4 : (i >> 2) * 64 + q * 16 + (i & 3) * 4)) = make_float4(r[0], r[1], r[2], r[3]);
+        *(float4*)(row + i * 16 + q * 4) = make_float4(r[0], r[1], r[2], r[3]);
       }
     }
     __syncthreads();
     if (col >= a.ni) continue;
 #pragma unroll 1
-    for (int r = tid / CG; r < ROWS; r += NT / CG) {
+    for (int r = threadIdx.x / CG; r < ROWS; r += G * NT / CG) {
       const int64_t row = j0 + (r / (FP * 16)) * TJ + p * (FP * 16) + r % (FP * 16);
       if (row >= a.nj) continue;
-      const float* from = tile + r * PITCH + (tid % CG) * 8;
-      const float4 lo = *(const float4*)from, hi = *(const float4*)(from + 4);
-      float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      const float* from = (const float*)smem_all + r * PITCH + (tid % CG) * 8;
+      float f[8];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float4 lo = *(const float4*)(from + g * (ROWS * PITCH)), hi = *(const float4*)(from + g * (ROWS * PITCH) + 4);
+        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int u = 0; u < 8; ++u) f[u] = g == 0 ? v[u] : f[u] + v[u];
+      }
       if (a.slices > 1)
         dense_st<float, 8>(a.part + ((int64_t)slice * a.nj + row) * a.ni + col, a.ni - col, f, a.ni % 4 == 0);
       else
@@ -287,22 +307,24 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_linear_gemm(LinearGemmArgs a) 
   }
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, int MODE>
+template <typename T, int BI, int BJ, int WI, int WJ, int G, int MODE>
 void linear_gemm_launch(const LinearGemmArgs& a, hipStream_t s) {
   const int64_t items = ((a.ni + BI - 1) / BI) * ((a.nj + BJ - 1) / BJ) * a.slices;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * WI * WJ);
+  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * WI * WJ * G);
   if (a.nk % LinearStep<T>::K == 0)
-    hipLaunchKernelGGL((k_linear_gemm<T, BI, BJ, WI, WJ, MODE, false>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((k_linear_gemm<T, BI, BJ, WI, WJ, MODE, true>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((k_linear_gemm<T, BI, BJ, WI, WJ, G, MODE, false>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((k_linear_gemm<T, BI, BJ, WI, WJ, G, MODE, true>), grid, block, 0, s, a);
 }
 
 template <typename T, int MODE>
 void linear_gemm_tile(const LinearGemmArgs& a, int tile, hipStream_t s) {
-  if (tile == 64) linear_gemm_launch<T, 128, 64, 2, 2, MODE>(a, s);
-  else if constexpr (sizeof(T) == 4) linear_gemm_launch<T, 128, 128, 2, 2, MODE>(a, s);
-  else if (tile == 128) linear_gemm_launch<T, 128, 128, 2, 2, MODE>(a, s);
-  else if (tile == 192 || sizeof(T) == 1) linear_gemm_launch<T, 256, 128, 4, 2, MODE>(a, s);
-  else if constexpr (sizeof(T) == 2) linear_gemm_launch<T, 256, 256, 4, 2, MODE>(a, s);
+  if (tile == LINEAR_TILE_64) linear_gemm_launch<T, 64, 64, 2, 2, 2, MODE>(a, s);
+  else if (tile == LINEAR_TILE_128_2) linear_gemm_launch<T, 128, 128, 2, 2, 2, MODE>(a, s);
+  else if (sizeof(T) == 4 || tile == LINEAR_TILE_128) linear_gemm_launch<T, 128, 128, 2, 2, 1, MODE>(a, s);
+  else if constexpr (sizeof(T) < 4) {
+    if (sizeof(T) == 1 || tile == LINEAR_TILE_256_128) linear_gemm_launch<T, 256, 128, 4, 2, 1, MODE>(a, s);
+    else if constexpr (sizeof(T) == 2) linear_gemm_launch<T, 256, 256, 4, 2, 1, MODE>(a, s);
+  }
 }
 
 template <typename T>
