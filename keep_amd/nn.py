@@ -11,6 +11,10 @@
   the three MFMA grouped GEMMs (``_shared_sorted_route_prefill``).
 - ``SwitchLinear`` -- the same stacked projection on dense weights, for experts
   that stay unquantised; differentiable.
+- ``DenseLinear``, ``DenseGLU`` -- a dense projection with its epilogue and a dense
+  shared expert; differentiable.
+- ``MoEGate`` -- the router's product and the choice of experts among groups
+  (``deepseek_v4_flash_adapter.py:989-1036``); differentiable.
 - ``LimitedSwiGLU`` -- ``deepseek_v4_flash_adapter.py:962-986``.
 - ``RoutedVQMoE`` -- router + experts + weighted combine
   (``DeepseekV4FlashVQMoE.__call__``, ``deepseek_v4_flash_adapter.py:1776-1784``),
@@ -27,7 +31,8 @@ import torch
 from keep_amd import _grad, _lib, ops
 from keep_amd.dense import gather_mm
 from keep_amd.lora import LoraAdapters
-from keep_amd.router import RouterOutput, _slot_args, router_dual_topk
+from keep_amd.projection import ACTIVATIONS, linear
+from keep_amd.router import ExpertRoutes, RouterOutput, _slot_args, route_experts, router_dual_topk
 
 CODEWORD_DIM = 8
 
@@ -354,6 +359,89 @@ class SwitchLinear:
         return y if adapter_indices is None else _add_adapters(self, y, rows.view(x.shape), indices, adapter_indices)
 
 
+class DenseLinear:
+    """A dense projection ``[out, in]`` with its epilogue (``linear``): ``residual + act(x W^T + bias)``, differentiable.
+    Rows are taken in the weight's dtype. Weights stay as they are given (a tensor that requires a gradient gets it)."""
+
+    code_bits = adapters = rht_signs = rotation_matrix = None  # no codes and no adapters
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None):
+        if weight.ndim != 2 or 0 in weight.shape or weight.dtype not in ops._DT:
+            raise ValueError("weight must be 2D [out, in] in float32, float16 or bfloat16, found "
+                             f"{tuple(weight.shape)} in {weight.dtype}")
+        self.output_dims, self.input_dims = weight.shape
+        if bias is not None and tuple(bias.shape) != (self.output_dims,):
+            raise ValueError(f"bias must have shape ({self.output_dims},), found {tuple(bias.shape)}")
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, found {activation!r}")
+        self.weight, self.bias, self.activation = weight, bias, activation
+
+    def __call__(self, x: torch.Tensor, *, residual: torch.Tensor | None = None,
+                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        return linear(x.to(self.weight.dtype), self.weight, self.bias, activation=self.activation, residual=residual,
+                      out_dtype=out_dtype)
+
+
+class DenseGLU:
+    """A dense SwiGLU expert, ``down(act(up(x), gate(x)))``: a shared expert of plain ``[out, in]`` projections (the
+    reference's are, ``deepseek_v4_flash_adapter.py:1777-1784``), without the routes of a one-expert
+    ``QuantizedVQSwitchGLU``. The projections have no activation of their own; without ``activation`` the gate's silu is
+    formed in its product's epilogue."""
+
+    num_experts = 1
+
+    def __init__(self, *, gate_proj: DenseLinear, up_proj: DenseLinear, down_proj: DenseLinear,
+                 activation: Callable | None = None):
+        if gate_proj.input_dims != up_proj.input_dims or gate_proj.output_dims != up_proj.output_dims:
+            raise ValueError("gate_proj and up_proj dimensions must match")
+        if down_proj.input_dims != gate_proj.output_dims or down_proj.output_dims != gate_proj.input_dims:
+            raise ValueError("down_proj must map the hidden dimension back to the input dimension")
+        if any(p.activation is not None for p in (gate_proj, up_proj, down_proj)):
+            raise ValueError("the projections of a DenseGLU have no activation of their own")
+        self.gate_proj, self.up_proj, self.down_proj, self.activation = gate_proj, up_proj, down_proj, activation
+        self.input_dims, self.hidden_dims = gate_proj.input_dims, gate_proj.output_dims
+
+    def __call__(self, x: torch.Tensor, *, residual: torch.Tensor | None = None,
+                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        g, up = self.gate_proj, self.up_proj(x)
+        if self.activation is None:
+            hidden = linear(x.to(g.weight.dtype), g.weight, g.bias, activation="silu") * up
+        else:
+            hidden = self.activation(up, g(x))
+        return self.down_proj(hidden, residual=residual, out_dtype=out_dtype)
+
+
+class MoEGate:
+    """The router of a MoE layer: float32 logits ``x W^T`` and ``route_experts`` on them, differentiable in ``x`` and
+    ``weight [E, H]``. ``bias [E]`` (float32) balances the choice: ``update_bias`` moves it against the experts'
+    loads."""
+
+    def __init__(self, weight: torch.Tensor, *, top_k: int, bias: torch.Tensor | None = None,
+                 score_func: str = "softmax", groups: int = 1, topk_groups: int | None = None, renormalize: bool = True,
+                 route_scale: float = 1.0, count_load: bool = False):
+        self.proj = DenseLinear(weight)
+        self.num_experts, self.input_dims = weight.shape
+        if bias is not None and tuple(bias.shape) != (self.num_experts,):
+            raise ValueError(f"bias must have shape ({self.num_experts},), found {tuple(bias.shape)}")
+        self.top_k, self.bias, self.score_func = top_k, bias, score_func
+        self.groups, self.topk_groups = groups, topk_groups
+        self.renormalize, self.route_scale, self.count_load = renormalize, route_scale, count_load
+
+    def __call__(self, x: torch.Tensor) -> ExpertRoutes:
+        return route_experts(self.proj(x, out_dtype=torch.float32), self.top_k, bias=self.bias,
+                             score_func=self.score_func, groups=self.groups, topk_groups=self.topk_groups,
+                             renormalize=self.renormalize, route_scale=self.route_scale, count_load=self.count_load)
+
+    def update_bias(self, load: torch.Tensor, rate: float) -> None:
+        """``bias += rate * sign(mean(load) - load)``: experts with more tokens than the mean lose, the others gain."""
+
+        if self.bias is None:
+            raise ValueError("the gate has no bias")
+        counts = load.to(torch.float32)
+        with torch.no_grad():
+            self.bias += rate * torch.sign(counts.mean() - counts)
+
+
 class HotTier:
     """The nested 3-bit tier of a routed SwiGLU block: for the experts with a
     row in ``hot_of_slot`` (``uint32 [E]``, ``0xFFFFFFFF`` = none), an 8-bit E8
@@ -497,9 +585,12 @@ class QuantizedVQSwitchGLU:
                 return False
         return True
 
-    def _can_use_shared_sorted_route_prefill(self, x: torch.Tensor, indices: torch.Tensor) -> bool:
+    def _can_use_shared_sorted_route_prefill(self, x: torch.Tensor, indices: torch.Tensor,
+                                             least: int | None = None) -> bool:
+        """``least``: the routes from which it pays, without any other reason to take it."""
+
         routes = indices.numel()
-        return (self._all_e8p() and routes >= ops.GEMM_ROUTE_THRESHOLD
+        return (self._all_e8p() and routes >= (ops.GEMM_ROUTE_THRESHOLD if least is None else least)
                 and all(ops.gemm_eligible(code_bits=16, x_dtype=x.dtype, input_dims=p.input_dims,
                                           group_size=p.group_size)
                         for p in (self.gate_proj, self.up_proj, self.down_proj)))
@@ -1006,7 +1097,8 @@ def moe_layer(x: torch.Tensor, logits: torch.Tensor, gate, up, down, *, k: int, 
 
 
 def _holds_codes(glu) -> bool:
-    return glu is not None and not all(isinstance(p, SwitchLinear) for p in (glu.gate_proj, glu.up_proj, glu.down_proj))
+    return glu is not None and not all(isinstance(p, (SwitchLinear, DenseLinear))
+                                       for p in (glu.gate_proj, glu.up_proj, glu.down_proj))
 
 
 def _has_adapters(glu) -> bool:
@@ -1049,8 +1141,14 @@ class RoutedVQMoE:
                  renormalize: bool = True, route_scale: float = 1.0, swiglu_limit: float = 0.0,
                  bias_served: torch.Tensor | None = None, bias_demand: torch.Tensor | None = None,
                  tau: float = float("inf"), decode_max_tokens: int = 64, out_dtype=torch.float32,
-                 shared_experts: QuantizedVQSwitchGLU | None = None, slot_map: torch.Tensor | None = None,
-                 one_launch: bool = False):
+                 shared_experts: QuantizedVQSwitchGLU | DenseGLU | None = None, slot_map: torch.Tensor | None = None,
+                 one_launch: bool = False, gate: MoEGate | None = None):
+        if gate is not None:
+            if slot_map is not None:
+                raise ValueError("a gate's experts are glu's own: it takes no slot_map")
+            if gate.input_dims != glu.input_dims or gate.num_experts != glu.num_experts or gate.top_k != top_k:
+                raise ValueError(f"the gate must route {glu.input_dims} values to {top_k} of {glu.num_experts} experts")
+        self.gate = gate
         self.glu, self.top_k, self.score_func = glu, top_k, score_func
         self.one_launch = bool(one_launch)
         self.renormalize, self.route_scale, self.limit = renormalize, route_scale, float(swiglu_limit)
@@ -1061,7 +1159,7 @@ class RoutedVQMoE:
             glu.activation = LimitedSwiGLU(self.limit)
         if shared_experts is not None:
             if shared_experts.num_experts != 1:
-                raise ValueError("shared_experts must be a one-expert QuantizedVQSwitchGLU")
+                raise ValueError("shared_experts must be a one-expert QuantizedVQSwitchGLU or a DenseGLU")
             if shared_experts.input_dims != glu.input_dims:
                 raise ValueError("shared_experts input dimension must match the routed experts'")
             if shared_experts.activation is None and self.limit > 0:
@@ -1074,6 +1172,8 @@ class RoutedVQMoE:
         adapters."""
 
         se = self.shared_experts
+        if isinstance(se, DenseGLU):
+            return se(x).float()
         T = x.shape[0]
         idx = torch.zeros((T, 1), dtype=torch.int32, device=x.device)
         w = torch.ones((T, 1), dtype=torch.float32, device=x.device)
@@ -1094,10 +1194,13 @@ class RoutedVQMoE:
         if adapter_indices is not None:
             return ops.route_combine(self.glu(x, idx, adapter_indices), weight, od)
         if (T <= self.decode_max_tokens and self.glu._all_e8p() and self.glu.hot_tier is None
-                and x.dtype in (torch.float16, torch.bfloat16)):
+                and x.dtype in (torch.float16, torch.bfloat16) and not _grad.wanted(weight)):
             return moe_decode(x, idx, weight, (g.codes, g.scales), (u.codes, u.scales), (d.codes, d.scales),
                               limit=self.limit, codebook=g.codebook, out_dtype=od)
-        y = self.glu(x, idx)  # [T, k, H]
+        if _grad.wanted(weight) and self.glu._can_use_shared_sorted_route_prefill(x, idx, least=1):
+            y = self.glu._shared_sorted_route_prefill(x, idx)  # few routes too: its rows are float32, as moe_decode's sums
+        else:
+            y = self.glu(x, idx)  # [T, k, H]
         out = ops.route_combine(y, weight, od)
         return _grad.partial(out, x) if out.requires_grad and _holds_codes(self.glu) else out
 
@@ -1124,8 +1227,10 @@ class RoutedVQMoE:
             return None  # fewer logits than pool rows: routed apart
         return None if entry is None else entry + "_layer"
 
-    def __call__(self, x: torch.Tensor, logits: torch.Tensor, *, residual: torch.Tensor | None = None,
+    def __call__(self, x: torch.Tensor, logits: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
                  adapter_indices=None):
+        if logits is None and self.gate is None:
+            raise ValueError("a layer without a gate needs logits")
         extra = self.shared_experts is not None or residual is not None
         od = torch.float32 if extra else self.out_dtype
         shared_adapters = None
@@ -1133,8 +1238,11 @@ class RoutedVQMoE:
             shared_adapters = adapter_indices
             if not _has_adapters(self.glu):
                 adapter_indices = None
-        entry = self._tiles_layer_path(x, logits) if adapter_indices is None else None
-        if entry is not None:
+        entry = self._tiles_layer_path(x, logits) if adapter_indices is None and logits is not None else None
+        if logits is None:
+            r = self.gate(x)
+            out = self.experts(x, r.idx, r.weight, out_dtype=od, adapter_indices=adapter_indices)
+        elif entry is not None:
             g, u, d = self.glu.gate_proj, self.glu.up_proj, self.glu.down_proj
             out, r = _tiles_layer(entry, x, logits, (g.codes, g.scales), (u.codes, u.scales), (d.codes, d.scales),
                                   self.top_k, self.bias_served, self.bias_demand, self.score_func, self.renormalize,
