@@ -214,8 +214,7 @@ __global__ __launch_bounds__(256) void k_linear_du(LinearDuArgs a) {
       linear_ld<T, 8>((const T*)a.dy + r * a.N + col, left, d, vec);
       if (a.act) {
         linear_ld<T, 8>((const T*)a.u + r * a.N + col, left, u, vec);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] *= linear_slope(u[i], a.act);
+        linear_slope<8>(d, u, a.act);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] += d[i];
@@ -223,7 +222,7 @@ __global__ __launch_bounds__(256) void k_linear_du(LinearDuArgs a) {
         if (left < 8)
 #pragma unroll
           for (int i = 0; i < 8; ++i) d[i] = i < left ? d[i] : 0.f;
-        dense_st<T, 8>((T*)a.du + r * a.ld + col, a.ld - col, d, true);
+        linear_st<T, 8>((T*)a.du + r * a.ld + col, a.ld - col, d, true);
       }
     }
   }

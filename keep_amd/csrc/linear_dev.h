@@ -1,6 +1,8 @@
 #pragma once
 // What the dense projection's kernels share: the epilogue and the arguments of the products through LDS.
 //   u = x W^T + b,  out = round(residual + act(u))
+#include <type_traits>
+
 #include "dense_dev.h"
 
 namespace keep {
@@ -17,7 +19,10 @@ __device__ __forceinline__ float linear_sigmoid(float u) { return __builtin_amdg
 
 constexpr float GELU_C = 0.7978845608028654f;  // sqrt(2 / pi)
 
-__device__ __forceinline__ float linear_act(float u, int act) {
+// (ACT by value: a choice per value would be a branch per value.)
+template <int ACT>
+__device__ __forceinline__ float linear_act(float u) {
+  constexpr int act = ACT;
   if (act == LINEAR_RELU) return u > 0.f ? u : u != u ? u : 0.f;
   if (act == LINEAR_SILU) return u * linear_sigmoid(u);
   if (act == LINEAR_GELU) return 0.5f * u * erfcf(u * -0.7071067811865476f);  // (erfc keeps the lower tail's bits)
@@ -26,7 +31,21 @@ __device__ __forceinline__ float linear_act(float u, int act) {
   return u;
 }
 
-__device__ __forceinline__ float linear_slope(float u, int act) {
+template <int V>
+__device__ __forceinline__ void linear_act(float (&f)[V], int act) {
+  const auto all = [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = linear_act<decltype(a)::value>(f[i]);
+  };
+  if (act == LINEAR_SILU) all(std::integral_constant<int, LINEAR_SILU>{});
+  else if (act == LINEAR_GELU) all(std::integral_constant<int, LINEAR_GELU>{});
+  else if (act == LINEAR_GELU_TANH) all(std::integral_constant<int, LINEAR_GELU_TANH>{});
+  else if (act == LINEAR_RELU) all(std::integral_constant<int, LINEAR_RELU>{});
+}
+
+template <int ACT>
+__device__ __forceinline__ float linear_slope(float u) {
+  constexpr int act = ACT;
   if (act == LINEAR_RELU) return u > 0.f ? 1.f : u != u ? u : 0.f;
   if (act == LINEAR_SILU) {
     const float p = linear_sigmoid(u);
@@ -65,6 +84,19 @@ __device__ __forceinline__ void linear_e4m3(const uint4& a, const uint4& b, line
   f[3] = linear_e4m3(b.z, b.w);
 }
 
+// d *= act'(u)
+template <int V>
+__device__ __forceinline__ void linear_slope(float (&d)[V], const float (&u)[V], int act) {
+  const auto all = [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] *= linear_slope<decltype(a)::value>(u[i]);
+  };
+  if (act == LINEAR_SILU) all(std::integral_constant<int, LINEAR_SILU>{});
+  else if (act == LINEAR_GELU) all(std::integral_constant<int, LINEAR_GELU>{});
+  else if (act == LINEAR_GELU_TANH) all(std::integral_constant<int, LINEAR_GELU_TANH>{});
+  else if (act == LINEAR_RELU) all(std::integral_constant<int, LINEAR_RELU>{});
+}
+
 // n <= V neighbouring values of a row; vec: V of them at an address aligned to them.
 template <typename T, int V>
 __device__ __forceinline__ void linear_ld(const T* p, int64_t n, float (&f)[V], bool vec) {
@@ -96,11 +128,37 @@ __device__ __forceinline__ void linear_ld_any(const void* p, int dt, int64_t at,
   else linear_ld<_Float16, V>((const _Float16*)p + at, n, f, vec);
 }
 
+// V neighbouring values of a row, n of them inside. Pairs are rounded by one instruction each (to nearest even, NaN kept).
+template <typename T, int V>
+__device__ __forceinline__ void linear_st(T* p, int64_t n, const float (&f)[V], bool vec) {
+  if constexpr (sizeof(T) == 2) {
+    if (vec && n >= V) {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+      uint32_t w[V / 2];
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        if constexpr (__is_same(T, bf16s))
+          w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{f[2 * i], f[2 * i + 1]}, b2_t));
+        else w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{f[2 * i], f[2 * i + 1]}, h2_t));
+      }
+      if constexpr (V % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < V / 8; ++i)
+          ((uint4*)p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      } else {
+        *(uint2*)p = make_uint2(w[0], w[1]);
+      }
+      return;
+    }
+  }
+  dense_st<T, V>(p, n, f, vec);
+}
+
 template <int V>
 __device__ __forceinline__ void linear_st_any(void* p, int dt, int64_t at, int64_t n, const float (&f)[V], bool vec) {
-  if (dt == KEEP_F32) dense_st<float, V>((float*)p + at, n, f, vec);
-  else if (dt == KEEP_BF16) dense_st<bf16s, V>((bf16s*)p + at, n, f, vec);
-  else dense_st<_Float16, V>((_Float16*)p + at, n, f, vec);
+  if (dt == KEEP_F32) linear_st<float, V>((float*)p + at, n, f, vec);
+  else if (dt == KEEP_BF16) linear_st<bf16s, V>((bf16s*)p + at, n, f, vec);
+  else linear_st<_Float16, V>((_Float16*)p + at, n, f, vec);
 }
 
 struct LinearEpilogue {
@@ -124,9 +182,7 @@ struct LinearEpilogue {
 #pragma unroll
       for (int i = 0; i < V; ++i) f[i] += b[i];
     if (u) linear_st_any<V>(u, udt, at, n, f, v);
-    if (act)
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = linear_act(f[i], act);
+    if (act) linear_act<V>(f, act);
     if (res) {
       float r[V];
       linear_ld_any<V>(res, rdt, at, n, r, v);

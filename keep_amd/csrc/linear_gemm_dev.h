@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * WI * WJ * G) void k_linear_gemm(LinearGemmArgs
     }
     __syncthreads();
     if (col >= a.ni) continue;
-#pragma unroll 1
+#pragma unroll 2
     for (int r = threadIdx.x / CG; r < ROWS; r += G * NT / CG) {
       const int64_t row = j0 + (r / (FP * 16)) * TJ + p * (FP * 16) + r % (FP * 16);
       if (row >= a.nj) continue;
