@@ -37,7 +37,7 @@ __device__ __forceinline__ float norm_pow2_ceil(float v) {
 }
 
 // X: type of x and y; R: of the residual (void: none).
-template <typename X, typename R, int TPR, int NV, bool EVEN, bool QUANT>
+template <typename X, typename R, int TPR, int NV, int END, bool QUANT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm(NormArgs a) {
   constexpr int BT = TPR < 256 ? 256 : TPR, RPB = BT / TPR;
   __shared__ float red[BT / 64];
@@ -50,11 +50,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm(NormArgs a) {
     float h[NV][8];
     float ss = 0.f;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) norm_ld<EVEN>((const X*)a.x + at, (v * TPR + t) * 8, n, h[v]);
+    for (int v = 0; v < NV; ++v) norm_ld<END>((const X*)a.x + at, (v * TPR + t) * 8, n, h[v]);
     if constexpr (RES) {
       float p[NV][8];
 #pragma unroll
-      for (int v = 0; v < NV; ++v) norm_ld<EVEN>((const R*)a.res + at, (v * TPR + t) * 8, n, p[v]);
+      for (int v = 0; v < NV; ++v) norm_ld<END>((const R*)a.res + at, (v * TPR + t) * 8, n, p[v]);
 #pragma unroll
       for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -75,7 +75,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm(NormArgs a) {
     if constexpr (RES) {
       if (live)
 #pragma unroll
-        for (int v = 0; v < NV; ++v) norm_st<EVEN>((R*)a.h + at, (v * TPR + t) * 8, n, h[v]);
+        for (int v = 0; v < NV; ++v) norm_st<END>((R*)a.h + at, (v * TPR + t) * 8, n, h[v]);
     }
     ss = norm_sum<TPR, BT>(ss, red);
     const float r = 1.f / sqrtf(ss / (float)n + a.eps);
@@ -84,11 +84,11 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm(NormArgs a) {
     for (int v = 0; v < NV; ++v) {
       const int i = (v * TPR + t) * 8;
       float w[8];
-      norm_weight<EVEN>(a.w, a.wdt, i, n, w);
+      norm_weight<END>(a.w, a.wdt, i, n, w);
 #pragma unroll
       for (int u = 0; u < 8; ++u) h[v][u] = h[v][u] * r * w[u];
       if constexpr (!QUANT) {
-        if (live) norm_st<EVEN>((X*)a.y + at, i, n, h[v]);
+        if (live) norm_st<END>((X*)a.y + at, i, n, h[v]);
       } else {
         // a maximum of the bits, which a NaN outranks
         uint32_t bits = 0u;
@@ -124,10 +124,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rmsnorm(NormArgs a) {
 
 template <typename X, typename R, bool QUANT>
 static void norm_launch(const NormArgs& a, hipStream_t s) {
-  norm_by_width(a.n, [&](auto tpr, auto nv, auto even) {
+  norm_by_width(a.n, [&](auto tpr, auto nv, auto end) {
     constexpr int TPR = decltype(tpr)::value, BT = TPR < 256 ? 256 : TPR;
     const dim3 grid((unsigned)std::min<int64_t>((a.T + BT / TPR - 1) / (BT / TPR), NORM_BLOCKS));
-    hipLaunchKernelGGL((k_rmsnorm<X, R, TPR, decltype(nv)::value, decltype(even)::value, QUANT>), grid, dim3(BT), 0, s, a);
+    hipLaunchKernelGGL((k_rmsnorm<X, R, TPR, decltype(nv)::value, decltype(end)::value, QUANT>), grid, dim3(BT), 0, s, a);
   });
 }
 

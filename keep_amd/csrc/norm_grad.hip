@@ -24,7 +24,7 @@ constexpr int norm_grad_block(int tpr) { return tpr < 256 ? 256 : tpr; }
 // H: type of h, dh and dresidual; X: of dy and dx. A block takes every gridDim-th group of rows, reads a group's values while
 // it works on the one before, and adds its share of dw in registers, so that the shares that are left for k_parts_sum are as
 // many as blocks.
-template <typename X, typename H, int TPR, int NV, bool EVEN>
+template <typename X, typename H, int TPR, int NV, int END>
 __global__ __launch_bounds__(norm_grad_block(TPR)) void k_rmsnorm_grad(NormGradArgs a) {
   constexpr int BT = norm_grad_block(TPR), RPB = BT / TPR;
   __shared__ float red[BT / 64];
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(norm_grad_block(TPR)) void k_rmsnorm_grad(NormGradA
     for (int u = 0; u < 8; ++u) dw[v][u] = 0.f;
   float w[NV][8];
 #pragma unroll
-  for (int v = 0; v < NV; ++v) norm_weight<EVEN>(a.w, a.wdt, (v * TPR + t) * 8, n, w[v]);
+  for (int v = 0; v < NV; ++v) norm_weight<END>(a.w, a.wdt, (v * TPR + t) * 8, n, w[v]);
   struct Row {
     NormRaw<H> h[NV], dh[NV];
     NormRaw<X> dy[NV];
@@ -48,27 +48,31 @@ __global__ __launch_bounds__(norm_grad_block(TPR)) void k_rmsnorm_grad(NormGradA
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int i = (v * TPR + t) * 8;
-      o.h[v].template load<EVEN>((const H*)a.h + at * n, i, n);
-      o.dy[v].template load<EVEN>((const X*)a.dy + at * n, i, n);
-      if (a.dh) o.dh[v].template load<EVEN>((const H*)a.dh + at * n, i, n);
+      o.h[v].template load<END>((const H*)a.h + at * n, i, n);
+      o.dy[v].template load<END>((const X*)a.dy + at * n, i, n);
+      if (a.dh) o.dh[v].template load<END>((const H*)a.dh + at * n, i, n);
     }
     o.r = a.rstd[at];
   };
   const int64_t step = (int64_t)gridDim.x * RPB;
+  // 1024 threads have 128 registers each, which two rows do not fit (2048 x 16384 bf16: 98 us with spills, 76 without)
+  constexpr bool AHEAD = TPR < 1024;
   Row next;
-  load(next, (int64_t)blockIdx.x * RPB + sub);
+  if constexpr (AHEAD) load(next, (int64_t)blockIdx.x * RPB + sub);
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.T; r0 += step) {
     const int64_t row = r0 + sub;
     const bool live = row < a.T;
     const int64_t at = row * n;
+    if constexpr (!AHEAD) load(next, row);
     const Row now = next;
-    if (r0 + step < a.T) load(next, row + step);
+    if (AHEAD && r0 + step < a.T) load(next, row + step);
     float h[NV][8], g[NV][8];
     float c = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      now.h[v].get(h[v]);
-      now.dy[v].get(g[v]);
+      const int i = (v * TPR + t) * 8;
+      now.h[v].template get<END>(i, n, h[v]);
+      now.dy[v].template get<END>(i, n, g[v]);
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         if (live) dw[v][u] = fmaf(g[v][u], h[v][u] * now.r, dw[v][u]);
@@ -83,14 +87,14 @@ __global__ __launch_bounds__(norm_grad_block(TPR)) void k_rmsnorm_grad(NormGradA
     for (int v = 0; v < NV; ++v) {
       const int i = (v * TPR + t) * 8;
       float d[8];
-      now.dh[v].get(d);
+      now.dh[v].template get<END>(i, n, d);
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const float e = now.r * fmaf(-h[v][u], k, g[v][u]);
         d[u] = a.dh ? e + d[u] : e;
       }
-      if (a.dx) norm_st<EVEN>((X*)a.dx + at, i, n, d);
-      if (a.dres) norm_st<EVEN>((H*)a.dres + at, i, n, d);
+      if (a.dx) norm_st<END>((X*)a.dx + at, i, n, d);
+      if (a.dres) norm_st<END>((H*)a.dres + at, i, n, d);
     }
   }
   if (!a.part) return;
@@ -112,25 +116,26 @@ __global__ __launch_bounds__(norm_grad_block(TPR)) void k_rmsnorm_grad(NormGradA
     if (sub > 0) return;
   }
 #pragma unroll
-  for (int v = 0; v < NV; ++v) norm_st<EVEN>(a.part + (int64_t)blockIdx.x * n, (v * TPR + t) * 8, n, dw[v]);
+  for (int v = 0; v < NV; ++v) norm_st<END>(a.part + (int64_t)blockIdx.x * n, (v * TPR + t) * 8, n, dw[v]);
 }
 
-// f(TPR, NV, EVEN) for rows of n values: two vectors a thread, whose row and the one to come are in registers.
+// f(TPR, NV, END) for rows of n values: two vectors a thread, whose row and the one to come are in registers.
 template <typename F>
 static void norm_grad_by_width(int64_t n, F f) {
   using std::integral_constant;
   constexpr integral_constant<int, 1> one;
   constexpr integral_constant<int, 2> two;
-  if (n % 8) {
-    if (n <= 1024) f(integral_constant<int, 64>{}, two, std::false_type{});
-    else if (n <= 4096) f(integral_constant<int, 256>{}, two, std::false_type{});
-    else f(integral_constant<int, 1024>{}, two, std::false_type{});
-  } else if (n <= 512) f(integral_constant<int, 64>{}, one, std::true_type{});
-  else if (n <= 1024) f(integral_constant<int, 64>{}, two, std::true_type{});
-  else if (n <= 2048) f(integral_constant<int, 128>{}, two, std::true_type{});
-  else if (n <= 4096) f(integral_constant<int, 256>{}, two, std::true_type{});
-  else if (n <= 8192) f(integral_constant<int, 512>{}, two, std::true_type{});
-  else f(integral_constant<int, 1024>{}, two, std::true_type{});
+  const auto by = [&](auto end) {
+    if (n <= 512) f(integral_constant<int, 64>{}, one, end);
+    else if (n <= 1024) f(integral_constant<int, 64>{}, two, end);
+    else if (n <= 2048) f(integral_constant<int, 128>{}, two, end);
+    else if (n <= 4096) f(integral_constant<int, 256>{}, two, end);
+    else if (n <= 8192) f(integral_constant<int, 512>{}, two, end);
+    else f(integral_constant<int, 1024>{}, two, end);
+  };
+  if (n < 8) f(integral_constant<int, 64>{}, one, integral_constant<int, NORM_TINY>{});
+  else if (n % 8) by(integral_constant<int, NORM_ODD>{});
+  else by(integral_constant<int, NORM_EVEN>{});
 }
 
 // Rows of a block of k_rmsnorm_grad, and its blocks: three per CU, as many as their registers let in.
@@ -146,9 +151,9 @@ static int64_t norm_parts(int64_t T, int64_t n) {
 
 template <typename X, typename H>
 static void norm_grad_launch(const NormGradArgs& a, int64_t blocks, hipStream_t s) {
-  norm_grad_by_width(a.n, [&](auto tpr, auto nv, auto even) {
+  norm_grad_by_width(a.n, [&](auto tpr, auto nv, auto end) {
     constexpr int TPR = decltype(tpr)::value, BT = norm_grad_block(TPR);
-    hipLaunchKernelGGL((k_rmsnorm_grad<X, H, TPR, decltype(nv)::value, decltype(even)::value>), dim3((unsigned)blocks), dim3(BT), 0, s, a);
+    hipLaunchKernelGGL((k_rmsnorm_grad<X, H, TPR, decltype(nv)::value, decltype(end)::value>), dim3((unsigned)blocks), dim3(BT), 0, s, a);
   });
 }
 
