@@ -77,7 +77,7 @@ __global__ __launch_bounds__(64 * WI * WJ * G) void k_linear_gemm(LinearGemmArgs
   // index that ends inside it, an address per lane, past the end that of a zero. Rows and columns past the last repeat it:
   // their results are not stored.
   constexpr int RI = BI * SZ / 16, RJ = BJ * SZ / 16;  // 16-byte slots of a transposed row
-  const auto col_t = [](int L, int R, int groups, bool) -> int {  // first column of slot L of a transposed operand
+  const auto col_t = [](int L, int R, int groups) -> int {  // first column of slot L of a transposed operand
     const int row = L / R, sl = L % R;
     if constexpr (SZ == 4) return (((sl >> 2) ^ lg_swz_tf(row)) * 4 + (sl & 3)) * 4;
     else return (((sl >> 1) ^ (((row & 3) | (((row >> 3) & 1) << 2)) & (groups - 1))) * 2 + (sl & 1)) * 8;
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(64 * WI * WJ * G) void k_linear_gemm(LinearGemmArgs
       oi[i] = (uint32_t)((min(i0 + row, a.ni - 1) - i0) * a.ldi * SZ) + ((L & 7) ^ dg_swz_j(row)) * 16;
     } else {
       const int64_t last = (a.ni + V - 1) / V * V - V;
-      oi[i] = (uint32_t)(((L / RI) * a.ldi + min(i0 + col_t(L, RI, BI / 16, false), last)) * SZ);
+      oi[i] = (uint32_t)(((L / RI) * a.ldi + min(i0 + col_t(L, RI, BI / 16), last)) * SZ);
     }
   }
 #pragma unroll
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(64 * WI * WJ * G) void k_linear_gemm(LinearGemmArgs
       oj[i] = (uint32_t)(min(row, count - 1) * a.ldj * SZ) + ((L & 7) ^ dg_swz_j(row)) * 16;
     } else {
       const int64_t last = (a.nj + V - 1) / V * V - V;
-      oj[i] = (uint32_t)(((L / RJ) * a.ldj + min(j0 + col_t(L, RJ, BJ / 16, true), last)) * SZ);
+      oj[i] = (uint32_t)(((L / RJ) * a.ldj + min(j0 + col_t(L, RJ, BJ / 16), last)) * SZ);
     }
   }
   const char* ibase = (const char*)a.pi + (TRI ? 0 : i0 * a.ldi * SZ);
