@@ -31,22 +31,29 @@ static int64_t linear_size(int dtype) { return dtype == KEEP_E4M3 ? 1 : dtype_si
 
 // ------------------------------------------------------------------ few rows
 
-constexpr int LINEAR_FEW = 16;  // rows of the kernel below
+// Rows of the kernel below. Against tiles of 64 x 64 through LDS, microseconds of bf16 in a graph, one row / 16 rows: 4096 -> 384
+// 7.1 / 9.9 against 8.6 / 9.5, 4096 -> 4096 7.7 / 10.4 against 11.2 / 12.6, 4096 -> 8192 13.6 / 17.6 against 16.9 / 16.9,
+// 512 -> 65536 14.1 / 18.1 against 16.6 / 17.2; 17 rows of 4096 -> 4096 take 12.6 there.
+constexpr int LINEAR_FEW = 16;
 
-// WAVES waves share 16 rows of W (and of x): wave s takes the s-th share of the summed index and the shares are added in order
-// through LDS. Lane (c, q) holds W row n0 + c, so that its results are outputs n0 + 4 q + v of row c.
-template <typename T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinearGemmArgs a) {
+// Eight waves share 16 rows of W (and the rows of x): wave s takes the s-th share of the summed index and the shares are added
+// in order through LDS. Lane (c, q) holds W row n0 + c, so that its results are outputs n0 + 4 q + v of row c. The loads of UN
+// steps are in flight at a time. 4096 -> 4096 bf16, one row: 7.7 us, 4.4 TB/s of W; what is left of a call of one strip a CU
+// (4096 -> 384: 7.1) is launch and the loads' latency. Sixteen waves: 7.7 and 7.1, but 512 -> 65536 22 us for 14; four or eight
+// rows of W a block where there are few strips: 7.4 for 7.1.
+template <typename T>
+__global__ __launch_bounds__(512) void k_linear_few(LinearGemmArgs a) {
+  constexpr int WAVES = 8;
   constexpr int SZ = sizeof(T), LB = SZ == 1 ? 32 : 16;  // bytes of a lane's piece
   constexpr int VL = LB / SZ, KS = 4 * VL, UN = SZ == 1 ? 4 : 8;
   __shared__ float4 red[WAVES][64];
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int64_t n0 = (int64_t)blockIdx.x * 16, j0 = (int64_t)blockIdx.y * 16;
-  const char* xrow = (const char*)a.pj + min(j0 + c, a.nj - 1) * a.ldj * SZ + q * LB;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const char* xrow = (const char*)a.pj + min((int64_t)c, a.nj - 1) * a.ldj * SZ + q * LB;
   const char* wrow = (const char*)a.pi + min(n0 + c, a.ni - 1) * a.ldi * SZ + q * LB;
   const int64_t kb = (a.nk + KS - 1) / KS;  // (8-bit: a scale's span each)
-  const float* xs = SZ == 1 ? a.sj + min(j0 + c, a.nj - 1) * kb : nullptr;
+  const float* xs = SZ == 1 ? a.sj + min((int64_t)c, a.nj - 1) * kb : nullptr;
   const float* ws = SZ == 1 ? a.si + n0 / 128 * kb : nullptr;
   const int steps = (int)kb, per = (steps + WAVES - 1) / WAVES;
   const int s0 = min(steps, wv * per), s1 = min(steps, s0 + per), whole = min(s1, (int)(a.nk / KS));
@@ -103,16 +110,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_linear_few(LinearGemmArgs a) {
     f[0] += p.x; f[1] += p.y; f[2] += p.z; f[3] += p.w;
   }
   const int64_t n = n0 + q * 4;
-  if (j0 + c >= a.nj || n >= a.ni) return;
+  if (c >= a.nj || n >= a.ni) return;
   a.e.load_bias<4>(n, a.ni - n, b);
-  a.e.store<4>(j0 + c, a.ni, n, a.ni - n, f, b);
+  a.e.store<4>(c, a.ni, n, a.ni - n, f, b);
 }
 
 template <typename T>
 static void linear_few_launch(const LinearGemmArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((a.ni + 15) / 16), (unsigned)((a.nj + 15) / 16));
-  if (grid.x * grid.y <= 256) hipLaunchKernelGGL((k_linear_few<T, 16>), grid, dim3(1024), 0, s, a);
-  else hipLaunchKernelGGL((k_linear_few<T, 8>), grid, dim3(512), 0, s, a);
+  hipLaunchKernelGGL(k_linear_few<T>, dim3((unsigned)((a.ni + 15) / 16)), dim3(512), 0, s, a);
 }
 
 static void linear_few(const LinearGemmArgs& a, int dtype, hipStream_t s) {

@@ -133,7 +133,11 @@ __device__ __forceinline__ float norm_sum(float v, float* red) {
   return v;
 }
 
-// f(TPR, NV, END) for rows of n values.
+// f(TPR, NV, END) for rows of n values: as many threads as a row has vectors, up to 512. Few rows wait for one row, which more
+// threads shorten, many rows for HBM. bf16 with a residual, 16 rows / 8192 rows, microseconds: 2048 values by 256 threads 3.5 /
+// 22.9, by 64 with four vectors 4.8 / 22.6; 4096 by 512 3.6 / 40.7, by 256 4.1 / 40.0; 7168 by 512 4.4 / 84.7, by 256 5.0 / 86.5,
+// by 1024 4.0 and the 8-bit form of 4096 rows 40.6 for 38.2. Where a wave holds a row no block waits: 1024 by 64 3.9 / 11.9, by
+// 256 3.6 / 14.4.
 template <typename F>
 void norm_by_width(int64_t n, F f) {
   using std::integral_constant;
@@ -146,9 +150,9 @@ void norm_by_width(int64_t n, F f) {
   const auto by = [&](auto end) {
     if (n <= 512) f(t64, v1, end);
     else if (n <= 1024) f(t64, v2, end);
-    else if (n <= 2048) f(t64, v4, end);
-    else if (n <= 4096) f(t256, v2, end);
-    else if (n <= 8192) f(t256, v4, end);
+    else if (n <= 2048) f(t256, v1, end);
+    else if (n <= 4096) f(t512, v1, end);
+    else if (n <= 8192) f(t512, v2, end);
     else f(t512, v4, end);
   };
   if (n < 8) f(t64, v1, integral_constant<int, NORM_TINY>{});
