@@ -14,8 +14,8 @@
 //
 // Bound by HBM: every value is read once, kept in registers as fp32 over the row's sum, and written once. bf16 with a
 // residual, 8192 rows of 4096: 40.4 us, 6.6 TB/s; of 2048 22.1; 65536 of 512 without one 23.9 (5.6 TB/s); 4096 of 7168 37.4,
-// in 8 bits 38.2; float32 4096 of 4096 42.8 (6.3 TB/s). One row of 7168: 3.5 us in a graph, a launch and the loads' way. The 8-bit rows
-// multiply by the scale's reciprocal: with a division a value 2048 rows of 4096 took 19.5 us, now 13.5.
+// in 8 bits 38.2; float32 4096 of 4096 42.8 (6.3 TB/s). One row of 7168: 3.5 us in a graph, a launch and the loads'
+// way. The 8-bit rows multiply by the scale's reciprocal: with a division a value 2048 rows of 4096 took 19.5 us, now 13.5.
 #include "norm_dev.h"
 
 namespace keep {

@@ -31,12 +31,8 @@ struct NormRaw {
   uint32_t w[2 * sizeof(T)];
   template <int END>
   __device__ __forceinline__ void load(const T* row, int i, int n) {
-    if constexpr (END == NORM_ODD) {
-      __builtin_memcpy(w, row + min(i, n - 8), 8 * sizeof(T));
-      return;
-    }
-    if (END == NORM_EVEN && i < n) {
-      __builtin_memcpy(w, row + i, 8 * sizeof(T));
+    if (END != NORM_TINY && i < n) {
+      __builtin_memcpy(w, row + (END == NORM_ODD ? min(i, n - 8) : i), 8 * sizeof(T));
     } else {
 #pragma unroll
       for (int u = 0; u < (int)(2 * sizeof(T)); ++u) w[u] = 0u;
