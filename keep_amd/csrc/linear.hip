@@ -152,22 +152,33 @@ struct LinearPlan {
   int64_t tiles;
 };
 
-// The tile and the slices of a product: the largest tile that still gives the CUs about one each. Microseconds of bf16, one
-// launch, tiles of 256 x 256 / 256 x 128 / 128 x 128: 8192 x 4096 -> 8192 454 / 520 / 590; 4096 x 4096 -> 2048 (128, 256
-// and 512 tiles) 106 / 73 / 87. Of fp16, 128 x 128 by one group of waves / by two / 64 x 64 by two: 600 x 4096 -> 2048 (80
-// and 320 tiles) 43 / 32 / 24, 333 x 2880 -> 1440 (36, 138) 31 / 24 / 11.
-// Slices take a second launch, 5 us: they pay where a group of waves would walk more than 24 steps and CUs have no work (64 x 64
-// tiles, one slice against four: 200 x 7168 -> 2048 35 / 14, 64 x 4096 -> 4096 22 / 9, 333 x 2880 -> 1440 11.2 / 11.4).
+// The tile and the slices of a product. Microseconds of bf16 in a graph:
+// - The largest tile that still gives the CUs about one each. Tiles of 256 x 256 / 256 x 128 / 128 x 128: 8192 x 4096 -> 8192
+//   454 / 520 / 590; 4096 x 4096 -> 2048 (128, 256 and 512 tiles) 106 / 73 / 87. 128 x 128 by two groups of waves / 64 x 64:
+//   1024 x 4096 -> 4096 (256 and 1024 tiles) 39 / 54, 4096 x 2048 -> 768 (192, 768) 22.3 / 26.3, 1024 x 4096 -> 2048 (128, 512)
+//   35 / 28, fp16 333 x 2880 -> 1440 (36, 138) 24 / 11. One group for two: 600 x 4096 -> 2048 43 / 32.
+// - float32's products take sixteen times as long, so that its tiles go by the rounds of 256 CUs, four and a half of 64 x 64
+//   for one of 128 x 128: 1024 x 4096 -> 2048 (128 and 512 tiles) 241 / 133, 1024 x 2880 -> 1440 and
+//   its dW (96 and 276, 368 and 1035) 225 / 174.
+// - Slices take a second launch, 4 us: they pay where the sum is long and CUs have no work. 64 x 64 tiles, one slice / more:
+//   512 x 4096 -> 2048 (256 tiles) 23.5 / 21.2 (two), 64 x 2880 -> 1440 (23) 11.7 / 9.9 (three), 384 x 2880 -> 1440 (138)
+//   12.3 / 15.6 (two), 64 x 2048 -> 768 (12) 9.4 / 9.5 (two). Two, four and eight of 128 x 4096 -> 2048 (64 tiles, 64 steps)
+//   13.5, 12.8 and 15.8; of 256 x 4096 -> 2048 in float32 (128, 128 steps) two 42, three 50, four 40. 128 x 128 tiles in two
+//   slices against 64 x 64: 1024 x 7168 -> 2048 42 / 46, of 4096 inputs 30 / 28.
 static LinearPlan linear_plan(int dtype, int mode, int64_t ni, int64_t nj, int64_t nk) {
   const auto tiles = [&](int64_t bi, int64_t bj) { return ((ni + bi - 1) / bi) * ((nj + bj - 1) / bj); };
   if (mode == LINEAR_FORWARD && nj <= LINEAR_FEW) return {LINEAR_TILE_FEW, 1, tiles(16, 16)};
   const bool small = dtype == KEEP_F32;
   if (!small && dtype != KEEP_E4M3 && tiles(256, 256) >= 224) return {LINEAR_TILE_256, 1, tiles(256, 256)};
   if (!small && tiles(256, 128) >= 192) return {LINEAR_TILE_256_128, 1, tiles(256, 128)};
-  const int64_t n = tiles(128, 128);
-  if (nj > 64 && ni > 64 && n >= 128) return {n <= 256 ? LINEAR_TILE_128_2 : LINEAR_TILE_128, 1, n};
-  const int64_t m = tiles(64, 64), steps = (nk * linear_size(dtype) + 127) / 128;
-  const int64_t slices = steps <= 48 ? 1 : std::max<int64_t>(1, std::min<int64_t>({512 / m, steps / 8, 32}));
+  const int64_t n = tiles(128, 128), m = tiles(64, 64), rn = (n + 255) / 256, rm = (m + 255) / 256;
+  const int64_t steps = (nk * std::max<int64_t>(linear_size(dtype), 2) + 127) / 128;  // (8-bit values are 16-bit ones' work)
+  if (nj > 64 && ni > 64) {
+    if (small ? 32 * rn <= 9 * rm : n >= 160) return {n <= 256 ? LINEAR_TILE_128_2 : LINEAR_TILE_128, 1, n};
+    if (!small && n >= 96 && n <= 128 && steps >= 96) return {LINEAR_TILE_128_2, 2, n};
+  }
+  const int64_t room = (small || steps <= 48 ? 256 : 512) / m;
+  const int64_t slices = steps < 40 ? 1 : std::max<int64_t>(1, std::min<int64_t>({room, steps / 14, 32}));
   return {LINEAR_TILE_64, (int)slices, m};
 }
 

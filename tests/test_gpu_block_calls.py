@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 import keep_amd
-from tests import test_gpu_norm
+from tests import test_gpu_norm, test_gpu_projection
 from tests.bounded import Bounded
 from tests.test_gpu_projection import _q8
 
@@ -217,3 +217,15 @@ def test_row_ends(dev, n, dtype, res, wdt):
     each = s.double().repeat_interleave(16, 1)[:, :n]
     bound = y.e + (y.v.abs() + y.e) * 2.0 ** -4 + each * 2.0 ** -10 + y.v.abs() * 2.0 ** -23
     assert ((q.double() * each - y.v).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("M, N, K, dtype", [(1000, 1900, 6200, BF16), (1000, 2300, 328, F16), (1000, 2300, 300, F32),
+                                            (70, 1500, 2900, F16), (600, 400, 4100, F32), (260, 2050, 4096, BF16)])
+def test_tiles_and_slices_between_the_large_and_the_small(dev, M, N, K, dtype):
+    test_gpu_projection._check(test_gpu_projection._case(dev, dtype, M, N, K, bias=F32), "silu")
+
+
+@pytest.mark.parametrize("M, N, K", [(1000, 1900, 6208), (300, 2050, 2064), (64, 2048, 4096)])
+def test_q8_tiles_and_slices(dev, M, N, K):
+    x, xs, w, ws = _q8(dev, M, N, K)
+    test_gpu_projection._q8_expected(x, xs, w, ws).round(BF16).check(keep_amd.linear_q8(x, xs, w, ws))
