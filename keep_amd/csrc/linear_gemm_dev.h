@@ -58,7 +58,9 @@ __global__ __launch_bounds__(64 * WI * WJ * G) void k_linear_gemm(LinearGemmArgs
   constexpr bool TRI = MODE != LINEAR_FORWARD, TRJ = MODE == LINEAR_WEIGHT;
   constexpr bool Q8 = sizeof(T) == 1;
   static_assert(!Q8 || MODE == LINEAR_FORWARD, "8-bit values have no gradient");
-  __shared__ __attribute__((aligned(16))) char smem_all[G * 2 * (SI + SJ)];
+  constexpr int FP = FJ > 4 ? 4 : FJ, ROWS = WJ * FP * 16, PITCH = BI + 4, CG = BI / 8;
+  constexpr int LDS = G * 2 * (SI + SJ) > G * ROWS * PITCH * 4 ? G * 2 * (SI + SJ) : G * ROWS * PITCH * 4;
+  __shared__ __attribute__((aligned(16))) char smem_all[LDS];
   const int gr = G > 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / NT) : 0;  // group
   char* smem = smem_all + gr * (2 * (SI + SJ));
   const int tid = threadIdx.x - gr * NT, lane = tid & 63, c = lane & 15, q = lane >> 4;
@@ -272,9 +274,9 @@ __global__ __launch_bounds__(64 * WI * WJ * G) void k_linear_gemm(LinearGemmArgs
   }
 
   // ---- results, through LDS: a lane's columns of a row are few and its rows many, a thread of the epilogue takes eight
-  // neighbouring columns, so that a row's pieces lie together in memory. FP fragments of every wave at a time.
-  constexpr int FP = FJ > 1 ? 2 : 1, ROWS = WJ * FP * 16, PITCH = BI + 4, CG = BI / 8;
-  static_assert(FJ % FP == 0 && ROWS * PITCH * 4 <= 2 * (SI + SJ) && NT % CG == 0, "LDS");
+  // neighbouring columns, so that a row's pieces lie together in memory. FP fragments of every wave at a time: four of the largest tile's
+  // eight (8192 x 128 -> 8192 bf16 65 us, by two 70; 8192 x 4096 -> 8192 407, 417), two where there are four (of four 1 % slower).
+  static_assert(FJ % FP == 0 && NT % CG == 0, "LDS");
   float* tile = (float*)smem_all + gr * (ROWS * PITCH);
   const int64_t col = i0 + (tid % CG) * 8;
   float b[8];
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(64 * WI * WJ * G) void k_linear_gemm(LinearGemmArgs
     }
     __syncthreads();
     if (col >= a.ni) continue;
-#pragma unroll 2
+#pragma unroll 4
     for (int r = threadIdx.x / CG; r < ROWS; r += G * NT / CG) {
       const int64_t row = j0 + (r / (FP * 16)) * TJ + p * (FP * 16) + r % (FP * 16);
       if (row >= a.nj) continue;
