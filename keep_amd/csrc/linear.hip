@@ -211,6 +211,8 @@ struct LinearDuArgs {
   int64_t M, N, ld;  // ld: of du, whole 16-byte pieces, zeros behind the columns
   void* du;          // or null
   float* part;       // [gridDim.y][N] sums of du, or null
+  void* db;          // one block of rows: their sum at once, in part's place
+  int bdt;
   int64_t rows;      // of a block
 };
 
@@ -242,7 +244,7 @@ __global__ __launch_bounds__(256) void k_linear_du(LinearDuArgs a) {
       }
     }
   }
-  if (!a.part) return;
+  if (!a.part && !a.db) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) red[rg][cg][i] = sum[i];
   __syncthreads();
@@ -252,7 +254,10 @@ __global__ __launch_bounds__(256) void k_linear_du(LinearDuArgs a) {
   float v = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) v += red[k][threadIdx.x >> 3][threadIdx.x & 7];
-  a.part[blockIdx.y * a.N + n] = v;
+  if (a.part) a.part[blockIdx.y * a.N + n] = v;
+  else if (a.bdt == KEEP_F32) ((float*)a.db)[n] = v;
+  else if (a.bdt == KEEP_BF16) ((bf16s*)a.db)[n] = from_float<bf16s>(v);
+  else ((_Float16*)a.db)[n] = from_float<_Float16>(v);
 }
 
 constexpr int64_t LINEAR_MAX = int64_t(1) << 20;  // N and K: a tile's rows then lie within 32-bit offsets
@@ -405,14 +410,16 @@ extern "C" int keep_linear_grad(const void* dy, const void* u, int act, const vo
     LinearDuArgs d{};
     d.dy = dy; d.u = u; d.act = act; d.M = M; d.N = N; d.ld = linear_pitch(N, size);
     d.du = products && !same ? ws + p.du : nullptr;
-    d.part = dbias ? (float*)(ws + p.db) : nullptr;
     const int64_t blocks = linear_du_blocks(M, N);
+    d.part = dbias && blocks > 1 ? (float*)(ws + p.db) : nullptr;
+    d.db = blocks > 1 ? nullptr : dbias;
+    d.bdt = bias_dtype;
     d.rows = (M + blocks - 1) / blocks;
     const dim3 grid((unsigned)((N + 255) / 256), (unsigned)blocks);
     if (dtype == KEEP_F32) hipLaunchKernelGGL(k_linear_du<float>, grid, dim3(256), 0, s, d);
     else if (dtype == KEEP_F16) hipLaunchKernelGGL(k_linear_du<_Float16>, grid, dim3(256), 0, s, d);
     else hipLaunchKernelGGL(k_linear_du<bf16s>, grid, dim3(256), 0, s, d);
-    if (dbias) parts_sum(d.part, blocks, N, dbias, bias_dtype, s);
+    if (d.part) parts_sum(d.part, blocks, N, dbias, bias_dtype, s);
   }
   LinearGemmArgs a{};
   a.e.odt = dtype;
