@@ -670,7 +670,8 @@ int keep_route_experts_grad(const void* logits, int dtype, int64_t T, int64_t E,
 
 /* Dense projection with its epilogue: u = x weight^T + bias, out = round(residual + act(u)). x [M, K] and weight [N, K] of one
  * dtype, their rows x_ld and w_ld values apart (whole 16-byte pieces; x and weight 16-byte aligned). Where K is no whole
- * number of pieces, what lies between a row's K values and the next piece enters the sums: zeros. bias [N], residual [M, N]
+ * number of pieces, what lies between a row's K values and the next piece enters the sums: zeros. Up to 16 rows: any pitch
+ * from K on and pointers aligned to their dtype, of which the K values alone are read. bias [N], residual [M, N]
  * and out [M, N] of any float dtype, dense; bias and residual may be NULL. u [M, N] (x's dtype) receives the values before the
  * activation, or NULL. fp32 sums in a fixed order. N, K <= 2^20. The workspace holds keep_linear_workspace_bytes (may be 0),
  * 16-byte aligned. */

@@ -36,12 +36,51 @@ static int64_t linear_size(int dtype) { return dtype == KEEP_E4M3 ? 1 : dtype_si
 // 512 -> 65536 14.1 / 18.1 against 16.6 / 17.2; 17 rows of 4096 -> 4096 take 12.6 there.
 constexpr int LINEAR_FEW = 16;
 
+// 16 bytes at any address of a value.
+__device__ __forceinline__ uint4 linear_ld16_any(const char* p) {
+  typedef unsigned int v4u __attribute__((ext_vector_type(4), aligned(2)));
+  const v4u v = *(const __attribute__((address_space(1))) v4u*)p;
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// The piece at value k of a row of n values that starts at row, zeros past its end: read whole from before the end and moved
+// down where the row ends inside it.
+template <typename T>
+__device__ __forceinline__ uint4 linear_piece_any(const char* row, int64_t k, int64_t n) {
+  constexpr int SZ = sizeof(T), V = 16 / SZ;
+  uint32_t m[4] = {0u, 0u, 0u, 0u};
+  if (k + V <= n) return linear_ld16_any(row + k * SZ);
+  if (k < n && n >= V) {
+    const uint4 r = linear_ld16_any(row + (n - V) * SZ);
+    m[0] = r.x; m[1] = r.y; m[2] = r.z; m[3] = r.w;
+    const int down = (int)(k + V - n) * SZ;  // bytes
+#pragma unroll
+    for (int s = 2; s > 0; --s)
+      if (down & 4 * s)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) m[u] = u + s < 4 ? m[u + s < 4 ? u + s : 0] : 0u;
+    if (down & 2)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) m[u] = m[u] >> 16 | (u < 3 ? m[u < 3 ? u + 1 : 0] << 16 : 0u);
+  } else if (k < n) {  // (k = 0)
+#pragma unroll
+    for (int u = 0; u < V - 1; ++u)
+      if (u < n) {
+        if constexpr (SZ == 4) m[u] = ((const uint32_t*)row)[u];
+        else m[u / 2] |= (uint32_t)((const uint16_t*)row)[u] << (16 * (u & 1));
+      }
+  }
+  return make_uint4(m[0], m[1], m[2], m[3]);
+}
+
 // Eight waves share 16 rows of W (and the rows of x): wave s takes the s-th share of the summed index and the shares are added
 // in order through LDS. Lane (c, q) holds W row n0 + c, so that its results are outputs n0 + 4 q + v of row c. The loads of UN
 // steps are in flight at a time. 4096 -> 4096 bf16, one row: 7.7 us, 4.4 TB/s of W; what is left of a call of one strip a CU
 // (4096 -> 384: 7.1) is launch and the loads' latency. Sixteen waves: 7.7 and 7.1, but 512 -> 65536 22 us for 14; four or eight
 // rows of W a block where there are few strips: 7.4 for 7.1.
-template <typename T>
+// ANY: rows at any address and of any length (1 x 3925 -> 3510 bf16 14.1 us, of 3924 values
+// 7.4; copied into whole pieces first 27).
+template <typename T, bool ANY>
 __global__ __launch_bounds__(512) void k_linear_few(LinearGemmArgs a) {
   constexpr int WAVES = 8;
   constexpr int SZ = sizeof(T), LB = SZ == 1 ? 32 : 16;  // bytes of a lane's piece
@@ -52,6 +91,10 @@ __global__ __launch_bounds__(512) void k_linear_few(LinearGemmArgs a) {
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const char* xrow = (const char*)a.pj + min((int64_t)c, a.nj - 1) * a.ldj * SZ + q * LB;
   const char* wrow = (const char*)a.pi + min(n0 + c, a.ni - 1) * a.ldi * SZ + q * LB;
+  const auto ld = [](const char* row, int at) {
+    if constexpr (ANY) return linear_ld16_any(row + at);
+    else return dense_ld16((const uint8_t*)row, at);
+  };
   const int64_t kb = (a.nk + KS - 1) / KS;  // (8-bit: a scale's span each)
   const float* xs = SZ == 1 ? a.sj + min((int64_t)c, a.nj - 1) * kb : nullptr;
   const float* ws = SZ == 1 ? a.si + n0 / 128 * kb : nullptr;
@@ -81,8 +124,8 @@ __global__ __launch_bounds__(512) void k_linear_few(LinearGemmArgs a) {
     for (int d = 0; d < UN; ++d) {
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        fi[d][p] = dense_ld16((const uint8_t*)wrow, (s + d) * (KS * SZ) + p * 16);
-        fj[d][p] = dense_ld16((const uint8_t*)xrow, (s + d) * (KS * SZ) + p * 16);
+        fi[d][p] = ld(wrow, (s + d) * (KS * SZ) + p * 16);
+        fj[d][p] = ld(xrow, (s + d) * (KS * SZ) + p * 16);
       }
       sc[d] = SZ == 1 ? xs[s + d] * ws[s + d] : 1.f;
     }
@@ -93,6 +136,12 @@ __global__ __launch_bounds__(512) void k_linear_few(LinearGemmArgs a) {
     uint4 fi[P], fj[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
+      if constexpr (ANY) {
+        const int64_t k = (int64_t)s * KS + q * VL;
+        fi[p] = linear_piece_any<T>(wrow - q * LB, k, a.nk);
+        fj[p] = linear_piece_any<T>(xrow - q * LB, k, a.nk);
+        continue;
+      }
       const bool in = (int64_t)s * KS + (q * LB + p * 16) / SZ < a.nk;  // (pieces are whole or past the end)
       const int64_t at = (int64_t)s * (KS * SZ) + p * 16;
       fi[p] = in ? dense_ld16((const uint8_t*)wrow, at) : make_uint4(0u, 0u, 0u, 0u);
@@ -117,7 +166,14 @@ __global__ __launch_bounds__(512) void k_linear_few(LinearGemmArgs a) {
 
 template <typename T>
 static void linear_few_launch(const LinearGemmArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(k_linear_few<T>, dim3((unsigned)((a.ni + 15) / 16)), dim3(512), 0, s, a);
+  const dim3 grid((unsigned)((a.ni + 15) / 16));
+  if constexpr (sizeof(T) > 1) {
+    if (a.any) {
+      hipLaunchKernelGGL((k_linear_few<T, true>), grid, dim3(512), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((k_linear_few<T, false>), grid, dim3(512), 0, s, a);
 }
 
 static void linear_few(const LinearGemmArgs& a, int dtype, hipStream_t s) {
@@ -347,9 +403,17 @@ extern "C" int keep_linear(const void* x, int64_t x_ld, int dtype, int64_t M, co
   KEEP_REQUIRE(dtype_ok(dtype), "bad dtype enum");
   if (M == 0) return KEEP_OK;
   KEEP_REQUIRE(x && weight && out, "null pointer argument");
-  KEEP_REQUIRE_PITCH(x, x_ld, K, linear_size(dtype), "x");
-  KEEP_REQUIRE_PITCH(weight, w_ld, K, linear_size(dtype), "weight");
   LinearGemmArgs a{};
+  const int64_t size = linear_size(dtype);
+  if (M <= LINEAR_FEW) {
+    KEEP_REQUIRE(aligned(x, size) && aligned(weight, size) && x_ld >= K && w_ld >= K && x_ld <= 4 * LINEAR_MAX &&
+                     w_ld <= 4 * LINEAR_MAX,
+                 "x and weight must be aligned to their dtype, their pitch at least a row");
+    a.any = !aligned(x, 16) || !aligned(weight, 16) || (x_ld | w_ld | K) * size % 16 != 0;
+  } else {
+    KEEP_REQUIRE_PITCH(x, x_ld, K, size, "x");
+    KEEP_REQUIRE_PITCH(weight, w_ld, K, size, "weight");
+  }
   a.pi = weight; a.pj = x; a.ldi = w_ld; a.ldj = x_ld; a.ni = N; a.nj = M; a.nk = K;
   if (const int rc = linear_epilogue(a.e, M, N, bias, bias_dtype, act, residual, residual_dtype, u, dtype, out, out_dtype))
     return rc;

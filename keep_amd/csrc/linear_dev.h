@@ -208,6 +208,7 @@ struct LinearGemmArgs {
   int64_t ni, nj, nk;
   int slices;       // of the summed index; more than one: sums go to part
   float* part;      // [slices][nj][ni]
+  int any;          // few rows: rows at any address, and any number of values
   const float *si, *sj;  // 8-bit: scales [ceil(ni / 128)][ceil(nk / 128)] and [nj][ceil(nk / 128)]
   LinearEpilogue e;
 };

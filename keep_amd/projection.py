@@ -3,8 +3,8 @@
 ``linear`` takes rows and weights of one float dtype (the router's own product, a shared expert's, a biased projection);
 ``linear_q8`` takes both in 8 bits (e4m3) with float32 scales, as ``rmsnorm_quant`` leaves its rows, for serving. Sums are
 float32 and rounded once. Up to 16 rows stream the weights, more run through LDS, in slices of the summed index where there
-are few tiles (``keep_linear``). Rows and weights may be views with a pitch; where rows are no whole number of 16-byte
-pieces, or start off one, they are copied first.
+are few tiles (``keep_linear``). Rows and weights may be views with a pitch; where more than 16 rows are no whole number of
+16-byte pieces, or start off one, they and the weights are copied first.
 """
 
 from __future__ import annotations
@@ -17,6 +17,7 @@ from keep_amd import _grad, _lib, ops
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 SCALE_BLOCK = 128  # values of a row, and rows of the weight, that share a scale of the 8-bit form
 MAX_DIMS = 1 << 20
+_FEW = 16  # rows up to which the kernels read rows of any address and length
 _E4M3 = 3
 
 
@@ -38,6 +39,15 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     if ld > K:
         out[:, K:].zero_()
     return out[:, :K], ld
+
+
+def _few_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``_rows`` of a call on few rows, which reads them as they lie where their values are neighbours."""
+
+    n, K = t.shape
+    if t.stride(1) == 1 and (n <= 1 or K <= t.stride(0) <= 4 * MAX_DIMS):
+        return t, K if n <= 1 else t.stride(0)
+    return t.contiguous(), K
 
 
 def _launch(x, weight, bias, act: int, residual, out_dtype, keep_u: bool):
@@ -153,7 +163,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         b = None if bias is None else bias.contiguous()
         r = None if residual is None else (residual if flat else residual.reshape(-1, shape[-1])).contiguous()
         if not _grad.wanted(x, weight, bias, residual):
-            out = _launch(_rows(rows), _rows(weight), b, act, r, od, False)[0]
+            lie = _few_rows if rows.shape[0] <= _FEW else _rows
+            out = _launch(lie(rows), lie(weight), b, act, r, od, False)[0]
         else:
             _grad.check_capture(x, weight, bias, residual)
             out = _grad.mark(_Linear.apply(rows, weight, b, r, act, od))

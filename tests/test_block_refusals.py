@@ -242,3 +242,8 @@ def test_layers_refuse():
         keep_amd.RoutedVQMoE(glu, top_k=2, gate=keep_amd.MoEGate(torch.zeros(4, 16), top_k=2), slot_map=torch.zeros(4))
     with pytest.raises(ValueError, match="needs logits"):
         keep_amd.RoutedVQMoE(glu, top_k=2)(torch.zeros(2, 16))
+
+
+@pytest.mark.parametrize("over", [dict(x=17), dict(w=17), dict(x_ld=63), dict(w_ld=63), dict(w_ld=1 << 23)])
+def test_few_rows_of_any_pitch_are_refused_by_their_dtype(over):
+    _refused("keep_linear", LINEAR, dict(M=16, **over), "x and weight must be")

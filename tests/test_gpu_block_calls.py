@@ -229,3 +229,22 @@ def test_tiles_and_slices_between_the_large_and_the_small(dev, M, N, K, dtype):
 def test_q8_tiles_and_slices(dev, M, N, K):
     x, xs, w, ws = _q8(dev, M, N, K)
     test_gpu_projection._q8_expected(x, xs, w, ws).round(BF16).check(keep_amd.linear_q8(x, xs, w, ws))
+
+
+@pytest.mark.parametrize("M", [1, 3, 16])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("K", [1, 2, 3, 5, 7, 8, 9, 31, 33, 70, 255, 257, 1029, 3925])
+def test_few_rows_at_any_address(dev, M, dtype, K):
+    """Rows of any length and start, with NaN around them: the sums of a copy."""
+    c = test_gpu_projection._case(dev, dtype, M, 37, K, bias=F32)
+    want = test_gpu_projection._expected(c, None, dtype, grads=False)[0]
+    want.check(keep_amd.linear(c["x"], c["w"], c["b"]))
+
+    def inside(t, left, right):
+        big = torch.full((t.shape[0], left + t.shape[1] + right), float("nan"), device=dev, dtype=t.dtype)
+        big[:, left:left + t.shape[1]] = t
+        return big[:, left:left + t.shape[1]]
+    for left, right in ((0, 1), (1, 0), (3, 2), (8, 8)):
+        got = keep_amd.linear(inside(c["x"], left, right), inside(c["w"], right, left), c["b"])
+        want.check(got)
+    want.check(keep_amd.linear(c["x"].t().contiguous().t(), c["w"].t().contiguous().t(), c["b"]))
