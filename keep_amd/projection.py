@@ -192,7 +192,8 @@ def linear_q8(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, wei
     if _grad.wanted(x_scales, weight_scales, bias, residual):
         raise ValueError("the 8-bit product has no gradients")
     with ops._on(device):
-        (xr, x_ld), (wr, w_ld) = _rows(x.reshape(-1, K)), _rows(weight)
+        flat = x.ndim == 2
+        (xr, x_ld), (wr, w_ld) = _rows(x if flat else x.reshape(-1, K)), _rows(weight)
         M = xr.shape[0]
         out = torch.empty((M, N), dtype=od, device=device)
         if M == 0:
@@ -206,4 +207,4 @@ def linear_q8(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, wei
                   ops._ptr(b), 0 if b is None else ops._DT[b.dtype], act, ops._ptr(r),
                   0 if r is None else ops._DT[r.dtype], out.data_ptr(), ops._DT[od], ops._ptr(work), need,
                   ops._stream(device))
-        return out.view(shape)
+        return out if flat else out.view(shape)
