@@ -10,16 +10,18 @@
 // The lower index comes first among equal keys, NaN ranks as -inf, and a choice does not depend on how fp32 rounds. Without
 // a bias the scores order as the logits do, and the logits are what is compared. With one (and for the groups' values) keys
 // are formed in fp32, and where two that decide the outcome lie closer than fp32 is sure of, the token is chosen again with
-// keys in 64 bits. Equal logits under equal biases are equal without a second look.
+// keys in 64 bits. Equal logits under equal biases are equal without a second look; where such a pair is the last winner and the
+// first that is not chosen, every key behind them that comes as close has to be their equal too.
 //
 // The groups are spread over the lanes: LG lanes share a group (the largest power of two with LG groups <= 64), so that a
 // group's two largest are found inside its lanes.
 //
 // Bound by what a wave issues one after another: 8192 tokens read 8.9 MB in all (1.7 us of HBM), and take 8.7 us (256 experts, 8
-// of them, sigmoid), of which 2.8 are the rounds of the selection, 10.8 with a bias or with 8 groups of which 4 are kept, 14 to 15
-// with both (sqrt(softplus) 14.3); 4096 of 384 softmax 6.8, with loads 10.4; one token 4.1 to 4.5. A round is one maximum of
-// the wave by lane moves and scalar reads, no LDS: with a round that looked through all of a lane's keys again 8192 tokens took
-// 23. Keys in 64 bits throughout would double every move of the selection; so only the tokens that need them take them.
+// of them, sigmoid), of which 2.8 are the rounds of the selection, 12.5 with a bias (one for all and 16-bit logits, whose
+// boundaries cut runs of equals: 11.1, and 10.4 without the look behind them), 14 to 15.5 with 8 groups too, of which 4 are kept
+// (sqrt(softplus) without either 14.3); 4096 of 384 softmax 6.8, with loads 10.4; one token 4.1 to 4.5. A round is one maximum
+// of the wave by lane moves and scalar reads, no LDS: with a round that looked through all of a lane's keys again 8192 tokens
+// took 23. Keys in 64 bits throughout would double every move of the selection; so only the tokens that need them take them.
 //
 // With c = scale / (sum s_i + 1e-20) and p_j = c (g_j - sum g_i s_i / (sum s_i + 1e-20)), the gradient of s_j
 // (not renormalised: p_j = scale g_j):
@@ -353,7 +355,17 @@ __global__ __launch_bounds__(256) void k_route_experts(ChooseArgs a) {
       const float zw = have ? to_float(row[mine]) : 0.f, bw = have ? a.bias[mine] : 0.f;
       const float zn = __shfl_down(zw, 1, 64), bn = __shfl_down(bw, 1, 64);
       const bool next = __shfl_down((int)have, 1, 64) != 0;
-      sure = sure && __all(!(close >> lane & 1) || !next || (zw == zn && bw == bn));
+      bool same = !(close >> lane & 1) || !next || (zw == zn && bw == bn);
+      if (close >> (a.k - 1) & 1) {  // the last winner's equal is left out: so must be all that come as close behind it
+        const float kl = ch_lane(kw, a.k - 1), zl = ch_lane(zw, a.k - 1), bl = ch_lane(bw, a.k - 1);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const float ki = key[i] ? rt_unsortable(key[i]) : -__builtin_inff();
+          if (key[i] && !(kl - ki > unsure + 0x1p-23f * (fabsf(kl) + fabsf(ki))))
+            same = same && to_float(row[at[i]]) == zl && a.bias[at[i]] == bl;
+        }
+      }
+      sure = sure && __all(same);
     }
   }
   if (!sure) mine = ch_exact<Z, PER>(a, l, t, lane);
