@@ -440,7 +440,7 @@ __global__ __launch_bounds__(256) void k_route_experts_grad(ChooseGradArgs a) {
   if (a.func == KEEP_SCORE_SOFTMAX) {
     dot = rt_wave_reduce(chosen ? p * se : 0.f, false);
   } else if (a.func == KEEP_SCORE_SIGMOID) {
-    p *= 1.f - se;  // (times the score below)
+    p *= score.of(-ze, KEEP_SCORE_SIGMOID);  // 1 - s with its bits where s rounds to 1 (times the score below)
   } else {
     // sigmoid(z) / (2 s) over s; where both vanish, s^2 -> e^z and the slope is s / 2
     p *= se > 0.f ? 0.5f * score.of(ze, KEEP_SCORE_SIGMOID) / se / se : 0.f;
