@@ -47,12 +47,16 @@ template <int ACT>
 __device__ __forceinline__ float linear_slope(float u) {
   constexpr int act = ACT;
   if (act == LINEAR_RELU) return u > 0.f ? 1.f : u != u ? u : 0.f;
+  // (at their ends 1 and 0 without infinity times 0: u that is kept in 16 bits may have become infinite)
   if (act == LINEAR_SILU) {
+    if (fabsf(u) > 128.f) return u > 0.f ? 1.f : 0.f;
     const float p = linear_sigmoid(u);
     return p * (1.f + u * (1.f - p));
   }
-  if (act == LINEAR_GELU)
+  if (act == LINEAR_GELU) {
+    if (fabsf(u) > 16.f) return u > 0.f ? 1.f : 0.f;
     return 0.5f * erfcf(u * -0.7071067811865476f) + u * __expf(-0.5f * u * u) * 0.3989422804014327f;
+  }
   if (act == LINEAR_GELU_TANH) {
     if (fabsf(u) > 16.f) return u > 0.f ? 1.f : 0.f;  // (u^2 of the largest values would overflow)
     const float p = linear_sigmoid(2.f * GELU_C * (u + 0.044715f * u * u * u));
