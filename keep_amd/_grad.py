@@ -67,6 +67,13 @@ def mark(out: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def saved(ctx) -> list:
+    """The tensors that the forward pass saved, dense: a saved-tensor hook (offloading, compression) may give them back
+    with other strides than it took them."""
+
+    return [None if t is None else t.contiguous() for t in ctx.saved_tensors]
+
+
 class _Partial(torch.autograd.Function):
     @staticmethod
     def forward(ctx, out, x):

@@ -115,7 +115,7 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
+        h, weight, rstd = _grad.saved(ctx)
         nx, nr, nw = ctx.needs_input_grad[:3]
         if dy is None:  # h alone was used
             return dh if nx else None, dh if nr else None, torch.zeros_like(weight) if nw else None, None

@@ -127,6 +127,7 @@ class _GatherMM(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, rhs = ctx.saved_tensors
+        x, rhs = x.contiguous(), rhs.contiguous()  # a saved-tensor hook may give back other strides
         with ops._on(x.device):
             return (*_backward(x, weight, rhs, ctx.plan, ctx.k, dy.contiguous(), ctx.needs_input_grad), None, None)
 

@@ -58,7 +58,7 @@ class _GatherLora(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, a, b, scales, idx, t = ctx.saved_tensors
+        x, a, b, scales, idx, t = _grad.saved(ctx)
         nx, na, nb, nbase = ctx.needs_input_grad[:4]
         (n, rank, K), N, R, device = a.shape, b.shape[1], idx.numel(), x.device
         make = torch.empty_like if R else torch.zeros_like

@@ -676,7 +676,7 @@ class _RouteCombine(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        y, w = ctx.saved_tensors
+        y, w = _grad.saved(ctx)
         T, k, H = y.shape
         d = dout.contiguous()
         dy = torch.empty_like(y) if ctx.needs_input_grad[0] else None

@@ -21,24 +21,33 @@ _FEW = 16  # rows up to which the kernels read rows of any address and length
 _E4M3 = 3
 
 
-def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """``t [n, K]`` as the kernels read it, whole 16-byte pieces a row, and the values between two rows. Copied behind
-    zeros where it lies otherwise."""
+def _packed(t: torch.Tensor) -> torch.Tensor | None:
+    """``t [n, K]`` with its rows filled up with zeros to whole 16-byte pieces, or None where ``t`` lies as the kernels
+    read it: whole, aligned pieces a row."""
 
     n, K = t.shape
     piece = 16 // t.element_size()
     if K % piece == 0 and t.data_ptr() % 16 == 0 and t.stride(1) == 1:
         if n <= 1:
-            return t, K
+            return None
         ld = t.stride(0)
         if ld >= K and ld % piece == 0 and ld <= 4 * MAX_DIMS:
-            return t, ld
+            return None
     ld = (K + piece - 1) // piece * piece
     out = torch.empty((n, ld), dtype=t.dtype, device=t.device)
     out[:, :K] = t
     if ld > K:
         out[:, K:].zero_()
-    return out[:, :K], ld
+    return out
+
+
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t [n, K]`` as the kernels read it (``_packed``), and the values between two rows."""
+
+    out = _packed(t)
+    if out is not None:
+        return out, out.shape[1]
+    return t, t.shape[1] if t.shape[0] <= 1 else t.stride(0)
 
 
 def _few_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -50,11 +59,11 @@ def _few_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     return t.contiguous(), K
 
 
-def _launch(x, weight, bias, act: int, residual, out_dtype, keep_u: bool):
-    """``(out, u or None)`` for ``x [M, K]`` and ``weight [N, K]`` from ``_rows``."""
+def _launch(x, weight, K: int, bias, act: int, residual, out_dtype, keep_u: bool):
+    """``(out, u or None)`` for rows ``x`` and ``weight`` of ``K`` values from ``_rows``."""
 
     (x, x_ld), (weight, w_ld) = x, weight
-    (M, K), N, device = x.shape, weight.shape[0], x.device
+    M, N, device = x.shape[0], weight.shape[0], x.device
     out = torch.empty((M, N), dtype=out_dtype, device=device)
     u = torch.empty((M, N), dtype=x.dtype, device=device) if keep_u else None
     if M == 0:
@@ -73,9 +82,10 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, out_dtype):
         xr, wr = _rows(x), _rows(weight)
-        out, u = _launch(xr, wr, bias, act, residual, out_dtype, act != 0)
+        out, u = _launch(xr, wr, x.shape[1], bias, act, residual, out_dtype, act != 0)
+        # packed rows whole, their zeros too; the pitches are those of what a saved-tensor hook gives back
         ctx.save_for_backward(xr[0], wr[0], u)
-        ctx.act, ctx.pitch = act, (xr[1], wr[1])
+        ctx.act, ctx.dims = act, x.shape[1]
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.residual_dtype = None if residual is None else residual.dtype
         return out
@@ -85,7 +95,6 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, u = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        (M, K), N, dtype = x.shape, weight.shape[0], x.dtype
         dres = dy.to(ctx.residual_dtype) if nr else None
         if not (nx or nw or nb):
             return None, None, None, dres, None, None
@@ -95,14 +104,13 @@ class _Linear(torch.autograd.Function):
 
 
 def _backward(ctx, x, weight, u, dy, nx: bool, nw: bool, nb: bool):
-    (M, K), N, dtype, device = x.shape, weight.shape[0], x.dtype, x.device
+    M, K, N, dtype, device = x.shape[0], ctx.dims, weight.shape[0], x.dtype, x.device
     make = torch.empty if M else torch.zeros
     wide = dy.dtype != dtype
     if wide:  # a float32 output of 16-bit rows: its gradient keeps its bits and range, so the products are float32's
-        (x, x_ld), (weight, w_ld) = _rows(x.float()), _rows(weight.float())
-        u = None if u is None else u.float()
-    else:
-        x_ld, w_ld = ctx.pitch
+        x, weight, u = x.float(), weight.float(), None if u is None else u.float()
+    (x, x_ld), (weight, w_ld) = _rows(x), _rows(weight)
+    u = None if u is None else u.contiguous()
     dx = make((M, K), dtype=x.dtype, device=device) if nx else None
     dw = make((N, K), dtype=x.dtype, device=device) if nw else None
     db = make((N,), dtype=ctx.bias_dtype, device=device) if nb else None
@@ -164,7 +172,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         r = None if residual is None else (residual if flat else residual.reshape(-1, shape[-1])).contiguous()
         if not _grad.wanted(x, weight, bias, residual):
             lie = _few_rows if rows.shape[0] <= _FEW else _rows
-            out = _launch(lie(rows), lie(weight), b, act, r, od, False)[0]
+            out = _launch(lie(rows), lie(weight), weight.shape[1], b, act, r, od, False)[0]
         else:
             _grad.check_capture(x, weight, bias, residual)
             out = _grad.mark(_Linear.apply(rows, weight, b, r, act, od))

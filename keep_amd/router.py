@@ -142,7 +142,7 @@ class _RouteExperts(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dweight):
-        z, idx = ctx.saved_tensors
+        z, idx = _grad.saved(ctx)
         dz, dw = torch.empty_like(z), dweight.contiguous()
         if z.shape[0]:
             with _on(z.device):
