@@ -1131,7 +1131,7 @@ class RoutedVQMoE:
     that gave up (NaN output).
 
     ``glu`` may hold dense projections (``SwitchLinear``): the layer is then differentiable in ``x``, the experts'
-    weights, the shared expert's and ``residual`` (the router's outputs take no gradient). Codes have no gradient:
+    weights, the shared expert's and ``residual`` (the residency router's outputs take none). Codes have no gradient:
     beside them ``residual`` and a dense shared expert's weights get theirs while ``x`` requires none; where it does,
     the backward pass raises. ``adapter_indices`` (one per token, -1: none) adds the adapters of the projections that
     have some, the shared expert's too; with ``slot_map`` a routed expert's are its pool row's, as its weights.
@@ -1144,8 +1144,6 @@ class RoutedVQMoE:
                  shared_experts: QuantizedVQSwitchGLU | DenseGLU | None = None, slot_map: torch.Tensor | None = None,
                  one_launch: bool = False, gate: MoEGate | None = None):
         if gate is not None:
-            if slot_map is not None:
-                raise ValueError("a gate's experts are glu's own: it takes no slot_map")
             if gate.input_dims != glu.input_dims or gate.num_experts != glu.num_experts or gate.top_k != top_k:
                 raise ValueError(f"the gate must route {glu.input_dims} values to {top_k} of {glu.num_experts} experts")
         self.gate = gate
@@ -1166,6 +1164,25 @@ class RoutedVQMoE:
                 shared_experts.activation = LimitedSwiGLU(self.limit)
         self.shared_experts = shared_experts
         self.slot_map = slot_map
+        self._check_gate()
+
+    def _check_gate(self) -> None:
+        """Refuse settings of the layer's own router beside a gate, which routes by its own."""
+
+        g = self.gate
+        if g is None:
+            return
+        if self.slot_map is not None:
+            raise ValueError("a gate's experts are glu's own: it takes no slot_map")
+        if self.bias_served is not None or self.bias_demand is not None or self.tau != float("inf"):
+            raise ValueError("a gate serves every expert: a layer with one takes no bias_served, bias_demand or tau "
+                             "(MoEGate's bias balances its choice)")
+        for name, default in (("score_func", "softmax"), ("renormalize", True), ("route_scale", 1.0)):
+            value = getattr(self, name)
+            if value != default and value != getattr(g, name):
+                raise ValueError(f"the gate routes with {name} {getattr(g, name)!r}, the layer was given {value!r}")
+        if self.one_launch:
+            raise ValueError("the one-launch layer routes from logits: it takes no gate")
 
     def shared(self, x: torch.Tensor, adapter_indices=None) -> torch.Tensor:
         """The shared expert's output for every row of ``x``, float32 ``[T, H]``; ``adapter_indices``: with its
@@ -1229,8 +1246,10 @@ class RoutedVQMoE:
 
     def __call__(self, x: torch.Tensor, logits: torch.Tensor | None = None, *, residual: torch.Tensor | None = None,
                  adapter_indices=None):
-        if logits is None and self.gate is None:
-            raise ValueError("a layer without a gate needs logits")
+        if (logits is None) == (self.gate is None):
+            raise ValueError("a layer without a gate needs logits" if logits is None else
+                             "a layer with a gate forms its own logits")
+        self._check_gate()
         extra = self.shared_experts is not None or residual is not None
         od = torch.float32 if extra else self.out_dtype
         shared_adapters = None
