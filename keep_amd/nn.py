@@ -386,7 +386,8 @@ class DenseGLU:
     """A dense SwiGLU expert, ``down(act(up(x), gate(x)))``: a shared expert of plain ``[out, in]`` projections (the
     reference's are, ``deepseek_v4_flash_adapter.py:1777-1784``), without the routes of a one-expert
     ``QuantizedVQSwitchGLU``. The projections have no activation of their own; without ``activation`` the gate's silu is
-    formed in its product's epilogue."""
+    formed in its product's epilogue. silu(gate), up and their product are each rounded to the weights' dtype, as a
+    module of plain layers rounds them."""
 
     num_experts = 1
 
@@ -409,6 +410,11 @@ class DenseGLU:
         else:
             hidden = self.activation(up, g(x))
         return self.down_proj(hidden, residual=residual, out_dtype=out_dtype)
+
+    def recorded(self, x: torch.Tensor) -> bool:
+        """Whether autograd records a call on ``x``."""
+
+        return _grad.wanted(x, *(t for p in (self.gate_proj, self.up_proj, self.down_proj) for t in (p.weight, p.bias)))
 
 
 class MoEGate:
@@ -1117,10 +1123,11 @@ class RoutedVQMoE:
     the router's ``num_experts``; ``RouterOutput.idx`` then holds pool rows.
 
     ``shared_experts`` (a one-expert ``QuantizedVQSwitchGLU``, every token on
-    expert 0 with weight 1) adds the shared expert to the routed sum, and
-    ``__call__(..., residual=h)`` adds the residual stream, both in fp32 and
-    rounded once to ``out_dtype`` (``DeepseekV4FlashVQMoE.__call__``,
-    ``deepseek_v4_flash_adapter.py:1777-1784``; ``omlx_lattice.py:374-388``).
+    expert 0 with weight 1, or a ``DenseGLU``) adds the shared expert to the
+    routed sum, and ``__call__(..., residual=h)`` adds the residual stream, both
+    in fp32 and rounded once to ``out_dtype`` (``DeepseekV4FlashVQMoE.__call__``,
+    ``deepseek_v4_flash_adapter.py:1777-1784``; ``omlx_lattice.py:374-388``). A
+    ``DenseGLU`` gives its rows in its weights' dtype where autograd records it.
 
     One token runs the fused two-launch layer (``keep_moe_layer``, or
     ``keep_moe_layer_nested`` with a hot tier). ``one_launch=True`` runs it as
@@ -1190,7 +1197,9 @@ class RoutedVQMoE:
 
         se = self.shared_experts
         if isinstance(se, DenseGLU):
-            return se(x).float()
+            # float32 sums, as an expert on codes gives them. Where a graph is recorded its output is rounded to the weights'
+            # dtype first: a float32 output's gradient would be float32 products, at a tenth of the 16-bit rate
+            return se(x).float() if se.recorded(x) else se(x, out_dtype=torch.float32)
         T = x.shape[0]
         idx = torch.zeros((T, 1), dtype=torch.int32, device=x.device)
         w = torch.ones((T, 1), dtype=torch.float32, device=x.device)
