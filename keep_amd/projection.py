@@ -197,7 +197,7 @@ def linear_q8(x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, wei
                           ("weight_scales", weight_scales, ((N + SCALE_BLOCK - 1) // SCALE_BLOCK, blocks))):
         if tuple(t.shape) != want or t.dtype != torch.float32:
             raise ValueError(f"{name} must be float32 of shape {want}, found {tuple(t.shape)} in {t.dtype}")
-    if _grad.wanted(x_scales, weight_scales, bias, residual):
+    if _grad.wanted(x, x_scales, weight, weight_scales, bias, residual):
         raise ValueError("the 8-bit product has no gradients")
     with ops._on(device):
         flat = x.ndim == 2
