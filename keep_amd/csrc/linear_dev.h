@@ -174,7 +174,7 @@ struct LinearEpilogue {
   int udt;
   void* out;  // [M][N]
   int odt;
-  int vec;  // rows of whole 16-value pieces at aligned addresses
+  int vec;  // N is a multiple of eight and every pointer 16-byte aligned: pieces of up to eight values are read and stored whole
 
   // The values at (row, col ..): n of them are inside.
   template <int V>

@@ -21,33 +21,23 @@ _FEW = 16  # rows up to which the kernels read rows of any address and length
 _E4M3 = 3
 
 
-def _packed(t: torch.Tensor) -> torch.Tensor | None:
-    """``t [n, K]`` with its rows filled up with zeros to whole 16-byte pieces, or None where ``t`` lies as the kernels
-    read it: whole, aligned pieces a row."""
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t [n, K]`` as the kernels read it, whole 16-byte pieces a row, and the values between two rows. Where it lies
+    otherwise it is copied, its rows filled up with zeros to ``[n, ld]``."""
 
-    n, K = t.shape
-    piece = 16 // t.element_size()
-    if K % piece == 0 and t.data_ptr() % 16 == 0 and t.stride(1) == 1:
+    (n, K), (ld, one), size = t.shape, t.stride(), t.element_size()
+    if one == 1 and K * size % 16 == 0 and t.data_ptr() % 16 == 0:
         if n <= 1:
-            return None
-        ld = t.stride(0)
-        if ld >= K and ld % piece == 0 and ld <= 4 * MAX_DIMS:
-            return None
+            return t, K
+        if K <= ld <= 4 * MAX_DIMS and ld * size % 16 == 0:
+            return t, ld
+    piece = 16 // size
     ld = (K + piece - 1) // piece * piece
     out = torch.empty((n, ld), dtype=t.dtype, device=t.device)
     out[:, :K] = t
     if ld > K:
         out[:, K:].zero_()
-    return out
-
-
-def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """``t [n, K]`` as the kernels read it (``_packed``), and the values between two rows."""
-
-    out = _packed(t)
-    if out is not None:
-        return out, out.shape[1]
-    return t, t.shape[1] if t.shape[0] <= 1 else t.stride(0)
+    return out, ld
 
 
 def _few_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
