@@ -142,7 +142,8 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e
 
     Without ``residual`` ``h = x``, and ``y`` is returned. With it (``x``'s shape, in ``x``'s dtype or float32)
     ``h = residual + x`` rounded to its dtype, the new residual stream, and ``(y, h)`` are returned: the norm is of the
-    rounded stream. ``weight [n]`` of any float dtype. Differentiable in ``x``, ``residual`` and ``weight``; the gradients
+    rounded stream. ``weight [n]`` of any float dtype. The squares' sum is float32's: values beyond 1e19 overflow it, and
+    the row is 0. Differentiable in ``x``, ``residual`` and ``weight``; the gradients
     of ``x`` and a ``residual`` of its dtype are the same values, in one tensor."""
 
     device = _norm_args(x, weight, eps, residual)

@@ -12,8 +12,8 @@
 // still it is cut into slices too, whose float32 sums k_linear_join adds. Both in order.
 //
 // Bound by the matrix cores' power and by LDS: 8192 x 8192 x 8192 bf16 1372 TFLOP/s, 8192 x 4096 -> 8192 with silu 410 to 436 us
-// (1340 to 1260 TFLOP/s), during which the clock falls to about 1.85 GHz: a step's products take 2048 clocks of a SIMD, a step
-// 3077, and four buffers for two, which cut the waits, left the time as it was. 4096 x 4096 -> 2048 (256 tiles of 256 x 128, one
+// (1340 to 1260 TFLOP/s), during which the clock falls to about 1.8 GHz: a step's products take 2048 clocks of a SIMD, 62 % of
+// what a step takes, and four buffers for two, which cut the waits, left the time as it was. 4096 x 4096 -> 2048 (256 tiles of 256 x 128, one
 // a CU) 73 us with its epilogue, 65 for dx and 68 for dW: a step of this tile reads 128 KB of LDS and writes 48 for 1024 clocks
 // of products, and a tile's first copies and its stores are not overlapped. float32 (16x16x4 products) 142 TFLOP/s of 157.
 //

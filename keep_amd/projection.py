@@ -4,7 +4,7 @@
 ``linear_q8`` takes both in 8 bits (e4m3) with float32 scales, as ``rmsnorm_quant`` leaves its rows, for serving. Sums are
 float32 and rounded once. Up to 16 rows stream the weights, more run through LDS, in slices of the summed index where there
 are few tiles (``keep_linear``). Rows and weights may be views with a pitch; where more than 16 rows are no whole number of
-16-byte pieces, or start off one, they and the weights are copied first.
+16-byte pieces, or start off one, they and the weights are copied first, in every call.
 """
 
 from __future__ import annotations
@@ -146,7 +146,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     ``residual`` (of the output's shape) have ``x``'s dtype or float32; the output takes ``residual``'s without
     ``out_dtype``. Differentiable in ``x``, ``weight``, ``bias`` and ``residual``: the values before the activation are
     kept in ``x``'s dtype, and the gradient before the products is rounded to it; a float32 output of 16-bit rows has
-    its products formed in float32.
+    its products formed in float32, several times as long.
     """
 
     device = ops._dense_device(x, weight, bias, residual)
